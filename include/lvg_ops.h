@@ -44,8 +44,9 @@ extern "C" {
 
 #define LVG_ABI_VERSION 1
 
-/* element types of activations; filters are always float32 */
-enum { LVG_F32 = 0, LVG_F16 = 1, LVG_BF16 = 2, LVG_F64 = 3 };
+/* element types of activations; filters are always float32. LVG_E4M3 (8 bits, OCP e4m3: 1 sign, 4 exponent, 3 mantissa bits, no infinities)
+   is the type of 8-bit rows and weights of the token-row operators only. */
+enum { LVG_F32 = 0, LVG_F16 = 1, LVG_BF16 = 2, LVG_F64 = 3, LVG_E4M3 = 4 };
 
 /* activation ids: identical to `cuda_idx` of bias_act.activation_funcs (bias_act.py:21-31) */
 enum {
@@ -520,6 +521,72 @@ int lvg_pointwise_wgrad(const void* x, const void* dy, float* part, const void* 
  * channels a multiple of 8; pointers 16-byte aligned.
  */
 int lvg_split32_stack(const float* x, void* out, int64_t pixels, int channels, int64_t x_pixel_stride, int blocks, int pattern, void* stream);
+
+/* --------------------------------------------------------------------------------------------------------------------
+ * Operators on matrices of token rows (csrc/token_*.hip, csrc/rms_norm.hip): the dense layers, gated units and norms of
+ * row-wise networks. The reference runs its dense layers as torch.addmm / matmul + bias_act (model/generator_lres.py:60-80)
+ * and has no gated unit, residual norm or 8-bit rows. Sizes and row strides are in elements, rows are dense (unit element
+ * stride) and may start at any element; 16-byte aligned rows are faster. Sums are float32, in a fixed order.
+ */
+
+/*
+ * y [rows, outer] = clamp(act(x [rows, inner] . w [outer, inner]^T + b) * gain) + residual                     gated == 0
+ * y [rows, outer] = gain * act(x . w[:outer]^T + b[:outer]) * (x . w[outer:]^T + b[outer:]),  w [2 outer, inner]  gated == 1
+ * act / alpha / gain / clamp as in lvg_bias_act (clamp < 0: none; a NaN stays a NaN). b, residual and y have type out_dtype, which is dtype,
+ * or float16 / bfloat16 for LVG_E4M3 operands; those come with x_scale [rows] and w_scale [outer] (gated: [2 outer]) float32: the value of an
+ * element is itself times its row's scale. b, residual, slopes may be NULL.
+ * slopes receives what lvg_linear_slope multiplies gradients with: slope_kind 1: float32 [rows, outer] (gated [rows, 2 outer]: the derivatives
+ * with respect to the gate's and the up half's sums), 2: one byte an element (0: clamped, 1: alpha, 2: one; linear, relu and lrelu only), 0: none.
+ * work: lvg_linear_act_work(...) bytes, 16-byte aligned (0 bytes: NULL will do); nothing in it outlives the call.
+ */
+int64_t lvg_linear_act_work(int64_t rows, int64_t outer, int64_t inner, int dtype, int gated);
+int lvg_linear_act(const void* x, const void* w, const void* b, const void* residual, const float* x_scale, const float* w_scale,
+                   void* y, void* slopes, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
+                   int64_t x_stride, int64_t w_stride, int64_t residual_stride, int64_t y_stride,
+                   int dtype, int out_dtype, int gated, int act, int slope_kind, float alpha, float gain, float clamp, void* stream);
+
+/*
+ * dz [rows, halves * outer] = dy [rows, outer] * slopes * gain   (slope_kind 0: dy * gain; 2: alpha stands for code 1), and the column sums of
+ * dz by row ranges: db_part [slots, halves * outer] float32, slots = lvg_linear_slope_slots(...); lvg_column_sum adds them. dz may be NULL (sums
+ * alone) and so may db_part.
+ */
+int lvg_linear_slope_slots(int64_t rows, int64_t outer, int halves, int dtype);
+int lvg_linear_slope(const void* dy, const void* slopes, void* dz, float* db_part, int64_t rows, int64_t outer, int64_t dy_stride, int64_t dz_stride,
+                     int halves, int slope_kind, int slots, float alpha, float gain, int dtype, void* stream);
+
+/* out [width] (type dtype) = gain * sum over slots of part [slots, width] float32, in slot order within four interleaved runs. */
+int lvg_column_sum(const float* part, void* out, int slots, int64_t width, float gain, int dtype, void* stream);
+
+/*
+ * The two products of the backward pass; grad is dense.
+ *   weight == 0: grad [rows, inner]  = gain * dz [rows, outer] . other, other = w [outer, inner]
+ *   weight == 1: grad [outer, inner] = gain * dz^T . other,             other = x [rows, inner]
+ * work: lvg_linear_grad_work(...) bytes, 16-byte aligned.
+ */
+int64_t lvg_linear_grad_work(int64_t rows, int64_t outer, int64_t inner, int weight, int dtype);
+int lvg_linear_grad(const void* dz, const void* other, void* grad, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
+                    int64_t dz_stride, int64_t other_stride, int weight, float gain, int dtype, void* stream);
+
+/*
+ * s = x + residual;  y = weight * s / sqrt(mean(s^2) + eps)   over rows [rows, width], width >= 1. residual (and then sum = s rounded to dtype),
+ * weight, rstd [rows] (the reciprocal root) may be NULL. quantize == 0: y has type dtype; 1: y is e4m3 bytes and scale [rows] = max |y| / 448 of the
+ * row (2^-64 at least; a row with a NaN has a NaN scale), y = result / scale. y and sum are dense.
+ */
+int lvg_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* sum, float* rstd, float* scale,
+                 int64_t rows, int64_t width, int64_t x_stride, int64_t residual_stride, float eps, int dtype, int quantize, void* stream);
+
+/*
+ * Gradient of lvg_rms_norm: with g = weight * dy, dx = rstd g - s rstd^3 mean(g s) + dsum (dsum: gradient of sum's other uses, or NULL); dx is also
+ * the residual's gradient. dw_part [slots, width] float32 (or NULL), slots = lvg_rms_norm_backward_slots(...): the weight's gradient by row ranges,
+ * added by lvg_column_sum. row_work: [rows] floats, used for rows of more than 32 KiB (NULL otherwise will do). dx is dense.
+ */
+int lvg_rms_norm_backward_slots(int64_t rows, int64_t width, int dtype);
+int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* rstd, void* dx, float* dw_part,
+                          float* row_work, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
+                          int slots, int dtype, void* stream);
+
+/* q [rows, width] e4m3 = x / scale, scale [rows] = max |x| of the row / 448 (2^-64 at least). q is dense. */
+int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t width, int64_t x_stride, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,535 @@
+// rms_norm.hip -- root-mean-square norm of rows with the residual's addition, its gradient, and rows of 8-bit values with one scale each:
+//
+//   s = x + residual,   r = 1 / sqrt(mean(s^2) + eps),   y = weight * s * r
+//   q = y / scale in e4m3,   scale = max |y| of the row / 448               (quantize)
+//   ds_in = r g - s r^3 mean(g s) + ds,   g = weight * dy,   dweight = sum over rows of dy s r
+//
+// What a program otherwise spells as add, square, mean, rsqrt, two products, an absolute maximum and a cast: eight passes over the rows where
+// one has to read x and residual and write s and y. One row is held in the registers of one wave (up to 8 vectors a lane) or of a workgroup of
+// four, so each value is read once and written once; the sums are float32 and their order is fixed. Rows of more than 4 x 64 x 8 vectors take
+// two passes over the row, the second of which finds it in L2.
+#include "row_common.h"
+
+namespace {
+
+struct NormArgs
+{
+    const void*  x;
+    const void*  residual;     // or NULL
+    const void*  weight;       // [width] or NULL
+    void*        y;            // T, or e4m3 bytes
+    void*        sum;          // T: x + residual, or NULL
+    float*       rstd;         // [rows] or NULL
+    float*       scale;        // [rows], 8-bit results
+    int64_t      rows, width, ldx, ldr, ldy;
+    float        eps;
+};
+
+struct NormBackArgs
+{
+    const void*  dy;
+    const void*  ds;           // gradient of the sum's other uses, or NULL
+    const void*  s;
+    const void*  weight;
+    const float* rstd;
+    void*        dx;
+    float*       part;         // [slots][width] or NULL
+    float*       coef;         // [rows]: wide rows only
+    int64_t      rows, width, lddy, ldds, lds;
+};
+
+template <int W> __device__ __forceinline__ float row_total(float v, float* lds, int wave)
+{
+    v = wave_total(v);
+    if (W == 1) return v;
+    lds[wave] = v;
+    __syncthreads();
+    float t = 0.f;
+    #pragma unroll
+    for (int i = 0; i < W; i++) t += lds[i];
+    return t;
+}
+
+template <int W> __device__ __forceinline__ uint32_t row_largest(uint32_t v, uint32_t* lds, int wave)
+{
+    v = wave_largest(v);
+    if (W == 1) return v;
+    lds[wave] = v;
+    __syncthreads();
+    uint32_t t = 0;
+    #pragma unroll
+    for (int i = 0; i < W; i++) t = max(t, lds[i]);
+    return t;
+}
+
+// W waves a row (1: four rows a workgroup of 256), NV vectors a lane; NORM = false: quantisation alone.
+template <class T, int W, int NV, bool QUANT, bool NORM>
+__global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
+{
+    constexpr int V = Elem<T>::kVec;
+    __shared__ float sums[4];
+    __shared__ uint32_t tops[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+    if (W == 1 && row >= p.rows) return;
+    const int t = W == 1 ? lane : (int)threadIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+
+    float v[NV][V];
+    #pragma unroll
+    for (int j = 0; j < NV; j++)
+    {
+        const int64_t at = (int64_t)(j * 64 * W + t) * V;
+        load_row<T>(x + at, p.width - at, v[j]);
+    }
+    if (NORM)
+    {
+        if (p.residual)
+        {
+            const T* r = static_cast<const T*>(p.residual) + row * p.ldr;
+            #pragma unroll
+            for (int j = 0; j < NV; j++)
+            {
+                const int64_t at = (int64_t)(j * 64 * W + t) * V;
+                float o[V];
+                load_row<T>(r + at, p.width - at, o);
+                #pragma unroll
+                for (int i = 0; i < V; i++) v[j][i] += o[i];
+                if (p.sum) store_row<T>(static_cast<T*>(p.sum) + row * p.width + at, p.width - at, v[j]);
+            }
+        }
+        float ss = 0.f;
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+            #pragma unroll
+            for (int i = 0; i < V; i++) ss = fmaf(v[j][i], v[j][i], ss);
+        ss = row_total<W>(ss, sums, wave);
+        const float r = 1.f / sqrtf(ss / (float)p.width + p.eps);
+        if (p.rstd && t == 0) p.rstd[row] = r;
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+        {
+            const int64_t at = (int64_t)(j * 64 * W + t) * V;
+            float w[V];
+            if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w);
+            #pragma unroll
+            for (int i = 0; i < V; i++) v[j][i] = p.weight ? v[j][i] * r * w[i] : v[j][i] * r;
+        }
+    }
+    if (QUANT)
+    {
+        uint32_t top = 0;
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+        {
+            const int64_t left = p.width - (int64_t)(j * 64 * W + t) * V;
+            #pragma unroll
+            for (int i = 0; i < V; i++) if (i < left) top = max(top, magnitude(v[j][i]));
+        }
+        const float scale = row_scale(row_largest<W>(top, tops, wave)), inv = 1.f / scale;
+        if (t == 0) p.scale[row] = scale;
+        uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldy;
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+        {
+            const int64_t at = (int64_t)(j * 64 * W + t) * V, left = p.width - at;
+            uint32_t w[V / 4];
+            #pragma unroll
+            for (int i = 0; i < V; i += 4) w[i / 4] = pack_e4m3(v[j][i] * inv, v[j][i + 1] * inv, v[j][i + 2] * inv, v[j][i + 3] * inv);
+            if (left >= V) __builtin_memcpy(q + at, w, V);
+            else
+            {
+                #pragma unroll
+                for (int i = 0; i < V; i++) if (i < left) q[at + i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
+            }
+        }
+    }
+    else
+    {
+        T* y = static_cast<T*>(p.y) + row * p.ldy;
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+        {
+            const int64_t at = (int64_t)(j * 64 * W + t) * V;
+            store_row<T>(y + at, p.width - at, v[j]);
+        }
+    }
+}
+
+// Rows wider than a workgroup's registers: one workgroup a row, the row read again for every statistic.
+template <class T, bool QUANT, bool NORM>
+__global__ __launch_bounds__(256) void rms_norm_wide_kernel(NormArgs p)
+{
+    constexpr int V = Elem<T>::kVec;
+    __shared__ float sums[4];
+    __shared__ uint32_t tops[4];
+    const int wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* res = NORM && p.residual ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
+    auto value = [&](int64_t at, float* v)
+    {
+        load_row<T>(x + at, p.width - at, v);
+        if (res)
+        {
+            float o[V];
+            load_row<T>(res + at, p.width - at, o);
+            #pragma unroll
+            for (int i = 0; i < V; i++) v[i] += o[i];
+        }
+    };
+    float r = 1.f;
+    if (NORM)
+    {
+        float ss = 0.f;
+        for (int64_t at = (int64_t)threadIdx.x * V; at < p.width; at += 256 * V)
+        {
+            float v[V];
+            value(at, v);
+            #pragma unroll
+            for (int i = 0; i < V; i++) ss = fmaf(v[i], v[i], ss);
+            if (res && p.sum) store_row<T>(static_cast<T*>(p.sum) + row * p.width + at, p.width - at, v);
+        }
+        ss = row_total<4>(ss, sums, wave);
+        r = 1.f / sqrtf(ss / (float)p.width + p.eps);
+        if (p.rstd && threadIdx.x == 0) p.rstd[row] = r;
+    }
+    auto result = [&](int64_t at, float* v)
+    {
+        value(at, v);
+        if (!NORM) return;
+        float w[V];
+        if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w);
+        #pragma unroll
+        for (int i = 0; i < V; i++) v[i] = p.weight ? v[i] * r * w[i] : v[i] * r;
+    };
+    float inv = 1.f;
+    if (QUANT)
+    {
+        uint32_t top = 0;
+        for (int64_t at = (int64_t)threadIdx.x * V; at < p.width; at += 256 * V)
+        {
+            float v[V];
+            result(at, v);
+            #pragma unroll
+            for (int i = 0; i < V; i++) if (at + i < p.width) top = max(top, magnitude(v[i]));
+        }
+        const float scale = row_scale(row_largest<4>(top, tops, wave));
+        if (threadIdx.x == 0) p.scale[row] = scale;
+        inv = 1.f / scale;
+    }
+    for (int64_t at = (int64_t)threadIdx.x * V; at < p.width; at += 256 * V)
+    {
+        float v[V];
+        result(at, v);
+        if (QUANT)
+        {
+            uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldy + at;
+            #pragma unroll
+            for (int i = 0; i < V; i += 4)
+            {
+                const uint32_t w = pack_e4m3(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+                #pragma unroll
+                for (int k = 0; k < 4; k++) if (at + i + k < p.width) q[i + k] = (uint8_t)(w >> (8 * k));
+            }
+        }
+        else store_row<T>(static_cast<T*>(p.y) + row * p.ldy + at, p.width - at, v);
+    }
+}
+
+// Gradient: a workgroup takes rows blockIdx.x, + gridDim.x, ... (W == 1: its four waves a row each) and keeps the weight's gradient of its
+// rows in registers; the four waves' sums meet in LDS in wave order and go to part[blockIdx.x][width].
+template <class T, int W, int NV>
+__global__ __launch_bounds__(256) void rms_norm_back_kernel(NormBackArgs p)
+{
+    constexpr int V = Elem<T>::kVec;
+    __shared__ float sums[2][4];
+    __shared__ float cols[W == 1 ? 64 * V : 1];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int t = W == 1 ? lane : (int)threadIdx.x;
+    float dw[NV][V];
+    #pragma unroll
+    for (int j = 0; j < NV; j++)
+        #pragma unroll
+        for (int i = 0; i < V; i++) dw[j][i] = 0.f;
+    const int64_t step = (int64_t)gridDim.x * (W == 1 ? 4 : 1);
+    int turn = 0;
+    for (int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x; row < p.rows; row += step, turn ^= 1)
+    {
+        const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
+        const T* s = static_cast<const T*>(p.s) + row * p.lds;
+        const float r = p.rstd[row];
+        float g[NV][V], sv[NV][V];
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+        {
+            const int64_t at = (int64_t)(j * 64 * W + t) * V;
+            load_row<T>(dy + at, p.width - at, g[j]);
+            load_row<T>(s + at, p.width - at, sv[j]);
+        }
+        float dot = 0.f;
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+        {
+            const int64_t at = (int64_t)(j * 64 * W + t) * V;
+            float w[V];
+            if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w);
+            #pragma unroll
+            for (int i = 0; i < V; i++)
+            {
+                dw[j][i] = fmaf(g[j][i], sv[j][i] * r, dw[j][i]);
+                if (p.weight) g[j][i] *= w[i];
+                dot = fmaf(g[j][i], sv[j][i], dot);
+            }
+        }
+        dot = row_total<W>(dot, sums[turn], wave);         // (two sets: a wave may reach the next row's while another still reads this one's)
+        const float c = r * r * r * (dot / (float)p.width);
+        #pragma unroll
+        for (int j = 0; j < NV; j++)
+        {
+            const int64_t at = (int64_t)(j * 64 * W + t) * V;
+            float d[V];
+            if (p.ds) load_row<T>(static_cast<const T*>(p.ds) + row * p.ldds + at, p.width - at, d);
+            #pragma unroll
+            for (int i = 0; i < V; i++) g[j][i] = fmaf(g[j][i], r, -c * sv[j][i]) + (p.ds ? d[i] : 0.f);
+            store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, p.width - at, g[j]);
+        }
+    }
+    if (!p.part) return;
+    float* out = p.part + (int64_t)blockIdx.x * p.width;
+    #pragma unroll
+    for (int j = 0; j < NV; j++)
+    {
+        const int64_t at = (int64_t)(j * 64 * W + t) * V;
+        if (W == 1)
+        {
+            for (int k = 0; k < 4; k++)         // the waves add in turn
+            {
+                if (wave == k)
+                {
+                    #pragma unroll
+                    for (int i = 0; i < V; i++) cols[lane * V + i] = k == 0 ? dw[j][i] : cols[lane * V + i] + dw[j][i];
+                }
+                __syncthreads();
+            }
+            for (int i = threadIdx.x; i < 64 * V; i += 256)
+                if ((int64_t)j * 64 * V + i < p.width) out[(int64_t)j * 64 * V + i] = cols[i];
+            __syncthreads();
+        }
+        else
+        {
+            #pragma unroll
+            for (int i = 0; i < V; i++) if (at + i < p.width) out[at + i] = dw[j][i];
+        }
+    }
+}
+
+// Wide rows: the row's coefficient first, then columns.
+template <class T>
+__global__ __launch_bounds__(256) void rms_norm_back_coef_kernel(NormBackArgs p)
+{
+    constexpr int V = Elem<T>::kVec;
+    __shared__ float sums[4];
+    const int64_t row = blockIdx.x;
+    const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
+    const T* s = static_cast<const T*>(p.s) + row * p.lds;
+    float dot = 0.f;
+    for (int64_t at = (int64_t)threadIdx.x * V; at < p.width; at += 256 * V)
+    {
+        float g[V], sv[V], w[V];
+        load_row<T>(dy + at, p.width - at, g);
+        load_row<T>(s + at, p.width - at, sv);
+        if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w);
+        #pragma unroll
+        for (int i = 0; i < V; i++) dot = fmaf(p.weight ? g[i] * w[i] : g[i], sv[i], dot);
+    }
+    dot = row_total<4>(dot, sums, threadIdx.x >> 6);
+    const float r = p.rstd[row];
+    if (threadIdx.x == 0) p.coef[row] = r * r * r * (dot / (float)p.width);
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void rms_norm_back_wide_kernel(NormBackArgs p)
+{
+    constexpr int V = Elem<T>::kVec;
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, left = p.width - at;
+    if (left <= 0) return;
+    float dw[V], w[V];
+    #pragma unroll
+    for (int i = 0; i < V; i++) { dw[i] = 0.f; w[i] = 1.f; }
+    if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, left, w);
+    for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y)
+    {
+        float g[V], sv[V], d[V];
+        load_row<T>(static_cast<const T*>(p.dy) + row * p.lddy + at, left, g);
+        load_row<T>(static_cast<const T*>(p.s) + row * p.lds + at, left, sv);
+        if (p.ds) load_row<T>(static_cast<const T*>(p.ds) + row * p.ldds + at, left, d);
+        const float r = p.rstd[row], c = p.coef[row];
+        #pragma unroll
+        for (int i = 0; i < V; i++)
+        {
+            dw[i] = fmaf(g[i], sv[i] * r, dw[i]);
+            g[i] = fmaf(g[i] * w[i], r, -c * sv[i]) + (p.ds ? d[i] : 0.f);
+        }
+        store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, left, g);
+    }
+    if (p.part)
+    {
+        #pragma unroll
+        for (int i = 0; i < V; i++) if (i < left) p.part[(int64_t)blockIdx.y * p.width + at + i] = dw[i];
+    }
+}
+
+// out[c] = sum over the slots of part[slot][c]: 64 columns a workgroup, its 4 waves take every fourth slot and add in wave order.
+template <class T>
+__global__ __launch_bounds__(256) void column_sum_kernel(const float* part, T* out, int slots, int64_t width, float gain)
+{
+    __shared__ float sums[4][64];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    float v = 0.f;
+    if (c < width)
+    {
+        #pragma unroll 4
+        for (int s = wave; s < slots; s += 4) v += part[(int64_t)s * width + c];
+    }
+    sums[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && c < width) out[c] = from_acc<T>((((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]) * gain);
+}
+
+int esize(int dtype) { return dtype == LVG_F32 ? 4 : 2; }
+bool row_type(int dtype) { return dtype == LVG_F32 || dtype == LVG_F16 || dtype == LVG_BF16; }
+
+// Waves a row and vectors a lane: one wave as long as a lane holds the row in 8 vectors, then a workgroup of four.
+struct Plan { int waves, vecs; };
+Plan plan(int64_t width, int dtype)
+{
+    const int64_t vecs = lvg_ceil_div(width, 16 / esize(dtype));
+    for (int nv : {1, 2, 4, 8}) if (vecs <= 64 * nv) return {1, nv};
+    for (int nv : {4, 8}) if (vecs <= 256 * nv) return {4, nv};
+    return {0, 0};
+}
+
+// Rows of one launch: a grid holds fewer than 2^32 threads.
+constexpr int64_t kLaunchRows = (int64_t)1 << 23;
+
+template <class T, bool QUANT, bool NORM> void launch_norm_rows(const NormArgs& a, const Plan& k, hipStream_t s)
+{
+    const dim3 block(256), grid((unsigned)(k.waves == 1 ? lvg_ceil_div(a.rows, 4) : a.rows));
+    #define LVG_ROW(W, NV) if (k.waves == W && k.vecs == NV) { hipLaunchKernelGGL((rms_norm_kernel<T, W, NV, QUANT, NORM>), grid, block, 0, s, a); return; }
+    LVG_ROW(1, 1) LVG_ROW(1, 2) LVG_ROW(1, 4) LVG_ROW(1, 8) LVG_ROW(4, 4) LVG_ROW(4, 8)
+    #undef LVG_ROW
+    hipLaunchKernelGGL((rms_norm_wide_kernel<T, QUANT, NORM>), grid, block, 0, s, a);
+}
+
+template <class T, bool QUANT, bool NORM> void launch_norm(const NormArgs& a, const Plan& k, hipStream_t s)
+{
+    for (int64_t r = 0; r < a.rows; r += kLaunchRows)
+    {
+        NormArgs b = a;
+        b.rows = std::min(kLaunchRows, a.rows - r);
+        b.x = static_cast<const T*>(a.x) + r * a.ldx;
+        if (a.residual) b.residual = static_cast<const T*>(a.residual) + r * a.ldr;
+        b.y = static_cast<char*>(a.y) + r * a.ldy * (QUANT ? 1 : (int64_t)sizeof(T));
+        if (a.sum) b.sum = static_cast<T*>(a.sum) + r * a.width;
+        if (a.rstd) b.rstd = a.rstd + r;
+        if (a.scale) b.scale = a.scale + r;
+        launch_norm_rows<T, QUANT, NORM>(b, k, s);
+    }
+}
+
+template <class T> void launch_back(const NormBackArgs& a, const Plan& k, int slots, hipStream_t s)
+{
+    const dim3 block(256), grid((unsigned)slots);
+    #define LVG_ROW(W, NV) if (k.waves == W && k.vecs == NV) { hipLaunchKernelGGL((rms_norm_back_kernel<T, W, NV>), grid, block, 0, s, a); return; }
+    LVG_ROW(1, 1) LVG_ROW(1, 2) LVG_ROW(1, 4) LVG_ROW(1, 8) LVG_ROW(4, 4) LVG_ROW(4, 8)
+    #undef LVG_ROW
+    hipLaunchKernelGGL(rms_norm_back_coef_kernel<T>, dim3((unsigned)a.rows), block, 0, s, a);
+    hipLaunchKernelGGL(rms_norm_back_wide_kernel<T>, dim3((unsigned)lvg_ceil_div(a.width, 256 * Elem<T>::kVec), (unsigned)slots), block, 0, s, a);
+}
+
+bool rows_ok(int64_t rows, int64_t width) { return rows >= 0 && rows <= 0x7fffffff && width >= 1 && width <= ((int64_t)1 << 40); }
+
+int back_slots(int64_t rows, int64_t width, int dtype)
+{
+    const Plan k = plan(width, dtype);
+    // about two workgroups for each of the 256 compute units
+    if (k.waves == 1) return (int)std::min<int64_t>(512, lvg_ceil_div(rows, 4));
+    if (k.waves == 4) return (int)std::min<int64_t>(512, rows);
+    return (int)std::min<int64_t>(64, rows);
+}
+
+} // namespace
+
+extern "C" int lvg_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* sum, float* rstd, float* scale,
+                            int64_t rows, int64_t width, int64_t x_stride, int64_t residual_stride, float eps, int dtype, int quantize, void* stream)
+{
+    LVG_REQUIRE(row_type(dtype), "lvg_rms_norm: float32 / float16 / bfloat16 only (dtype %d)", dtype);
+    LVG_REQUIRE(rows_ok(rows, width), "lvg_rms_norm: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
+    if (rows == 0) return LVG_OK;
+    LVG_REQUIRE(x && y && (!quantize || scale) && (!sum || residual), "lvg_rms_norm: missing pointer");
+    LVG_REQUIRE(x_stride >= 0 && residual_stride >= 0, "lvg_rms_norm: negative row stride");
+    LVG_REQUIRE(eps >= 0.f, "lvg_rms_norm: eps must not be negative");
+    NormArgs a = {x, residual, weight, y, sum, rstd, scale, rows, width, x_stride, residual_stride, width, eps};
+    const Plan k = plan(width, dtype);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    #define LVG_TYPE(T) { if (quantize) launch_norm<T, true, true>(a, k, s); else launch_norm<T, false, true>(a, k, s); }
+    if (dtype == LVG_F32) LVG_TYPE(float) else if (dtype == LVG_F16) LVG_TYPE(f16_t) else LVG_TYPE(bf16_t)
+    #undef LVG_TYPE
+    return lvg_check_launch("lvg_rms_norm");
+}
+
+extern "C" int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t width, int64_t x_stride, int dtype, void* stream)
+{
+    LVG_REQUIRE(row_type(dtype), "lvg_quantize_rows: float32 / float16 / bfloat16 only (dtype %d)", dtype);
+    LVG_REQUIRE(rows_ok(rows, width), "lvg_quantize_rows: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
+    if (rows == 0) return LVG_OK;
+    LVG_REQUIRE(x && q && scale && x_stride >= 0, "lvg_quantize_rows: missing pointer or negative row stride");
+    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f};
+    const Plan k = plan(width, dtype);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == LVG_F32) launch_norm<float, true, false>(a, k, s);
+    else if (dtype == LVG_F16) launch_norm<f16_t, true, false>(a, k, s);
+    else launch_norm<bf16_t, true, false>(a, k, s);
+    return lvg_check_launch("lvg_quantize_rows");
+}
+
+extern "C" int lvg_rms_norm_backward_slots(int64_t rows, int64_t width, int dtype)
+{
+    return row_type(dtype) && rows_ok(rows, width) && rows > 0 ? back_slots(rows, width, dtype) : 0;
+}
+
+extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s_in, const void* weight, const float* rstd, void* dx, float* dw_part,
+                                     float* row_work, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
+                                     int slots, int dtype, void* stream)
+{
+    LVG_REQUIRE(row_type(dtype), "lvg_rms_norm_backward: float32 / float16 / bfloat16 only (dtype %d)", dtype);
+    LVG_REQUIRE(rows_ok(rows, width), "lvg_rms_norm_backward: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
+    if (rows == 0) return LVG_OK;
+    const Plan k = plan(width, dtype);
+    LVG_REQUIRE(dy && s_in && rstd && dx && (k.waves || row_work), "lvg_rms_norm_backward: missing pointer");
+    LVG_REQUIRE(k.waves || rows <= kLaunchRows, "lvg_rms_norm_backward: more than %lld rows of %lld values", (long long)kLaunchRows, (long long)width);
+    LVG_REQUIRE(dy_stride >= 0 && dsum_stride >= 0 && s_stride >= 0, "lvg_rms_norm_backward: negative row stride");
+    LVG_REQUIRE(slots == back_slots(rows, width, dtype), "lvg_rms_norm_backward: slots must be lvg_rms_norm_backward_slots(...) (= %d)", back_slots(rows, width, dtype));
+    NormBackArgs a = {dy, dsum, s_in, weight, rstd, dx, dw_part, row_work, rows, width, dy_stride, dsum_stride, s_stride};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == LVG_F32) launch_back<float>(a, k, slots, s);
+    else if (dtype == LVG_F16) launch_back<f16_t>(a, k, slots, s);
+    else launch_back<bf16_t>(a, k, slots, s);
+    return lvg_check_launch("lvg_rms_norm_backward");
+}
+
+extern "C" int lvg_column_sum(const float* part, void* out, int slots, int64_t width, float gain, int dtype, void* stream)
+{
+    LVG_REQUIRE(row_type(dtype), "lvg_column_sum: float32 / float16 / bfloat16 only (dtype %d)", dtype);
+    LVG_REQUIRE(slots >= 0 && width >= 0 && width <= ((int64_t)1 << 36), "lvg_column_sum: bad size");
+    if (width == 0) return LVG_OK;
+    LVG_REQUIRE((part || slots == 0) && out, "lvg_column_sum: missing pointer");
+    const dim3 grid((unsigned)lvg_ceil_div(width, 64)), block(256);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == LVG_F32) hipLaunchKernelGGL(column_sum_kernel<float>, grid, block, 0, s, part, static_cast<float*>(out), slots, width, gain);
+    else if (dtype == LVG_F16) hipLaunchKernelGGL(column_sum_kernel<f16_t>, grid, block, 0, s, part, static_cast<f16_t*>(out), slots, width, gain);
+    else hipLaunchKernelGGL(column_sum_kernel<bf16_t>, grid, block, 0, s, part, static_cast<bf16_t*>(out), slots, width, gain);
+    return lvg_check_launch("lvg_column_sum");
+}

@@ -1,0 +1,82 @@
+// row_common.h -- pieces shared by the kernels on matrices of rows (rms_norm.hip, token_*.hip): masked vector access to rows that may start at
+// any element, e4m3 conversion, the activations in float32 with their derivatives.
+#pragma once
+#include "lvg_common.h"
+#include <algorithm>
+#include <string.h>
+
+namespace {
+
+constexpr float kE4m3Max = 448.f;
+constexpr float kScaleMin = 5.421010862427522e-20f;     // 2^-64: the scale of a row of zeros; its reciprocal is still finite
+
+__device__ __forceinline__ float row_load(float v)  { return v; }
+__device__ __forceinline__ float row_load(f16_t v)  { return to_acc(v); }
+__device__ __forceinline__ float row_load(bf16_t v) { return to_acc(v); }
+
+// n of the V elements at p (the others zero). A row starts wherever its stride puts it, so the full access is an unaligned 16-byte one, which
+// the global memory path takes; only the last vector of a row goes element by element.
+template <class T> __device__ __forceinline__ void load_row(const T* p, int64_t n, float* v)
+{
+    constexpr int V = Elem<T>::kVec;
+    if (n >= V)
+    {
+        T r[V];
+        __builtin_memcpy(r, p, 16);
+        #pragma unroll
+        for (int i = 0; i < V; i++) v[i] = row_load(r[i]);
+    }
+    else
+    {
+        #pragma unroll
+        for (int i = 0; i < V; i++) v[i] = i < n ? row_load(p[i]) : 0.f;
+    }
+}
+
+template <class T> __device__ __forceinline__ void store_row(T* p, int64_t n, const float* v)
+{
+    constexpr int V = Elem<T>::kVec;
+    T r[V];
+    #pragma unroll
+    for (int i = 0; i < V; i++) r[i] = from_acc<T>(v[i]);
+    if (n >= V) __builtin_memcpy(p, r, 16);
+    else
+    {
+        #pragma unroll
+        for (int i = 0; i < V; i++) if (i < n) p[i] = r[i];
+    }
+}
+
+// Four values to e4m3 (round to nearest even), clamped to the finite range; a NaN stays one.
+__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d)
+{
+    auto bound = [](float v) { return v != v ? v : fminf(fmaxf(v, -kE4m3Max), kE4m3Max); };
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(bound(a), bound(b), 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(bound(c), bound(d), w, true);
+    return (uint32_t)w;
+}
+
+__device__ __forceinline__ float wave_total(float v)
+{
+    #pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// Largest magnitude as bits: integers order like the floats they are, with infinity above every number and NaN above infinity, so a NaN is kept.
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t wave_largest(uint32_t v)
+{
+    #pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+// scale = largest / 448, at least 2^-64 (a NaN stays one).
+__device__ __forceinline__ float row_scale(uint32_t largest)
+{
+    const float s = __uint_as_float(largest) / kE4m3Max;
+    return s < kScaleMin ? kScaleMin : s;
+}
+
+} // namespace

@@ -1,0 +1,324 @@
+// token_finish.hip -- the products of token rows as entry points: how a product is laid out over the chip, the pass that adds the parts of a
+// split product, and the element-wise step between a result's gradient and the two products of the backward pass:
+//
+//   dz[m][n] = dy[m][n] * slope[m][n] * gain,   db[n] = sum over rows of dz
+//
+// (gated: dy meets both slopes, dz has the gate's columns and then the up half's). One pass: dy and the slopes are read once, dz is written once
+// for both products, the column sums stay in registers until a workgroup's rows are done.
+#include "token_gemm.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Adding the parts of a split product, in their order.
+
+template <class O, bool GATED>
+__global__ __launch_bounds__(256) void token_finish_kernel(const float* part, int splits, int64_t ldpart, Finish f)
+{
+    const int64_t quads = (f.cols + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= f.rows * quads) return;
+    const int64_t m = i / quads, n = (i - m * quads) * 4;
+    const float* at = part + m * ldpart + n;
+    const int64_t step = f.rows * ldpart;
+    float v[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+    #pragma unroll 4
+    for (int s = 0; s < splits; s++, at += step)
+    {
+        const float4 a = *reinterpret_cast<const float4*>(at);
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        if (GATED)
+        {
+            const float4 b = *reinterpret_cast<const float4*>(at + ldpart / 2);
+            u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
+        }
+    }
+    finish4<O, GATED>(f, m, n, v, u);
+}
+
+int launch_finish(const TokenArgs& a, int out_dtype, bool gated, hipStream_t s)
+{
+    const int64_t threads = a.fin.rows * ((a.fin.cols + 3) / 4);
+    const dim3 grid((unsigned)lvg_ceil_div(threads, 256)), block(256);
+    #define LVG_FINISH(O) { \
+        if (gated) hipLaunchKernelGGL((token_finish_kernel<O, true>), grid, block, 0, s, a.part, a.splits, a.ldpart, a.fin); \
+        else       hipLaunchKernelGGL((token_finish_kernel<O, false>), grid, block, 0, s, a.part, a.splits, a.ldpart, a.fin); }
+    if (out_dtype == LVG_F32) LVG_FINISH(float) else if (out_dtype == LVG_F16) LVG_FINISH(f16_t) else LVG_FINISH(bf16_t)
+    #undef LVG_FINISH
+    return lvg_check_launch("token product, adding its parts");
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// dy, slopes -> dz and column sums.
+
+struct SlopeArgs
+{
+    const void* dy;
+    const void* slopes;        // [rows][halves * cols], or NULL
+    void*       dz;            // or NULL: column sums alone
+    float*      part;          // [gridDim.y][halves * cols], or NULL
+    int64_t     rows, cols, lddy, lddz;
+    int         halves, kind;
+    int         lanes;         // threads of a workgroup along the columns, a power of two
+    float       alpha, gain;
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
+{
+    constexpr int V = Elem<T>::kVec;
+    __shared__ float sums[256][V + 1];
+    const int tid = threadIdx.x, cl = tid & (p.lanes - 1), rl = tid / p.lanes, rstep = 256 / p.lanes;
+    const int64_t per = (p.cols + V - 1) / V;                          // vectors of one half
+    const int64_t vi = (int64_t)blockIdx.x * p.lanes + cl;
+    const int half = vi >= per ? 1 : 0;
+    const int64_t n = (vi - half * per) * V, left = vi < per * p.halves ? p.cols - n : 0;
+    const int64_t chunk = (p.rows + gridDim.y - 1) / gridDim.y;
+    const int64_t r0 = chunk * blockIdx.y, r1 = min(r0 + chunk, p.rows);
+    float db[V];
+    #pragma unroll
+    for (int i = 0; i < V; i++) db[i] = 0.f;
+    if (left > 0)
+    {
+        for (int64_t m = r0 + rl; m < r1; m += rstep)
+        {
+            float g[V];
+            load_row<T>(static_cast<const T*>(p.dy) + m * p.lddy + n, left, g);
+            const int64_t at = (m * p.halves + half) * p.cols + n;
+            if (p.kind == LVG_SLOPE_F32)
+            {
+                const float* s = static_cast<const float*>(p.slopes) + at;
+                #pragma unroll
+                for (int k = 0; k < V; k += 4)
+                {
+                    float d[4];
+                    load_row<float>(s + k, left - k, d);
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) g[k + i] *= d[i];
+                }
+            }
+            else if (p.kind == LVG_SLOPE_CODE)
+            {
+                const uint8_t* s = static_cast<const uint8_t*>(p.slopes) + at;
+                uint8_t c[V];
+                if (left >= V) __builtin_memcpy(c, s, V);
+                else
+                {
+                    #pragma unroll
+                    for (int i = 0; i < V; i++) c[i] = i < left ? s[i] : (uint8_t)0;
+                }
+                #pragma unroll
+                for (int i = 0; i < V; i++) g[i] = c[i] == 2 ? g[i] : c[i] == 1 ? g[i] * p.alpha : 0.f;
+            }
+            #pragma unroll
+            for (int i = 0; i < V; i++) { g[i] *= p.gain; db[i] += g[i]; }
+            if (p.dz) store_row<T>(static_cast<T*>(p.dz) + m * p.lddz + half * p.cols + n, left, g);
+        }
+    }
+    if (!p.part) return;
+    #pragma unroll
+    for (int i = 0; i < V; i++) sums[tid][i] = db[i];
+    __syncthreads();
+    if (rl == 0 && left > 0)
+    {
+        for (int k = 1; k < rstep; k++)
+        {
+            #pragma unroll
+            for (int i = 0; i < V; i++) db[i] += sums[k * p.lanes + cl][i];
+        }
+        float* out = p.part + (int64_t)blockIdx.y * p.halves * p.cols + half * p.cols + n;
+        #pragma unroll
+        for (int i = 0; i < V; i++) if (i < left) out[i] = db[i];
+    }
+}
+
+int slope_lanes(int64_t cols, int halves, int esize)
+{
+    const int64_t vecs = lvg_ceil_div(cols, 16 / esize) * halves;
+    int lanes = 1;
+    while (lanes < 256 && lanes < vecs) lanes *= 2;
+    return lanes;
+}
+
+// Row chunks: about eight workgroups for each compute unit, at least four rows a thread.
+int slope_slots(int64_t rows, int64_t cols, int halves, int esize)
+{
+    const int lanes = slope_lanes(cols, halves, esize);
+    const int64_t across = lvg_ceil_div(lvg_ceil_div(cols, 16 / esize) * halves, lanes);
+    const int64_t most = lvg_ceil_div(rows, 4 * (256 / lanes));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(most, std::max<int64_t>(1, 2048 / across)));
+}
+
+int esize_of(int dtype) { return dtype == LVG_F32 ? 4 : dtype == LVG_E4M3 ? 1 : 2; }
+bool float_type(int dtype) { return dtype == LVG_F32 || dtype == LVG_F16 || dtype == LVG_BF16; }
+bool size_ok(int64_t v) { return v >= 0 && v <= (int64_t)0x7fffffff; }
+
+int64_t part_pitch(int64_t cols, bool gated) { return (cols + 3) / 4 * 4 * (gated ? 2 : 1); }
+
+int64_t work_bytes(int64_t rows, int64_t cols, int64_t inner, int dtype, bool gated)
+{
+    const TokenPlan k = token_plan(rows, cols, inner, esize_of(dtype), gated);
+    return k.splits > 1 ? (int64_t)k.splits * rows * part_pitch(cols, gated) * 4 : 0;
+}
+
+// Operands that can travel to LDS without registers: 16-byte aligned rows, offsets inside a tile below 2^32, whole chunks of columns.
+bool direct_ok(const void* base, int64_t ld, int64_t count, int layout, int es, bool gated)
+{
+    if (!lvg_aligned16(base) || ld % 16 != 0) return false;
+    if (layout == ALONG) return 256 * ld + (gated ? count * ld : 0) < ((int64_t)1 << 32);
+    return (128 / es) * ld + 1024 < ((int64_t)1 << 32) && (count * es) % 16 == 0 && count * es >= 16;
+}
+
+// The product itself: rows x cols results over `inner`, args with operands and finish filled in.
+int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, int64_t work_size, hipStream_t s, const char* what)
+{
+    const int es = esize_of(dtype);
+    const bool gated = form == LVG_TOKEN_GATED;
+    const int64_t rows = a.qRows, cols = a.pRows;
+    const TokenPlan k = token_plan(rows, cols, a.inner, es, gated);
+    const int bm = k.tile == LVG_TILE_256 ? 256 : k.tile == LVG_TILE_128 ? 128 : 64, bn = (k.tile == LVG_TILE_256 ? 256 : 128) / (gated ? 2 : 1);
+    a.steps = lvg_ceil_div(a.inner * es, 128);
+    a.stepsPerSplit = lvg_ceil_div(a.steps, k.splits);
+    a.splits = k.splits;
+    a.tilesM = (int)lvg_ceil_div(rows, bm);
+    a.tilesN = lvg_ceil_div(cols, bn);
+    a.tiles = (int64_t)a.tilesM * a.tilesN;
+    a.part = nullptr;
+    a.ldpart = part_pitch(cols, gated);
+    if (k.splits > 1)
+    {
+        LVG_REQUIRE(work && lvg_aligned16(work) && work_size >= work_bytes(rows, cols, a.inner, dtype, gated), "%s: the workspace must be 16-byte aligned and hold %lld bytes",
+                    what, (long long)work_bytes(rows, cols, a.inner, dtype, gated));
+        a.part = static_cast<float*>(work);
+    }
+    const int pl = form == LVG_TOKEN_ROW_GRAD || form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG, ql = form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG;
+    const bool direct = direct_ok(a.p, a.ldp, cols, pl, es, gated) && direct_ok(a.q, a.ldq, rows, ql, es, false);
+    Finish& f = a.fin;
+    const int os = esize_of(out_dtype);
+    auto whole = [&](const void* p, int64_t ld) { return !p || (((uintptr_t)p) % (4 * os) == 0 && ld % 4 == 0); };
+    f.vec = cols % 4 == 0 && whole(f.bias, 0) && whole(f.residual, f.ldr) && whole(f.out, f.ldo) && (!f.slopes || lvg_aligned16(f.slopes));
+    int rc;
+    if (dtype == LVG_E4M3)      rc = token_launch_8bit(form, k.tile, direct, out_dtype, a, s);
+    else if (dtype == LVG_F32)  rc = token_launch_f32(form, k.tile, direct, a, s);
+    else if (dtype == LVG_F16)  rc = token_launch_f16(form, k.tile, direct, a, s);
+    else                        rc = token_launch_bf16(form, k.tile, direct, a, s);
+    if (rc != LVG_OK || k.splits <= 1) return rc;
+    return launch_finish(a, out_dtype, gated, s);
+}
+
+} // namespace
+
+// Layout of a product over the 256 compute units. A tile's step costs its matrix instructions (in cycles, with what the K loop reaches of the
+// peak) and at least the latency of the operands' way to LDS; a compute unit holds 1 / 2 / 3 workgroups of the 256 / 128 / 64-row tiles. Splitting
+// the summed index fills the chip when there are few tiles, and costs the float32 parts' way to memory and back and one more launch.
+TokenPlan token_plan(int64_t rows, int64_t cols, int64_t inner, int esize, bool gated)
+{
+    static const struct { int bm, bn, held; double cycles; } kTile[3] = {{256, 256, 1, 3000.}, {128, 128, 2, 900.}, {64, 128, 3, 600.}};
+    const int64_t steps = std::max<int64_t>(1, lvg_ceil_div(inner * esize, 128));
+    TokenPlan best = {LVG_TILE_128, 1};
+    double least = 1e300;
+    for (int t = 0; t < 3; t++)
+    {
+        const double step = kTile[t].cycles * (esize == 4 ? 8. : 1.);
+        const int64_t tiles = lvg_ceil_div(rows, kTile[t].bm) * lvg_ceil_div(cols, kTile[t].bn / (gated ? 2 : 1));
+        for (int64_t splits = 1; splits <= 64 && splits <= steps; splits = splits < 4 ? splits + 1 : splits * 3 / 2)
+        {
+            const int64_t each = lvg_ceil_div(steps, splits);
+            if (lvg_ceil_div(steps, each) != splits) continue;
+            const int64_t perCu = lvg_ceil_div(tiles * splits, 256), rounds = lvg_ceil_div(perCu, kTile[t].held);
+            const double held = (double)std::min<int64_t>(perCu, kTile[t].held);
+            double cost = (double)rounds * ((double)each * std::max(1500., held * step) + 5000.);
+            if (splits > 1) cost += 8000. + (double)splits * (double)rows * (double)cols * (gated ? 2 : 1) * 8. / 1800.;   // bytes / (bytes a cycle)
+            if (cost < least) { least = cost; best = {t, (int)splits}; }
+        }
+    }
+    return best;
+}
+
+extern "C" int64_t lvg_linear_act_work(int64_t rows, int64_t outer, int64_t inner, int dtype, int gated)
+{
+    if (!(float_type(dtype) || dtype == LVG_E4M3) || !size_ok(rows) || !size_ok(outer) || !size_ok(inner)) return LVG_ERR_INVALID;
+    return rows && outer ? work_bytes(rows, outer, inner, dtype, gated != 0) : 0;
+}
+
+extern "C" int lvg_linear_act(const void* x, const void* w, const void* b, const void* residual, const float* x_scale, const float* w_scale,
+                              void* y, void* slopes, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
+                              int64_t x_stride, int64_t w_stride, int64_t residual_stride, int64_t y_stride,
+                              int dtype, int out_dtype, int gated, int act, int slope_kind, float alpha, float gain, float clamp, void* stream)
+{
+    LVG_REQUIRE(float_type(dtype) || dtype == LVG_E4M3, "lvg_linear_act: operands must be float32 / float16 / bfloat16 / e4m3 (dtype %d)", dtype);
+    if (dtype == LVG_E4M3)
+        LVG_REQUIRE((out_dtype == LVG_BF16 || out_dtype == LVG_F16) && x_scale && w_scale, "lvg_linear_act: 8-bit operands need both scales and a float16 / bfloat16 result");
+    else
+        LVG_REQUIRE(out_dtype == dtype && !x_scale && !w_scale, "lvg_linear_act: the result has the operands' type, scales belong to 8-bit operands");
+    LVG_REQUIRE(size_ok(rows) && size_ok(outer) && size_ok(inner) && (!gated || size_ok(2 * outer)), "lvg_linear_act: bad size");
+    LVG_REQUIRE(act >= LVG_ACT_LINEAR && act <= LVG_ACT_SWISH, "lvg_linear_act: unknown activation %d", act);
+    if (rows == 0 || outer == 0) return LVG_OK;
+    LVG_REQUIRE(y && (inner == 0 || (x && w)), "lvg_linear_act: missing pointer");
+    LVG_REQUIRE(x_stride >= 0 && w_stride >= 0 && residual_stride >= 0 && y_stride >= outer, "lvg_linear_act: bad row stride");
+    LVG_REQUIRE(!gated || (!residual && clamp < 0.f), "lvg_linear_act: a gated unit has neither residual nor clamp");
+    LVG_REQUIRE(slope_kind == LVG_SLOPE_NONE || (slopes && (slope_kind == LVG_SLOPE_F32 || (slope_kind == LVG_SLOPE_CODE && !gated &&
+                (act == LVG_ACT_LINEAR || act == LVG_ACT_RELU || act == LVG_ACT_LRELU)))), "lvg_linear_act: bad slopes");
+    TokenArgs a;
+    memset(&a, 0, sizeof(a));
+    const int es = esize_of(dtype);
+    a.p = w; a.q = x;
+    a.ldp = w_stride * es; a.ldq = x_stride * es;
+    a.inner = inner; a.pRows = outer; a.qRows = rows;
+    Finish& f = a.fin;
+    f.qs = x_scale; f.ps = w_scale; f.bias = b; f.residual = residual; f.out = y; f.slopes = slope_kind ? slopes : nullptr;
+    f.ldr = residual_stride; f.ldo = y_stride; f.rows = rows; f.cols = outer;
+    f.act = act; f.slopeKind = slope_kind; f.alpha = alpha; f.gain = gain; f.clamp = clamp;
+    return run_product(a, gated ? LVG_TOKEN_GATED : LVG_TOKEN_FORWARD, dtype, out_dtype, work, work_size, static_cast<hipStream_t>(stream), "lvg_linear_act");
+}
+
+extern "C" int64_t lvg_linear_grad_work(int64_t rows, int64_t outer, int64_t inner, int weight, int dtype)
+{
+    if (!float_type(dtype) || !size_ok(rows) || !size_ok(outer) || !size_ok(inner)) return LVG_ERR_INVALID;
+    if (inner == 0 || (weight ? outer : rows) == 0) return 0;
+    return weight ? work_bytes(outer, inner, rows, dtype, false) : work_bytes(rows, inner, outer, dtype, false);
+}
+
+extern "C" int lvg_linear_grad(const void* dz, const void* other, void* grad, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
+                               int64_t dz_stride, int64_t other_stride, int weight, float gain, int dtype, void* stream)
+{
+    LVG_REQUIRE(float_type(dtype), "lvg_linear_grad: float32 / float16 / bfloat16 only (dtype %d)", dtype);
+    LVG_REQUIRE(size_ok(rows) && size_ok(outer) && size_ok(inner), "lvg_linear_grad: bad size");
+    if (inner == 0 || (weight ? outer : rows) == 0) return LVG_OK;
+    LVG_REQUIRE(grad && ((weight ? rows : outer) == 0 || (dz && other)), "lvg_linear_grad: missing pointer");
+    LVG_REQUIRE(dz_stride >= 0 && other_stride >= 0, "lvg_linear_grad: negative row stride");
+    TokenArgs a;
+    memset(&a, 0, sizeof(a));
+    const int es = esize_of(dtype);
+    a.p = other; a.q = dz;
+    a.ldp = other_stride * es; a.ldq = dz_stride * es;
+    a.inner = weight ? rows : outer; a.pRows = inner; a.qRows = weight ? outer : rows;
+    Finish& f = a.fin;
+    f.out = grad; f.ldo = inner; f.rows = a.qRows; f.cols = inner;
+    f.act = LVG_ACT_LINEAR; f.gain = gain; f.clamp = -1.f;
+    return run_product(a, weight ? LVG_TOKEN_WEIGHT_GRAD : LVG_TOKEN_ROW_GRAD, dtype, dtype, work, work_size, static_cast<hipStream_t>(stream), "lvg_linear_grad");
+}
+
+extern "C" int lvg_linear_slope_slots(int64_t rows, int64_t outer, int halves, int dtype)
+{
+    if (!float_type(dtype) || !size_ok(rows) || !size_ok(outer) || rows == 0 || outer == 0 || (halves != 1 && halves != 2)) return 0;
+    return slope_slots(rows, outer, halves, esize_of(dtype));
+}
+
+extern "C" int lvg_linear_slope(const void* dy, const void* slopes, void* dz, float* db_part, int64_t rows, int64_t outer, int64_t dy_stride, int64_t dz_stride,
+                                int halves, int slope_kind, int slots, float alpha, float gain, int dtype, void* stream)
+{
+    LVG_REQUIRE(float_type(dtype), "lvg_linear_slope: float32 / float16 / bfloat16 only (dtype %d)", dtype);
+    LVG_REQUIRE(size_ok(rows) && size_ok(outer) && (halves == 1 || halves == 2), "lvg_linear_slope: bad size");
+    if (rows == 0 || outer == 0) return LVG_OK;
+    LVG_REQUIRE(dy && (dz || db_part), "lvg_linear_slope: missing pointer");
+    LVG_REQUIRE(slope_kind == LVG_SLOPE_NONE ? halves == 1 : (slopes && (slope_kind == LVG_SLOPE_F32 || (slope_kind == LVG_SLOPE_CODE && halves == 1))), "lvg_linear_slope: bad slopes");
+    LVG_REQUIRE(dy_stride >= 0 && (!dz || dz_stride >= outer * halves), "lvg_linear_slope: bad row stride");
+    LVG_REQUIRE(slots == slope_slots(rows, outer, halves, esize_of(dtype)), "lvg_linear_slope: slots must be lvg_linear_slope_slots(...)");
+    SlopeArgs a = {dy, slopes, dz, db_part, rows, outer, dy_stride, dz_stride, halves, slope_kind, slope_lanes(outer, halves, esize_of(dtype)), alpha, gain};
+    const dim3 grid((unsigned)lvg_ceil_div(lvg_ceil_div(outer, 16 / esize_of(dtype)) * halves, a.lanes), (unsigned)slots), block(256);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (dtype == LVG_F32) hipLaunchKernelGGL(token_slope_kernel<float>, grid, block, 0, s, a);
+    else if (dtype == LVG_F16) hipLaunchKernelGGL(token_slope_kernel<f16_t>, grid, block, 0, s, a);
+    else hipLaunchKernelGGL(token_slope_kernel<bf16_t>, grid, block, 0, s, a);
+    return lvg_check_launch("lvg_linear_slope");
+}

@@ -1,0 +1,198 @@
+"""Dense layer on token rows with everything behind the product in its epilogue (csrc/token_gemm.h):
+
+    y = clamp(act(x w^T + b) * gain) + residual
+
+the dense counterpart of the convolutions' fused epilogues, with the activations of `bias_act`. The reference runs its dense layers as
+torch.addmm or matmul + bias_act (model/generator_lres.py:60-80). GPU tensors run the HIP kernels, forward and backward (float32, float16,
+bfloat16), and the 8-bit product (e4m3 rows and weights with one scale a row, forward only); CPU tensors and impl='ref' run the
+plain-PyTorch definition."""
+
+import torch
+
+from . import _hip
+from . import _rows
+from .bias_act import _resolve, activation_funcs
+
+SLOPE_NONE, SLOPE_F32, SLOPE_CODE = 0, 1, 2
+
+
+def linear_act(x, weight, b=None, residual=None, act='linear', alpha=None, gain=None, clamp=None, x_scale=None, weight_scale=None,
+               out_dtype=None, impl='cuda'):
+    r"""y = clamp(act(x w^T + b) * gain) + residual.
+
+    Args:
+        x:            rows [..., inner] in float32, float16, bfloat16 or float8_e4m3fn. Any strides; rows with unit element stride that start
+                      at multiples of 16 bytes are fastest.
+        weight:       [outer, inner] in x's dtype.
+        b:            [outer] in the result's dtype, or None.
+        residual:     [..., outer] in the result's dtype, added last, or None.
+        act:          key of `bias_act.activation_funcs`; alpha, gain, clamp as in `bias_act` (None = the activation's default / no clamp).
+        x_scale:      8-bit x only: float32 [...], the value of an element is itself times its row's scale.
+        weight_scale: 8-bit x only: float32 [outer], likewise for the rows of the weight.
+        out_dtype:    dtype of the result: x's, or for 8-bit x float16 or bfloat16 (default bfloat16).
+        impl:         'cuda' (HIP kernels when x is on the GPU) or 'ref' (plain PyTorch).
+
+    Differentiable once in x, weight, b and residual (not with 8-bit operands). Sums are float32; the result is rounded once."""
+    assert impl in ['ref', 'cuda']
+    out_dtype = _check(x, weight, b, x_scale, weight_scale, out_dtype, halves=1)
+    if residual is not None:
+        assert residual.shape == x.shape[:-1] + weight.shape[:1] and residual.dtype == out_dtype and residual.device == x.device
+        _no_grad_with_8bit(x, residual)
+    assert act in activation_funcs
+    _, alpha, gain, clamp = _resolve(act, alpha, gain, clamp)
+    if impl == 'ref' or not x.is_cuda:
+        return _linear_act_ref(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype)
+    if _rows.wants_grad(x, weight, b, residual):
+        return _LinearAct.apply(x, weight, b, residual, act, alpha, gain, clamp)
+    return _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype, False, SLOPE_NONE)[0]
+
+
+def _no_grad_with_8bit(x, *others):
+    assert x.dtype != torch.float8_e4m3fn or not _rows.wants_grad(*others), 'the product of 8-bit rows has no gradient'
+
+
+def _check(x, weight, b, x_scale, weight_scale, out_dtype, halves):
+    """Checks what the dense products share; returns the result's dtype. halves: 2 = the weight holds two projections."""
+    assert isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor)
+    assert x.ndim >= 1 and weight.ndim == 2 and x.shape[-1] == weight.shape[1], f'rows of {tuple(x.shape)} do not fit a weight of {tuple(weight.shape)}'
+    assert weight.shape[0] % halves == 0
+    assert weight.dtype == x.dtype and weight.device == x.device
+    if x.dtype == torch.float8_e4m3fn:
+        out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+        assert out_dtype in (torch.float16, torch.bfloat16), '8-bit operands give a float16 or bfloat16 result'
+        assert x_scale is not None and weight_scale is not None, '8-bit operands come with their scales'
+        assert x_scale.dtype == weight_scale.dtype == torch.float32 and x_scale.device == weight_scale.device == x.device
+        assert x_scale.shape == x.shape[:-1] and weight_scale.shape == weight.shape[:1]
+        _no_grad_with_8bit(x, b, x_scale, weight_scale)
+    else:
+        assert x.dtype in _rows.ROW_DTYPES, f'dtype {x.dtype} is not supported'
+        assert out_dtype in (None, x.dtype), 'the result has the operands\' dtype'
+        assert x_scale is None and weight_scale is None, 'scales belong to 8-bit operands'
+        out_dtype = x.dtype
+    if b is not None:
+        assert b.shape == weight.shape[:1] and b.dtype == out_dtype and b.device == x.device
+    return out_dtype
+
+
+def _sums_ref(x, weight, b, x_scale, weight_scale):
+    """x w^T + b, 16-bit and 8-bit operands in float32."""
+    x, weight = x.float(), weight.float()
+    if x_scale is not None:
+        x, weight = x * x_scale.unsqueeze(-1), weight * weight_scale.unsqueeze(-1)
+    return torch.nn.functional.linear(x, weight, None if b is None else b.float())
+
+
+def _linear_act_ref(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype):
+    """Definition of the op in stock PyTorch ops (CPU path and impl='ref')."""
+    y = activation_funcs[act].func(_sums_ref(x, weight, b, x_scale, weight_scale), alpha=alpha) * gain
+    if clamp >= 0:
+        y = y.clamp(-clamp, clamp)
+    if residual is not None:
+        y = y + residual.float()
+    return y.to(out_dtype)
+
+
+#----------------------------------------------------------------------------
+# HIP path.
+
+def slope_kind(act, gated):
+    """How the forward pass keeps the derivative: piecewise linear activations as one byte an element, smooth ones as float32."""
+    return SLOPE_CODE if not gated and act in ('linear', 'relu', 'lrelu') else SLOPE_F32
+
+
+def _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype, gated, kind):
+    """One product on x's device and the current stream: (y, slopes or None)."""
+    inner, halves = weight.shape[1], 2 if gated else 1
+    outer = weight.shape[0] // halves
+    y = torch.empty(x.shape[:-1] + (outer,), dtype=out_dtype, device=x.device)
+    x2, w2 = _rows.rows_of(x, inner), _rows.rows_of(weight, inner)
+    rows = x2.shape[0]
+    slopes = None
+    if kind != SLOPE_NONE:
+        slopes = torch.empty((rows, halves * outer), dtype=torch.float32 if kind == SLOPE_F32 else torch.uint8, device=x.device)
+    if y.numel() == 0:
+        return y, slopes
+    r2 = None if residual is None else _rows.rows_of(residual, outer)
+    b = None if b is None else b.contiguous()
+    if x_scale is not None:
+        x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+    code = _rows.type_code(x.dtype)
+    lib = _hip.lib()
+    with torch.cuda.device(x.device):
+        size = _hip.check(lib.lvg_linear_act_work(rows, outer, inner, code, int(gated)), 'lvg_linear_act')
+        work = _rows.work_of(size, x.device)
+        _hip.check(lib.lvg_linear_act(
+            _hip.ptr(x2), _hip.ptr(w2), _hip.ptr(b), _hip.ptr(r2), _hip.ptr(x_scale), _hip.ptr(weight_scale), y.data_ptr(), _hip.ptr(slopes), _hip.ptr(work), size,
+            rows, outer, inner, _rows.row_stride(x2), _rows.row_stride(w2), 0 if r2 is None else _rows.row_stride(r2), outer,
+            code, _hip.dtype_code(out_dtype), int(gated), activation_funcs[act].cuda_idx, kind, alpha, gain, clamp, _hip.stream(x.device)), 'lvg_linear_act')
+    return y, slopes
+
+
+def _grad_product(dz, other, rows, outer, inner, weight, gain, dtype):
+    """dz [rows, outer] against the weight [outer, inner] (weight False) or the rows [rows, inner] (True)."""
+    grad = torch.empty((outer if weight else rows, inner), dtype=dtype, device=dz.device)
+    if grad.numel() == 0:
+        return grad
+    lib, code = _hip.lib(), _hip.dtype_code(dtype)
+    size = _hip.check(lib.lvg_linear_grad_work(rows, outer, inner, int(weight), code), 'lvg_linear_grad')
+    work = _rows.work_of(size, dz.device)
+    _hip.check(lib.lvg_linear_grad(_hip.ptr(dz), _hip.ptr(other), grad.data_ptr(), _hip.ptr(work), size, rows, outer, inner, dz.stride(0) if rows > 1 else outer,
+                                   _rows.row_stride(other), int(weight), gain, code, _hip.stream(dz.device)), 'lvg_linear_grad')
+    return grad
+
+
+def _backward(dy, x, weight, slopes, kind, halves, alpha, gain, need_x, need_w, need_b):
+    """Gradients of x, weight and b from dy [..., outer]; kind SLOPE_NONE: dy itself times the gain is the gradient of the sums."""
+    inner, total = weight.shape[1], weight.shape[0]
+    outer = total // halves
+    x2, w2, dy2 = _rows.rows_of(x, inner), _rows.rows_of(weight, inner), _rows.rows_of(dy, outer)
+    rows, dtype, dev = x2.shape[0], x.dtype, x.device
+    dx = dw = db = None
+    with torch.cuda.device(dev):
+        if rows == 0 or outer == 0:
+            # nothing to sum over
+            return (x2.new_zeros(x.shape) if need_x else None, w2.new_zeros(weight.shape) if need_w else None, w2.new_zeros(total) if need_b else None)
+        lib, code = _hip.lib(), _hip.dtype_code(dtype)
+        plain = kind == SLOPE_NONE
+        dz, part = dy2, None
+        if not plain:
+            # rows of dz start at multiples of 16 bytes whatever the width: both products read them as they like it best
+            each = 16 // dtype.itemsize
+            dz = torch.empty((rows, -(-total // each) * each), dtype=dtype, device=dev)
+        if not plain or need_b:
+            slots = lib.lvg_linear_slope_slots(rows, outer, halves, code)
+            if need_b:
+                part = torch.empty((slots, total), dtype=torch.float32, device=dev)
+            _hip.check(lib.lvg_linear_slope(dy2.data_ptr(), _hip.ptr(slopes), None if plain else dz.data_ptr(), _hip.ptr(part), rows, outer, _rows.row_stride(dy2),
+                                            total if plain else dz.shape[1], halves, kind, slots, alpha, 1.0 if plain else gain, code, _hip.stream(dev)), 'lvg_linear_slope')
+        if need_b:
+            db = _rows.column_sum(part, dtype, gain if plain else 1.0)
+        scale = gain if plain else 1.0
+        if need_x:
+            dx = _grad_product(dz, w2, rows, total, inner, False, scale, dtype).reshape(x.shape)
+        if need_w:
+            dw = _grad_product(dz, x2, rows, total, inner, True, scale, dtype)
+    return dx, dw, db
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, b, residual, act, alpha, gain, clamp):
+        needed = any(ctx.needs_input_grad[:3])
+        kind = slope_kind(act, False) if needed and (act != 'linear' or clamp >= 0) else SLOPE_NONE
+        y, slopes = _forward(x, weight, b, residual, act, alpha, gain, clamp, None, None, x.dtype, False, kind)
+        ctx.save_for_backward(x, weight, slopes)
+        # (relu's lower side has no gradient whatever alpha a caller passed)
+        ctx.args = kind, 0.0 if act == 'relu' else alpha, gain
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, slopes = ctx.saved_tensors
+        kind, alpha, gain = ctx.args
+        need = ctx.needs_input_grad
+        dx = dw = db = None
+        if any(need[:3]):
+            dx, dw, db = _backward(dy, x, weight, slopes, kind, 1, alpha, gain, *need[:3])
+        return dx, dw, db, dy if need[3] else None, None, None, None, None

@@ -1,0 +1,143 @@
+"""Root-mean-square norm of token rows with the residual's addition, and 8-bit rows with one scale each (csrc/rms_norm.hip):
+
+    s = x + residual,   y = weight * s / sqrt(mean(s^2) + eps)
+    q = y / scale in e4m3,   scale = max |y| of the row / 448
+
+Without weight and residual it is what the reference's mapping networks do to their input in tensor expressions
+(model/generator_lres.py:444-480). GPU tensors run the HIP kernels, CPU tensors and impl='ref' the plain-PyTorch definition."""
+
+import torch
+
+from . import _hip
+from . import _rows
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-8, quantize=False, impl='cuda'):
+    r"""y = weight * s / sqrt(mean(s^2) + eps), s = x + residual, over the last dimension.
+
+    Args:
+        x:        rows [..., width] in float32, float16 or bfloat16.
+        weight:   [width] in x's dtype, or None (= 1).
+        residual: x's shape and dtype, or None.
+        eps:      added to the mean square.
+        quantize: return y as float8_e4m3fn rows and their scales.
+        impl:     'cuda' (HIP kernels when x is on the GPU) or 'ref' (plain PyTorch).
+
+    Returns y; with quantize (q, scale), scale float32 [...]; with a residual also s (rounded to x's dtype) behind them. The norm is taken of
+    the sum before that rounding. Differentiable once in x, weight and residual, through y and s; not with quantize."""
+    assert impl in ['ref', 'cuda']
+    assert isinstance(x, torch.Tensor) and x.ndim >= 1 and x.shape[-1] >= 1 and x.dtype in _rows.ROW_DTYPES
+    assert eps >= 0
+    if weight is not None:
+        assert weight.shape == x.shape[-1:] and weight.dtype == x.dtype and weight.device == x.device
+    if residual is not None:
+        assert residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device
+    grad = _rows.wants_grad(x, weight, residual)
+    assert not (quantize and grad), '8-bit rows have no gradient'
+    if impl == 'ref' or not x.is_cuda:
+        out = _rms_norm_ref(x, weight, residual, eps, quantize)
+    elif grad:
+        out = _RmsNorm.apply(x, weight, residual, eps)
+    else:
+        y, scale, total, _ = _forward(x, weight, residual, eps, quantize, False)
+        out = tuple(t for t in (y, scale, total) if t is not None)
+    return out[0] if len(out) == 1 else out
+
+
+def quantize_rows(x, impl='cuda'):
+    """(q, scale): x [..., width] as float8_e4m3fn rows and float32 scales [...], x = q * scale; scale = max |x| of the row / 448, at least 2^-64.
+    A row with a NaN has a NaN scale. For float32, float16 and bfloat16; no gradient."""
+    assert impl in ['ref', 'cuda']
+    assert isinstance(x, torch.Tensor) and x.ndim >= 1 and x.shape[-1] >= 1 and x.dtype in _rows.ROW_DTYPES
+    assert not _rows.wants_grad(x), '8-bit rows have no gradient'
+    if impl == 'ref' or not x.is_cuda:
+        return _quantize_ref(x.float())
+    width = x.shape[-1]
+    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    if x.numel():
+        x2 = _rows.rows_of(x, width)
+        with torch.cuda.device(x.device):
+            _hip.check(_hip.lib().lvg_quantize_rows(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], width, _rows.row_stride(x2),
+                                                    _hip.dtype_code(x.dtype), _hip.stream(x.device)), 'lvg_quantize_rows')
+    return q, scale
+
+
+def _quantize_ref(v):
+    scale = (v.abs().amax(dim=-1) / _rows.E4M3_MAX).clamp(min=_rows.SCALE_MIN)
+    return (v / scale.unsqueeze(-1)).clamp(-_rows.E4M3_MAX, _rows.E4M3_MAX).to(torch.float8_e4m3fn), scale
+
+
+def _rms_norm_ref(x, weight, residual, eps, quantize):
+    """Definition of the op in stock PyTorch ops (CPU path and impl='ref')."""
+    s = x.float()
+    if residual is not None:
+        s = s + residual.float()
+    y = s * torch.rsqrt(s.square().mean(dim=-1, keepdim=True) + eps)
+    if weight is not None:
+        y = y * weight.float()
+    out = _quantize_ref(y) if quantize else (y.to(x.dtype),)
+    return out if residual is None else out + (s.to(x.dtype),)
+
+
+#----------------------------------------------------------------------------
+# HIP path.
+
+def _forward(x, weight, residual, eps, quantize, keep):
+    """(y or q, scale or None, s or None, rstd or None) on x's device and the current stream."""
+    width = x.shape[-1]
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if quantize else x.dtype, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quantize else None
+    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    x2 = _rows.rows_of(x, width)
+    rows = x2.shape[0]
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep else None
+    if rows:
+        r2 = None if residual is None else _rows.rows_of(residual, width)
+        weight = None if weight is None else weight.contiguous()
+        with torch.cuda.device(x.device):
+            _hip.check(_hip.lib().lvg_rms_norm(x2.data_ptr(), _hip.ptr(r2), _hip.ptr(weight), y.data_ptr(), _hip.ptr(total), _hip.ptr(rstd), _hip.ptr(scale),
+                                               rows, width, _rows.row_stride(x2), 0 if r2 is None else _rows.row_stride(r2), eps, _hip.dtype_code(x.dtype),
+                                               int(quantize), _hip.stream(x.device)), 'lvg_rms_norm')
+    return y, scale, total, rstd
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, _, total, rstd = _forward(x, weight, residual, eps, False, True)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x if total is None else total, weight, rstd)
+        return (y,) if total is None else (y, total)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, weight, rstd = ctx.saved_tensors
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        dw = None
+        if dy is None:
+            # only the sum was used
+            dx = ds
+            if need_w:
+                dw = torch.zeros_like(weight)
+        else:
+            width = s.shape[-1]
+            s2, dy2 = _rows.rows_of(s, width), _rows.rows_of(dy, width)
+            ds2 = None if ds is None else _rows.rows_of(ds, width)
+            rows, dev = s2.shape[0], s.device
+            dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
+            if rows == 0:
+                return dx, torch.zeros_like(weight) if need_w else None, dx if need_r else None, None
+            lib, code = _hip.lib(), _hip.dtype_code(s.dtype)
+            with torch.cuda.device(dev):
+                slots = lib.lvg_rms_norm_backward_slots(rows, width, code)
+                part = torch.empty((slots, width), dtype=torch.float32, device=dev) if need_w else None
+                row_work = torch.empty(rows, dtype=torch.float32, device=dev)
+                weight = None if weight is None else weight.contiguous()
+                _hip.check(lib.lvg_rms_norm_backward(dy2.data_ptr(), _hip.ptr(ds2), s2.data_ptr(), _hip.ptr(weight), rstd.data_ptr(), dx.data_ptr(), _hip.ptr(part),
+                                                     row_work.data_ptr(), rows, width, _rows.row_stride(dy2), 0 if ds2 is None else _rows.row_stride(ds2),
+                                                     _rows.row_stride(s2), slots, code, _hip.stream(dev)), 'lvg_rms_norm_backward')
+                if need_w:
+                    dw = _rows.column_sum(part, s.dtype)
+        return dx if need_x else None, dw, dx if need_r else None, None
