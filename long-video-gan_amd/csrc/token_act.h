@@ -109,19 +109,18 @@ template <class T> __device__ __forceinline__ void quad_store(T* p, int64_t n, b
     }
 }
 
-// Four neighbouring results: row m, columns n .. n + 3 (those below cols). v: sums; gated: v of the gate half, u of the up half.
-template <class O, bool GATED> __device__ __forceinline__ void finish4(const Finish& f, int64_t m, int64_t n, float* v, float* u)
+// Four neighbouring sums, row m, columns n .. n + 3 (those below cols): scales and bias. v: sums; gated: v of the gate half, u of the up half.
+template <class O, bool GATED> __device__ __forceinline__ void prepare4(const Finish& f, int64_t m, int64_t n, float* v, float* u)
 {
     const int64_t left = f.cols - n;
-    if (m >= f.rows || left <= 0) return;
     if (f.qs)
     {
         const float s = f.qs[m];
         #pragma unroll
         for (int i = 0; i < 4; i++) if (i < left)
         {
-            v[i] = v[i] * s * f.ps[n + i];
-            if (GATED) u[i] = u[i] * s * f.ps[f.cols + n + i];
+            v[i] *= s * f.ps[n + i];
+            if (GATED) u[i] *= s * f.ps[f.cols + n + i];
         }
     }
     if (f.bias)
@@ -137,6 +136,12 @@ template <class O, bool GATED> __device__ __forceinline__ void finish4(const Fin
             for (int i = 0; i < 4; i++) u[i] += b[i];
         }
     }
+}
+
+// The results of four such sums: activation, slopes, residual, store.
+template <class O, bool GATED> __device__ __forceinline__ void finish4(const Finish& f, int64_t m, int64_t n, float* v, float* u)
+{
+    const int64_t left = f.cols - n;
     float a[4], d[4];
     const bool want = f.slopeKind != LVG_SLOPE_NONE;
     #pragma unroll

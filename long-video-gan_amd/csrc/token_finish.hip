@@ -32,6 +32,7 @@ __global__ __launch_bounds__(256) void token_finish_kernel(const float* part, in
             u[0] += b.x; u[1] += b.y; u[2] += b.z; u[3] += b.w;
         }
     }
+    prepare4<O, GATED>(f, m, n, v, u);
     finish4<O, GATED>(f, m, n, v, u);
 }
 
@@ -176,8 +177,8 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
     const int64_t rows = a.qRows, cols = a.pRows;
     const TokenPlan k = token_plan(rows, cols, a.inner, es, gated);
     const int bm = k.tile == LVG_TILE_256 ? 256 : k.tile == LVG_TILE_128 ? 128 : 64, bn = (k.tile == LVG_TILE_256 ? 256 : 128) / (gated ? 2 : 1);
-    a.steps = lvg_ceil_div(a.inner * es, 128);
-    a.stepsPerSplit = lvg_ceil_div(a.steps, k.splits);
+    a.steps = (int)lvg_ceil_div(a.inner * es, 128);
+    a.stepsPerSplit = (int)lvg_ceil_div(a.steps, k.splits);
     a.splits = k.splits;
     a.tilesM = (int)lvg_ceil_div(rows, bm);
     a.tilesN = lvg_ceil_div(cols, bn);

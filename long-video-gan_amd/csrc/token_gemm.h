@@ -12,6 +12,8 @@
 //
 // The column operand is the matrix instruction's first one: a lane then holds four neighbouring columns of one row, and what is done with the
 // sums (token_act.h) moves whole vectors. The tile leaves through LDS, wave by wave without a barrier, in rows of 64 columns.
+// A wave of the largest tile owns 128 x 128 results (256 accumulator registers, one wave a SIMD): 32 fragment reads feed 64 products a step, where
+// eight waves of 128 x 64 would read 48.
 //
 // Aligned operands go from memory to LDS without registers; rows that start at odd places are loaded (unaligned 16-byte accesses), held over the
 // step's products and written to LDS behind them. Steps past the operand's last whole 128 bytes are loaded under masks, zeros beyond the end.
@@ -30,7 +32,7 @@ struct TokenArgs
     int64_t     ldp, ldq;      // bytes between stored rows
     int64_t     inner;         // summed index
     int64_t     pRows, qRows;  // columns / rows of the result (gated: pRows of each half)
-    int64_t     steps, stepsPerSplit;
+    int         steps, stepsPerSplit;
     int64_t     tiles, tilesN;
     int         tilesM;
     int         splits;
@@ -61,9 +63,10 @@ template <class T, int BX> struct Fragments<T, BX, ALONG>
         for (int ks = 0; ks < 4; ks++)
             off[ks] = (uint32_t)(base + (lane & 31)) * 128u + (uint32_t)(((2 * ks + (lane >> 5)) ^ ((lane >> 1) & 7)) << 4);
     }
-    __device__ __forceinline__ uint4 read(uint32_t tile, int j, int ks) const
+    // at: the operand's place in the tile buffer
+    __device__ __forceinline__ uint4 read(uint32_t tile, int at, int j, int ks) const
     {
-        const u32x4 v = *(lds_vec_ptr)(uintptr_t)(tile + off[ks] + (uint32_t)j * 4096u);
+        const u32x4 v = ((lds_vec_ptr)(uintptr_t)(tile + off[ks]))[at / 16 + j * 256];
         uint4 r;
         __builtin_memcpy(&r, &v, 16);
         return r;
@@ -88,20 +91,20 @@ template <class T, int BX> struct Fragments<T, BX, DOWN>
         for (int j = 0; j < 4; j++)
             off[j] = row * kPitch + (((uint32_t)(base / 32 + j) ^ sw) << 6) + 32u * ((lane >> 4) & 1) + 8u * (lane & 3);
     }
-    __device__ __forceinline__ uint4 read(uint32_t tile, int j, int ks) const
+    __device__ __forceinline__ uint4 read(uint32_t tile, int at, int j, int ks) const
     {
         uint4 r;
         if (sizeof(T) == 4)
         {
             uint32_t w[4];
             #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = *(lds_word_ptr)(uintptr_t)(tile + off[j] + (uint32_t)((8 * ks + i) * kPitch));
+            for (int i = 0; i < 4; i++) w[i] = ((lds_word_ptr)(uintptr_t)(tile + off[j]))[(at + (8 * ks + i) * kPitch) / 4];
             __builtin_memcpy(&r, w, 16);
             return r;
         }
-        const uint32_t at = tile + off[j] + (uint32_t)(16 * ks * kPitch);
-        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(uintptr_t)at);
-        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr_ptr)(uintptr_t)(at + 4u * kPitch));
+        const lds_tr_ptr from = (lds_tr_ptr)(uintptr_t)(tile + off[j]);
+        const short4v lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(from + (at + 16 * ks * kPitch) / 8);
+        const short4v hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(from + (at + (16 * ks + 4) * kPitch) / 8);
         __builtin_memcpy(&r, &lo, 8);
         __builtin_memcpy(reinterpret_cast<char*>(&r) + 8, &hi, 8);
         return r;
@@ -171,7 +174,7 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
             }
         }
     }
-    __device__ __forceinline__ uint4 masked(int64_t step, int i) const
+    __device__ __forceinline__ uint4 masked(int step, int i) const
     {
         int row, chunk;
         chunk_of(i, row, chunk);
@@ -181,13 +184,13 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
         {
             bool up;
             const int64_t r = place(row, up);
-            const int64_t k = step * kDepth + chunk * kE;
+            const int64_t k = (int64_t)step * kDepth + chunk * kE;
             at = base + r * ld + (up ? upOff : 0) + k * (int64_t)sizeof(T);
             n = inner - k;
         }
         else
         {
-            const int64_t k = step * kDepth + row;
+            const int64_t k = (int64_t)step * kDepth + row;
             at = base + k * ld + (int64_t)chunk * 16;
             n = k < inner ? left - (int64_t)chunk * kE : 0;
         }
@@ -212,31 +215,34 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
         __builtin_memcpy(&w, &v, 16);
         *(lds_vec_ptr)(uintptr_t)(tile + (uint32_t)(i * NTHR + tid) * 16u) = w;
     }
-    // before a step's products: start what the next step needs
-    __device__ __forceinline__ void begin(int64_t step, uint32_t tile)
+    // a whole step's tile straight to LDS, this thread's chunk i of it
+    __device__ __forceinline__ void send(int i, int step, uint32_t tile, int wave) const
     {
-        if (DIRECT)
+        const char* b = base + (int64_t)step * (LAYOUT == ALONG ? 128 : kDepth * ld);
+        wdma16(reinterpret_cast<const unsigned char*>(b), off[DIRECT ? i : 0], tile + (uint32_t)(i * NTHR + wave * 64) * 16u);
+    }
+    // A step's tile is started in two halves (0, 1). Rows that go through registers are all loaded in the first, masked steps of direct ones are
+    // written in the second.
+    __device__ __forceinline__ void begin(int half, int step, uint32_t tile, int wave)
+    {
+        if (!DIRECT)
         {
-            if ((step + 1) * kDepth <= inner)
-            {
-                const char* b = base + (LAYOUT == ALONG ? step * 128 : step * kDepth * ld);
-                #pragma unroll
-                for (int i = 0; i < kNum; i++)
-                    wdma16(reinterpret_cast<const unsigned char*>(b), off[i], tile + (uint32_t)(i * NTHR + (tid & ~63)) * 16u);
-            }
-            else
-            {
-                #pragma unroll 1
-                for (int i = 0; i < kNum; i++) put(tile, i, masked(step, i));
-            }
-        }
-        else
-        {
+            if (half) return;
             #pragma unroll
             for (int i = 0; i < kNum; i++) hold[i] = masked(step, i);
         }
+        else if ((int64_t)(step + 1) * kDepth <= inner)
+        {
+            #pragma unroll
+            for (int i = 0; i < kNum; i++) if ((i < kNum / 2) == (half == 0)) send(i, step, tile, wave);
+        }
+        else if (half)
+        {
+            #pragma unroll 1
+            for (int i = 0; i < kNum; i++) put(tile, i, masked(step, i));
+        }
     }
-    // behind them
+    // registers to LDS
     __device__ __forceinline__ void end(uint32_t tile)
     {
         if (DIRECT) return;
@@ -278,12 +284,58 @@ __device__ __forceinline__ void wave_lds_order()
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// T operands, O results; WR x WC waves, each with a (BM / WR) x 64 part of the tile.
+// Values that are the same for the whole workgroup, kept in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// The sums' way out: four columns of a row a lane, the same four for all rows, so what belongs to columns is loaded once.
+template <class O, bool GATED> struct Columns
+{
+    float bias[4], biasUp[4], scale[4], scaleUp[4];
+    __device__ __forceinline__ void init(const Finish& f, int64_t n)
+    {
+        const int64_t left = f.cols - n;
+        #pragma unroll
+        for (int i = 0; i < 4; i++) { bias[i] = biasUp[i] = 0.f; scale[i] = scaleUp[i] = 1.f; }
+        if (left <= 0) return;
+        if (f.bias)
+        {
+            quad_load(static_cast<const O*>(f.bias) + n, left, f.vec, bias);
+            if (GATED) quad_load(static_cast<const O*>(f.bias) + f.cols + n, left, f.vec, biasUp);
+        }
+        if (f.qs)
+        {
+            quad_load(f.ps + n, left, false, scale);
+            if (GATED) quad_load(f.ps + f.cols + n, left, false, scaleUp);
+        }
+    }
+    __device__ __forceinline__ void apply(const Finish& f, int64_t m, float* v, float* u) const
+    {
+        if (f.qs)
+        {
+            const float s = f.qs[m];
+            #pragma unroll
+            for (int i = 0; i < 4; i++)
+            {
+                v[i] *= s * scale[i];
+                if (GATED) u[i] *= s * scaleUp[i];
+            }
+        }
+        #pragma unroll
+        for (int i = 0; i < 4; i++)
+        {
+            v[i] += bias[i];
+            if (GATED) u[i] += biasUp[i];
+        }
+    }
+};
+
+// T operands, O results; WR x WC waves, each with a (BM / WR) x (BN / WC) part of the tile.
 template <class T, class O, int BM, int BN, int WR, int WC, int PL, int QL, bool GATED, bool DIRECT>
 __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
 {
     constexpr int kThreads = WR * WC * 64, MT = BM / WR / 32, NT = BN / WC / 32;
-    static_assert(NT == 2 && MT >= 1 && MT <= 4, "a wave owns two blocks of 32 columns");
+    static_assert((NT == 2 || NT == 4) && MT >= 1 && MT <= 4, "a wave owns 64 or 128 columns");
+    constexpr int kFrags = sizeof(T) == 1 ? 2 : 1, kGroups = 4 / kFrags;    // 16-byte fragments a product takes; groups of products a step
     constexpr uint32_t kBufBytes = (uint32_t)(BM + BN) * 128u;
     constexpr int kOutPitch = 64 * 4 + 16;                         // bytes of a row of a wave's results on their way out
     static_assert(WR * WC * 32 * kOutPitch <= 2 * (int)kBufBytes, "the results leave through the operands' LDS");
@@ -300,12 +352,12 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
         const int64_t each = total / 8, more = total % 8, x = id % 8;
         id = x * each + (x < more ? x : more) + id / 8;
     }
-    const int split = (int)(id / a.tiles);
+    const int split = uniform((int)(id / a.tiles));
     id -= (int64_t)split * a.tiles;
     const int64_t band = 4 * a.tilesN, g = id / band;
     const int64_t high = min((int64_t)4, (int64_t)a.tilesM - g * 4);
     const int64_t tm = g * 4 + (id - g * band) % high, tn = (id - g * band) / high;
-    const int64_t m0 = tm * BM, n0 = tn * (GATED ? BN / 2 : BN);
+    const int64_t m0 = (int64_t)uniform((int)tm) * BM, n0 = (int64_t)uniform((int)tn) * (GATED ? BN / 2 : BN);
 
     Loader<T, BN, PL, kThreads, GATED, DIRECT> pl;
     Loader<T, BM, QL, kThreads, false, DIRECT> ql;
@@ -313,7 +365,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
     ql.init(a.q, a.ldq, a.inner, m0, a.qRows, tid);
     Fragments<T, BN, PL> pf;
     Fragments<T, BM, QL> qf;
-    pf.init(lane, wc * 64);
+    pf.init(lane, wc * NT * 32);
     qf.init(lane, wr * MT * 32);
 
     f32x16 acc[MT][NT];
@@ -325,101 +377,196 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
             for (int r = 0; r < 16; r++) acc[i][j][r] = 0.f;
 
     const uint32_t lds = (uint32_t)(uintptr_t)smem;
-    const int64_t s0 = split * a.stepsPerSplit, s1 = min(s0 + a.stepsPerSplit, a.steps);
+    const int s0 = split * a.stepsPerSplit, s1 = min(s0 + a.stepsPerSplit, a.steps);
+
+    // The fragments of a group of products are read while the group before it is multiplied, over the step's end too: once the last group's
+    // fragments are in registers the step's buffer is free, every wave meets at the barrier, the next step's tiles (on their way for a whole
+    // step) are there, and the tiles of the step after that start into the freed buffer.
+    uint4 pv[2][kFrags][NT], qv[2][kFrags][MT];
+    auto fetch = [&](uint32_t pt, int group, int set)
+    {
+        #pragma unroll
+        for (int f = 0; f < kFrags; f++)
+        {
+            #pragma unroll
+            for (int j = 0; j < NT; j++) pv[set][f][j] = pf.read(pt, 0, j, group * kFrags + f);
+            #pragma unroll
+            for (int i = 0; i < MT; i++) qv[set][f][i] = qf.read(pt, BN * 128, i, group * kFrags + f);
+        }
+    };
+    // between: called behind every product with its number, for work that the matrix unit's time covers
+    auto multiply = [&](int set, auto between)
+    {
+        #pragma unroll
+        for (int i = 0; i < MT; i++)
+            #pragma unroll
+            for (int j = 0; j < NT; j++)
+            {
+                if constexpr (kFrags == 2) acc[i][j] = product8(pv[set][0][j], pv[set][1][j], qv[set][0][i], qv[set][1][i], acc[i][j]);
+                else acc[i][j] = Product<T>::run(pv[set][0][j], qv[set][0][i], acc[i][j]);
+                between(i * NT + j);
+            }
+    };
+    auto start = [&](int half, int step, uint32_t pt) { pl.begin(half, step, pt, wave); ql.begin(half, step, pt + BN * 128, wave); };
+    auto meet = [&] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     if (s0 < s1)
     {
-        pl.begin(s0, lds);
-        ql.begin(s0, lds + BN * 128);
+        start(0, s0, lds);
+        start(1, s0, lds);
         pl.end(lds);
         ql.end(lds + BN * 128);
+        meet();
+        if (s0 + 1 < s1) start(0, s0 + 1, lds + kBufBytes);
+        fetch(lds, 0, 0);
     }
-    for (int64_t s = s0; s < s1; s++)
+    int s = s0;
+    if (DIRECT)
     {
-        const uint32_t pt = lds + (uint32_t)((s - s0) & 1) * kBufBytes, qt = pt + BN * 128;
-        const uint32_t pn = lds + (uint32_t)((s - s0 + 1) & 1) * kBufBytes, qn = pn + BN * 128;
-        // this step's tiles have arrived, and every wave is done with the other buffer
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + 1 < s1)
+        // Steps whose second next one is whole: no branches. The sends for a step lie between the products of the group behind the barrier that
+        // frees its buffer and of the group after that.
+        auto spread = [&](int k, int half, int step, uint32_t pt)
         {
-            pl.begin(s + 1, pn);
-            ql.begin(s + 1, qn);
-        }
-        if constexpr (sizeof(T) == 1)
-        {
+            constexpr int kP = BN * 8 / kThreads / 2, kAll = kP + BM * 8 / kThreads / 2, kMma = MT * NT;
             #pragma unroll
-            for (int ks = 0; ks < 4; ks += 2)
+            for (int i = 0; i < kAll; i++)
+                if (i * kMma / kAll == k)
+                {
+                    if (i < kP) pl.send(half * kP + i, step, pt, wave);
+                    else ql.send(half * (kAll - kP) + i - kP, step, pt + BN * 128, wave);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const int whole = min(s1, (int)(a.inner / (128 / (int)sizeof(T))));
+        for (; s + 2 < whole; s++)
+        {
+            const uint32_t pt = lds + (uint32_t)((s - s0) & 1) * kBufBytes, pn = lds + (uint32_t)((s - s0 + 1) & 1) * kBufBytes;
+            __builtin_amdgcn_s_waitcnt(0xc07f);        // lgkmcnt(0): the first group's fragments, asked for a group of products ago
+            #pragma unroll
+            for (int group = 0; group < kGroups; group++)
             {
-                uint4 pv[NT][2], qv[MT][2];
-                #pragma unroll
-                for (int j = 0; j < NT; j++) { pv[j][0] = pf.read(pt, j, ks); pv[j][1] = pf.read(pt, j, ks + 1); }
-                #pragma unroll
-                for (int i = 0; i < MT; i++) { qv[i][0] = qf.read(qt, i, ks); qv[i][1] = qf.read(qt, i, ks + 1); }
-                #pragma unroll
-                for (int i = 0; i < MT; i++)
-                    #pragma unroll
-                    for (int j = 0; j < NT; j++) acc[i][j] = product8(pv[j][0], pv[j][1], qv[i][0], qv[i][1], acc[i][j]);
+                if (group + 1 < kGroups) fetch(pt, group + 1, (group + 1) & 1);
+                else
+                {
+                    meet();
+                    fetch(pn, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (group == 0) multiply(0, [&](int k) { spread(k, 1, s + 1, pn); });
+                else if (group + 1 == kGroups) multiply(group & 1, [&](int k) { spread(k, 0, s + 2, pt); });
+                else multiply(group & 1, [](int) {});
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        else
+    }
+    for (; s < s1; s++)
+    {
+        const uint32_t pt = lds + (uint32_t)((s - s0) & 1) * kBufBytes, pn = lds + (uint32_t)((s - s0 + 1) & 1) * kBufBytes;
+        if (s + 1 < s1) start(1, s + 1, pn);
+        #pragma unroll
+        for (int group = 0; group < kGroups; group++)
         {
-            #pragma unroll
-            for (int ks = 0; ks < 4; ks++)
+            if (group + 1 < kGroups) fetch(pt, group + 1, (group + 1) & 1);
+            else if (s + 1 < s1)
             {
-                uint4 pv[NT], qv[MT];
-                #pragma unroll
-                for (int j = 0; j < NT; j++) pv[j] = pf.read(pt, j, ks);
-                #pragma unroll
-                for (int i = 0; i < MT; i++) qv[i] = qf.read(qt, i, ks);
-                #pragma unroll
-                for (int i = 0; i < MT; i++)
-                    #pragma unroll
-                    for (int j = 0; j < NT; j++) acc[i][j] = Product<T>::run(pv[j], qv[i], acc[i][j]);
+                pl.end(pn);
+                ql.end(pn + BN * 128);
+                meet();
+                fetch(pn, 0, 0);
+                if (s + 2 < s1) start(0, s + 2, pt);
             }
-        }
-        if (s + 1 < s1)
-        {
-            pl.end(pn);
-            ql.end(qn);
+            multiply(group & 1, [](int) {});
         }
     }
     __syncthreads();
 
-    // A block's lane holds row lane & 31, columns 8 (r / 4) + 4 (lane / 32) + r % 4.
+    // 32 rows x 64 columns of a wave's sums at a time. A block's lane holds row lane & 31, columns 8 (r / 4) + 4 (lane / 32) + r % 4; read back
+    // from LDS, neighbouring lanes hold neighbouring columns, and whole rows go to memory.
     unsigned char* const out = smem + wave * 32 * kOutPitch;
-    #pragma unroll
-    for (int i = 0; i < MT; i++)
+    constexpr int kLanes = GATED ? 8 : 16, kRows = 64 / kLanes, kTurns = 32 / kRows;   // lanes a row (four columns each), rows a turn
+    const int c = (lane % kLanes) * 4;
+    const Finish& f = a.fin;
+    const bool quick = !GATED && f.act == LVG_ACT_LINEAR && f.slopeKind == LVG_SLOPE_NONE && f.clamp < 0.f && f.vec;
+    #pragma unroll 1
+    for (int h = 0; h < NT / 2; h++)
     {
-        #pragma unroll
-        for (int j = 0; j < NT; j++)
-            #pragma unroll
-            for (int c = 0; c < 4; c++)
-                *reinterpret_cast<float4*>(out + (lane & 31) * kOutPitch + (32 * j + 8 * c + 4 * (lane >> 5)) * 4) =
-                    make_float4(acc[i][j][4 * c], acc[i][j][4 * c + 1], acc[i][j][4 * c + 2], acc[i][j][4 * c + 3]);
-        wave_lds_order();
-        const int64_t mBase = m0 + wr * MT * 32 + i * 32;
-        constexpr int kLanes = GATED ? 8 : 16;                     // lanes a row, four columns each
+        const int64_t n = n0 + (wc * NT / 2 + h) * (GATED ? 32 : 64) + c;
+        Columns<O, GATED> cols;
+        if (!a.part) cols.init(f, n);
         #pragma unroll 1
-        for (int r = 0; r < 32; r += 64 / kLanes)
+        for (int i = 0; i < MT; i++)
         {
-            const int row = r + lane / kLanes, c = (lane % kLanes) * 4;
-            const int64_t m = mBase + row, n = n0 + wc * (GATED ? 32 : 64) + c;
-            const float4 v4 = *reinterpret_cast<const float4*>(out + row * kOutPitch + c * 4);
-            float v[4] = {v4.x, v4.y, v4.z, v4.w}, u[4] = {0.f, 0.f, 0.f, 0.f};
-            if (GATED)
+            const int64_t m1 = m0 + wr * MT * 32 + i * 32 + lane / kLanes;
+            Quad<O> res[kTurns];
+            const bool add = quick && !a.part && f.residual && n < f.cols;
+            if (add)
             {
-                const float4 u4 = *reinterpret_cast<const float4*>(out + row * kOutPitch + (32 + c) * 4);
-                u[0] = u4.x; u[1] = u4.y; u[2] = u4.z; u[3] = u4.w;
+                #pragma unroll
+                for (int t = 0; t < kTurns; t++)
+                    if (m1 + t * kRows < f.rows) res[t] = *reinterpret_cast<const Quad<O>*>(static_cast<const O*>(f.residual) + (m1 + t * kRows) * f.ldr + n);
             }
+            wave_lds_order();
+            #pragma unroll
+            for (int ii = 0; ii < MT; ii++)
+                #pragma unroll
+                for (int hh = 0; hh < NT / 2; hh++)
+                    if (ii == i && hh == h)
+                    {
+                        #pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            #pragma unroll
+                            for (int q = 0; q < 4; q++)
+                                *reinterpret_cast<float4*>(out + (lane & 31) * kOutPitch + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) =
+                                    make_float4(acc[ii][2 * hh + j][4 * q], acc[ii][2 * hh + j][4 * q + 1], acc[ii][2 * hh + j][4 * q + 2], acc[ii][2 * hh + j][4 * q + 3]);
+                    }
+            wave_lds_order();
             if (a.part)
             {
-                if (m >= a.qRows || n >= a.pRows) continue;
-                float* at = a.part + ((int64_t)split * a.qRows + m) * a.ldpart + n;      // (ldpart, or each half of it, is a multiple of four)
-                *reinterpret_cast<float4*>(at) = make_float4(v[0], v[1], v[2], v[3]);
-                if (GATED) *reinterpret_cast<float4*>(at + a.ldpart / 2) = make_float4(u[0], u[1], u[2], u[3]);
+                #pragma unroll
+                for (int t = 0; t < kTurns; t++)
+                {
+                    const int64_t m = m1 + t * kRows;
+                    const unsigned char* from = out + (lane / kLanes + t * kRows) * kOutPitch + c * 4;
+                    if (m >= a.qRows || n >= a.pRows) continue;
+                    float* at = a.part + ((int64_t)split * a.qRows + m) * a.ldpart + n;      // (ldpart, or each half of it, is a multiple of four)
+                    *reinterpret_cast<float4*>(at) = *reinterpret_cast<const float4*>(from);
+                    if (GATED) *reinterpret_cast<float4*>(at + a.ldpart / 2) = *reinterpret_cast<const float4*>(from + 128);
+                }
             }
-            else finish4<O, GATED>(a.fin, m, n, v, u);
+            else if (quick)
+            {
+                #pragma unroll
+                for (int t = 0; t < kTurns; t++)
+                {
+                    const int64_t m = m1 + t * kRows;
+                    const float4 v4 = *reinterpret_cast<const float4*>(out + (lane / kLanes + t * kRows) * kOutPitch + c * 4);
+                    if (m >= f.rows || n >= f.cols) continue;
+                    float v[4] = {v4.x, v4.y, v4.z, v4.w}, u[4];
+                    cols.apply(f, m, v, u);
+                    #pragma unroll
+                    for (int k = 0; k < 4; k++) v[k] = v[k] * f.gain + (add ? row_load(res[t].v[k]) : 0.f);
+                    quad_store(static_cast<O*>(f.out) + m * f.ldo + n, 4, true, v);
+                }
+            }
+            else
+            {
+                #pragma unroll 1
+                for (int t = 0; t < kTurns; t++)
+                {
+                    const int64_t m = m1 + t * kRows;
+                    const unsigned char* from = out + (lane / kLanes + t * kRows) * kOutPitch + c * 4;
+                    const float4 v4 = *reinterpret_cast<const float4*>(from);
+                    float v[4] = {v4.x, v4.y, v4.z, v4.w}, u[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (GATED)
+                    {
+                        const float4 u4 = *reinterpret_cast<const float4*>(from + 128);
+                        u[0] = u4.x; u[1] = u4.y; u[2] = u4.z; u[3] = u4.w;
+                    }
+                    if (m >= f.rows || n >= f.cols) continue;
+                    cols.apply(f, m, v, u);
+                    finish4<O, GATED>(f, m, n, v, u);
+                }
+            }
         }
-        wave_lds_order();
     }
 }
 
@@ -447,7 +594,7 @@ template <class T, class O, int PL, int QL, bool GATED> int token_launch_form(in
     #define LVG_TILE(ID, BM, BN, WR, WC) if (tile == ID) { \
         if (direct) hipLaunchKernelGGL((token_gemm_kernel<T, O, BM, BN, WR, WC, PL, QL, GATED, true>), grid, dim3(WR * WC * 64), 0, s, a); \
         else        hipLaunchKernelGGL((token_gemm_kernel<T, O, BM, BN, WR, WC, PL, QL, GATED, false>), grid, dim3(WR * WC * 64), 0, s, a); }
-    LVG_TILE(LVG_TILE_256, 256, 256, 2, 4)
+    LVG_TILE(LVG_TILE_256, 256, 256, 2, 2)
     LVG_TILE(LVG_TILE_128, 128, 128, 2, 2)
     LVG_TILE(LVG_TILE_64, 64, 128, 2, 2)
     #undef LVG_TILE
