@@ -31,52 +31,64 @@ struct Finish
 
 namespace {
 
-// a = act(v); with WANT also d = act'(v). Branches are uniform over the launch.
-__device__ __forceinline__ void act_value(int act, float alpha, float v, bool want, float& a, float& d)
+// 1 / (1 + exp(-v)). QUICK (results of 16 bits): the hardware's 2^x of the product's rounded value, times 1 + ln 2 * what the rounding left, and its
+// reciprocal: three units in the last place in all, where expf and a division take three times the instructions -- and the vector unit's time
+// on a tile's results is what a gated product of a short summed index waits for.
+template <bool QUICK> __device__ __forceinline__ float sigmoid(float v)
+{
+    if (!QUICK) return 1.f / (1.f + expf(-v));
+    constexpr float kLog2e = 1.44269504088896340736f, kLog2eRest = 1.92596299112661746887e-8f, kLn2 = 0.693147180559945309417f;
+    const float h = -v * kLog2e;
+    const float rest = fmaf(-v, kLog2eRest, fmaf(-v, kLog2e, -h));
+    // an exponent past the range gives infinity or zero; its rest (a NaN of infinities, too) is not looked at
+    const float e = __builtin_amdgcn_exp2f(h);
+    return __builtin_amdgcn_rcpf(1.f + (fabsf(h) < 126.f ? e * fmaf(rest, kLn2, 1.f) : e));
+}
+
+// Four values: a = act(v), d = act'(v) (where `want` is set). ACT = 0: the activation `act`, one branch for the four, uniform over the launch.
+template <int ACT, bool QUICK> __device__ __forceinline__ void act4(int act, float alpha, const float* v, bool want, float* a, float* d)
 {
     constexpr float kSeluScale = 1.0507009873554804934193349852946f, kSeluAlpha = 1.6732632423543772848170429916717f;
-    d = 1.f;
-    switch (act)
+    #define LVG_EACH _Pragma("unroll") for (int i = 0; i < 4; i++)
+    switch (ACT ? ACT : act)
     {
         case LVG_ACT_RELU:
-            // (a NaN stays one)
-            a = v <= 0.f ? 0.f : v;
-            d = v > 0.f ? 1.f : 0.f;
+            LVG_EACH { a[i] = v[i] <= 0.f ? 0.f : v[i]; d[i] = v[i] > 0.f ? 1.f : 0.f; }      // (a NaN stays one)
             break;
         case LVG_ACT_LRELU:
-            a = v > 0.f ? v : v * alpha;
-            d = v > 0.f ? 1.f : alpha;
+            LVG_EACH { a[i] = v[i] > 0.f ? v[i] : v[i] * alpha; d[i] = v[i] > 0.f ? 1.f : alpha; }
             break;
         case LVG_ACT_TANH:
-            a = tanhf(v);
-            d = fmaf(-a, a, 1.f);
+            LVG_EACH { a[i] = tanhf(v[i]); d[i] = fmaf(-a[i], a[i], 1.f); }
             break;
         case LVG_ACT_SIGMOID:
-            a = 1.f / (1.f + expf(-v));
-            d = a * (1.f - a);
+            LVG_EACH { a[i] = sigmoid<QUICK>(v[i]); d[i] = a[i] * (1.f - a[i]); }
             break;
         case LVG_ACT_ELU:
-            a = v >= 0.f ? v : expm1f(v);
-            if (want) d = v >= 0.f ? 1.f : expf(v);
+            LVG_EACH { a[i] = v[i] >= 0.f ? v[i] : expm1f(v[i]); d[i] = v[i] >= 0.f || !want ? 1.f : expf(v[i]); }
             break;
         case LVG_ACT_SELU:
-            a = v >= 0.f ? kSeluScale * v : (kSeluScale * kSeluAlpha) * expm1f(v);
-            if (want) d = v >= 0.f ? kSeluScale : (kSeluScale * kSeluAlpha) * expf(v);
+            LVG_EACH
+            {
+                a[i] = v[i] >= 0.f ? kSeluScale * v[i] : (kSeluScale * kSeluAlpha) * expm1f(v[i]);
+                d[i] = v[i] >= 0.f || !want ? kSeluScale : (kSeluScale * kSeluAlpha) * expf(v[i]);
+            }
             break;
         case LVG_ACT_SOFTPLUS:
-            a = fmaxf(v, 0.f) + log1pf(expf(-fabsf(v)));
-            if (want) d = 1.f / (1.f + expf(-v));
+            LVG_EACH { a[i] = fmaxf(v[i], 0.f) + log1pf(expf(-fabsf(v[i]))); d[i] = want ? sigmoid<QUICK>(v[i]) : 1.f; }
             break;
         case LVG_ACT_SWISH:
-        {
-            const float s = 1.f / (1.f + expf(-v));
-            a = v * s;
-            d = s * fmaf(v, 1.f - s, 1.f);
+            LVG_EACH
+            {
+                const float s = sigmoid<QUICK>(v[i]);
+                a[i] = v[i] * s;
+                d[i] = s * fmaf(v[i], 1.f - s, 1.f);
+            }
             break;
-        }
         default:
-            a = v;
+            LVG_EACH { a[i] = v[i]; d[i] = 1.f; }
     }
+    #undef LVG_EACH
 }
 
 template <class T> struct alignas(4 * sizeof(T)) Quad { T v[4]; };
@@ -138,14 +150,42 @@ template <class O, bool GATED> __device__ __forceinline__ void prepare4(const Fi
     }
 }
 
-// The results of four such sums: activation, slopes, residual, store.
-template <class O, bool GATED> __device__ __forceinline__ void finish4(const Finish& f, int64_t m, int64_t n, float* v, float* u)
+// Where four results go: the element of the first in each array.
+template <class O> struct Place
 {
-    const int64_t left = f.cols - n;
+    O*       out;
+    const O* residual;
+    float*   slopes;           // (as bytes: LVG_SLOPE_CODE)
+    int64_t  left;             // columns from it on
+    __device__ __forceinline__ Place(const Finish& f, int64_t m, int64_t n, bool gated)
+    {
+        left = f.cols - n;
+        out = static_cast<O*>(f.out) + m * f.ldo + n;
+        residual = f.residual ? static_cast<const O*>(f.residual) + m * f.ldr + n : nullptr;
+        const int64_t s = m * (gated ? 2 : 1) * f.cols + n;
+        slopes = f.slopeKind == LVG_SLOPE_F32 ? static_cast<float*>(f.slopes) + s
+               : f.slopeKind == LVG_SLOPE_CODE ? reinterpret_cast<float*>(static_cast<uint8_t*>(f.slopes) + s) : nullptr;
+    }
+    // `rows` rows on
+    __device__ __forceinline__ Place down(const Finish& f, int rows, bool gated) const
+    {
+        Place p = *this;
+        p.out += rows * f.ldo;
+        if (f.residual) p.residual += rows * f.ldr;
+        const int64_t s = rows * (gated ? 2 : 1) * f.cols;
+        if (f.slopeKind == LVG_SLOPE_F32) p.slopes += s;
+        else if (f.slopeKind == LVG_SLOPE_CODE) p.slopes = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.slopes) + s);
+        return p;
+    }
+};
+
+// The results of four such sums: activation, slopes, residual, store. ACT as in act4.
+template <class O, bool GATED, int ACT = 0> __device__ __forceinline__ void finish4(const Finish& f, const Place<O>& at, const float* v, const float* u)
+{
+    const int64_t left = at.left;
     float a[4], d[4];
     const bool want = f.slopeKind != LVG_SLOPE_NONE;
-    #pragma unroll
-    for (int i = 0; i < 4; i++) act_value(f.act, f.alpha, v[i], want, a[i], d[i]);
+    act4<ACT, sizeof(O) == 2>(f.act, f.alpha, v, want, a, d);
     if (GATED)
     {
         float up[4];
@@ -158,11 +198,10 @@ template <class O, bool GATED> __device__ __forceinline__ void finish4(const Fin
         }
         if (want)
         {
-            float* s = static_cast<float*>(f.slopes) + m * 2 * f.cols + n;
-            quad_store(s, left, f.vec, d);
-            quad_store(s + f.cols, left, f.vec, up);
+            quad_store(at.slopes, left, f.vec, d);
+            quad_store(at.slopes + f.cols, left, f.vec, up);
         }
-        quad_store(static_cast<O*>(f.out) + m * f.ldo + n, left, f.vec, a);
+        quad_store(at.out, left, f.vec, a);
         return;
     }
     uint32_t code = 0;
@@ -179,10 +218,10 @@ template <class O, bool GATED> __device__ __forceinline__ void finish4(const Fin
         // 0: no gradient, 1: alpha (lrelu's lower side; relu has alpha 0), 2: one
         code |= (uint32_t)(!inside ? 0 : (f.act != LVG_ACT_LINEAR && !(v[i] > 0.f)) ? 1 : 2) << (8 * i);
     }
-    if (f.slopeKind == LVG_SLOPE_F32) quad_store(static_cast<float*>(f.slopes) + m * f.cols + n, left, f.vec, d);
+    if (f.slopeKind == LVG_SLOPE_F32) quad_store(at.slopes, left, f.vec, d);
     else if (f.slopeKind == LVG_SLOPE_CODE)
     {
-        uint8_t* s = static_cast<uint8_t*>(f.slopes) + m * f.cols + n;
+        uint8_t* s = reinterpret_cast<uint8_t*>(at.slopes);
         if (f.vec && left >= 4) *reinterpret_cast<uint32_t*>(s) = code;
         else
         {
@@ -193,11 +232,11 @@ template <class O, bool GATED> __device__ __forceinline__ void finish4(const Fin
     if (f.residual)
     {
         float r[4];
-        quad_load(static_cast<const O*>(f.residual) + m * f.ldr + n, left, f.vec, r);
+        quad_load(at.residual, left, f.vec, r);
         #pragma unroll
         for (int i = 0; i < 4; i++) a[i] += r[i];
     }
-    quad_store(static_cast<O*>(f.out) + m * f.ldo + n, left, f.vec, a);
+    quad_store(at.out, left, f.vec, a);
 }
 
 } // namespace

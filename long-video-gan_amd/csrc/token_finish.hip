@@ -33,16 +33,16 @@ __global__ __launch_bounds__(256) void token_finish_kernel(const float* part, in
         }
     }
     prepare4<O, GATED>(f, m, n, v, u);
-    finish4<O, GATED>(f, m, n, v, u);
+    finish4<O, GATED>(f, Place<O>(f, m, n, GATED), v, u);
 }
 
-int launch_finish(const TokenArgs& a, int out_dtype, bool gated, hipStream_t s)
+int launch_finish(const float* part, int splits, int64_t ldpart, const Finish& f, int out_dtype, bool gated, hipStream_t s)
 {
-    const int64_t threads = a.fin.rows * ((a.fin.cols + 3) / 4);
+    const int64_t threads = f.rows * ((f.cols + 3) / 4);
     const dim3 grid((unsigned)lvg_ceil_div(threads, 256)), block(256);
     #define LVG_FINISH(O) { \
-        if (gated) hipLaunchKernelGGL((token_finish_kernel<O, true>), grid, block, 0, s, a.part, a.splits, a.ldpart, a.fin); \
-        else       hipLaunchKernelGGL((token_finish_kernel<O, false>), grid, block, 0, s, a.part, a.splits, a.ldpart, a.fin); }
+        if (gated) hipLaunchKernelGGL((token_finish_kernel<O, true>), grid, block, 0, s, part, splits, ldpart, f); \
+        else       hipLaunchKernelGGL((token_finish_kernel<O, false>), grid, block, 0, s, part, splits, ldpart, f); }
     if (out_dtype == LVG_F32) LVG_FINISH(float) else if (out_dtype == LVG_F16) LVG_FINISH(f16_t) else LVG_FINISH(bf16_t)
     #undef LVG_FINISH
     return lvg_check_launch("token product, adding its parts");
@@ -155,10 +155,13 @@ bool size_ok(int64_t v) { return v >= 0 && v <= (int64_t)0x7fffffff; }
 
 int64_t part_pitch(int64_t cols, bool gated) { return (cols + 3) / 4 * 4 * (gated ? 2 : 1); }
 
-int64_t work_bytes(int64_t rows, int64_t cols, int64_t inner, int dtype, bool gated)
+bool streams(int64_t rows, int form) { return rows <= kStreamRows && (form == LVG_TOKEN_FORWARD || form == LVG_TOKEN_GATED); }
+
+int64_t work_bytes(int64_t rows, int64_t cols, int64_t inner, int dtype, int form)
 {
-    const TokenPlan k = token_plan(rows, cols, inner, esize_of(dtype), gated);
-    return k.splits > 1 ? (int64_t)k.splits * rows * part_pitch(cols, gated) * 4 : 0;
+    const bool gated = form == LVG_TOKEN_GATED;
+    const int es = esize_of(dtype), splits = streams(rows, form) ? token_stream_splits(rows, cols, inner * es, gated) : token_plan(rows, cols, inner, es, gated).splits;
+    return splits > 1 ? (int64_t)splits * rows * part_pitch(cols, gated) * 4 : 0;
 }
 
 // Operands that can travel to LDS without registers: 16-byte aligned rows, offsets inside a tile below 2^32, whole chunks of columns.
@@ -172,38 +175,43 @@ bool direct_ok(const void* base, int64_t ld, int64_t count, int layout, int es, 
 // The product itself: rows x cols results over `inner`, args with operands and finish filled in.
 int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, int64_t work_size, hipStream_t s, const char* what)
 {
-    const int es = esize_of(dtype);
+    const int es = esize_of(dtype), os = esize_of(out_dtype);
     const bool gated = form == LVG_TOKEN_GATED;
-    const int64_t rows = a.qRows, cols = a.pRows;
-    const TokenPlan k = token_plan(rows, cols, a.inner, es, gated);
-    const int bm = k.tile == LVG_TILE_256 ? 256 : k.tile == LVG_TILE_128 ? 128 : 64, bn = (k.tile == LVG_TILE_256 ? 256 : 128) / (gated ? 2 : 1);
-    a.steps = (int)lvg_ceil_div(a.inner * es, 128);
-    a.stepsPerSplit = (int)lvg_ceil_div(a.steps, k.splits);
-    a.splits = k.splits;
-    a.tilesM = (int)lvg_ceil_div(rows, bm);
-    a.tilesN = lvg_ceil_div(cols, bn);
-    a.tiles = (int64_t)a.tilesM * a.tilesN;
-    a.part = nullptr;
+    const int64_t rows = a.qRows, cols = a.pRows, need = work_bytes(rows, cols, a.inner, dtype, form);
+    LVG_REQUIRE(need == 0 || (work && lvg_aligned16(work) && work_size >= need), "%s: the workspace must be 16-byte aligned and hold %lld bytes", what, (long long)need);
+    a.part = need ? static_cast<float*>(work) : nullptr;
     a.ldpart = part_pitch(cols, gated);
-    if (k.splits > 1)
-    {
-        LVG_REQUIRE(work && lvg_aligned16(work) && work_size >= work_bytes(rows, cols, a.inner, dtype, gated), "%s: the workspace must be 16-byte aligned and hold %lld bytes",
-                    what, (long long)work_bytes(rows, cols, a.inner, dtype, gated));
-        a.part = static_cast<float*>(work);
-    }
-    const int pl = form == LVG_TOKEN_ROW_GRAD || form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG, ql = form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG;
-    const bool direct = direct_ok(a.p, a.ldp, cols, pl, es, gated) && direct_ok(a.q, a.ldq, rows, ql, es, false);
     Finish& f = a.fin;
-    const int os = esize_of(out_dtype);
     auto whole = [&](const void* p, int64_t ld) { return !p || (((uintptr_t)p) % (4 * os) == 0 && ld % 4 == 0); };
     f.vec = cols % 4 == 0 && whole(f.bias, 0) && whole(f.residual, f.ldr) && whole(f.out, f.ldo) && (!f.slopes || lvg_aligned16(f.slopes));
-    int rc;
-    if (dtype == LVG_E4M3)      rc = token_launch_8bit(form, k.tile, direct, out_dtype, a, s);
-    else if (dtype == LVG_F32)  rc = token_launch_f32(form, k.tile, direct, a, s);
-    else if (dtype == LVG_F16)  rc = token_launch_f16(form, k.tile, direct, a, s);
-    else                        rc = token_launch_bf16(form, k.tile, direct, a, s);
-    if (rc != LVG_OK || k.splits <= 1) return rc;
-    return launch_finish(a, out_dtype, gated, s);
+    int rc, splits;
+    if (streams(rows, form))
+    {
+        splits = token_stream_splits(rows, cols, a.inner * es, gated);
+        StreamArgs t = {a.p, a.q, a.ldp, a.ldq, a.inner * es, rows, cols, 0, 0, a.part, a.ldpart, f};
+        t.spans = (int)lvg_ceil_div(t.bytes, 256);
+        t.spansPerSplit = (int)lvg_ceil_div(t.spans, splits);
+        rc = token_stream_launch(t, dtype, out_dtype, gated, splits, s);
+    }
+    else
+    {
+        const TokenPlan k = token_plan(rows, cols, a.inner, es, gated);
+        const int bm = k.tile == LVG_TILE_256 ? 256 : k.tile == LVG_TILE_128 ? 128 : 64, bn = (k.tile == LVG_TILE_256 ? 256 : 128) / (gated ? 2 : 1);
+        a.steps = (int)lvg_ceil_div(a.inner * es, 128);
+        a.stepsPerSplit = (int)lvg_ceil_div(a.steps, k.splits);
+        a.splits = splits = k.splits;
+        a.tilesM = (int)lvg_ceil_div(rows, bm);
+        a.tilesN = lvg_ceil_div(cols, bn);
+        a.tiles = (int64_t)a.tilesM * a.tilesN;
+        const int pl = form == LVG_TOKEN_ROW_GRAD || form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG, ql = form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG;
+        const bool direct = direct_ok(a.p, a.ldp, cols, pl, es, gated) && direct_ok(a.q, a.ldq, rows, ql, es, false);
+        if (dtype == LVG_E4M3)      rc = token_launch_8bit(form, k.tile, direct, out_dtype, a, s);
+        else if (dtype == LVG_F32)  rc = token_launch_f32(form, k.tile, direct, a, s);
+        else if (dtype == LVG_F16)  rc = token_launch_f16(form, k.tile, direct, a, s);
+        else                        rc = token_launch_bf16(form, k.tile, direct, a, s);
+    }
+    if (rc != LVG_OK || splits <= 1) return rc;
+    return launch_finish(a.part, splits, a.ldpart, f, out_dtype, gated, s);
 }
 
 } // namespace
@@ -238,7 +246,7 @@ TokenPlan token_plan(int64_t rows, int64_t cols, int64_t inner, int esize, bool 
 extern "C" int64_t lvg_linear_act_work(int64_t rows, int64_t outer, int64_t inner, int dtype, int gated)
 {
     if (!(float_type(dtype) || dtype == LVG_E4M3) || !size_ok(rows) || !size_ok(outer) || !size_ok(inner)) return LVG_ERR_INVALID;
-    return rows && outer ? work_bytes(rows, outer, inner, dtype, gated != 0) : 0;
+    return rows && outer ? work_bytes(rows, outer, inner, dtype, gated ? LVG_TOKEN_GATED : LVG_TOKEN_FORWARD) : 0;
 }
 
 extern "C" int lvg_linear_act(const void* x, const void* w, const void* b, const void* residual, const float* x_scale, const float* w_scale,
@@ -276,7 +284,7 @@ extern "C" int64_t lvg_linear_grad_work(int64_t rows, int64_t outer, int64_t inn
 {
     if (!float_type(dtype) || !size_ok(rows) || !size_ok(outer) || !size_ok(inner)) return LVG_ERR_INVALID;
     if (inner == 0 || (weight ? outer : rows) == 0) return 0;
-    return weight ? work_bytes(outer, inner, rows, dtype, false) : work_bytes(rows, inner, outer, dtype, false);
+    return weight ? work_bytes(outer, inner, rows, dtype, LVG_TOKEN_WEIGHT_GRAD) : work_bytes(rows, inner, outer, dtype, LVG_TOKEN_ROW_GRAD);
 }
 
 extern "C" int lvg_linear_grad(const void* dz, const void* other, void* grad, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,

@@ -22,8 +22,7 @@
 #pragma once
 #include "wgrad_common.h"
 #include "token_act.h"
-
-struct e4m3_t { uint8_t bits; };
+#include "token_stream.h"
 
 struct TokenArgs
 {
@@ -287,6 +286,8 @@ __device__ __forceinline__ void wave_lds_order()
 // Values that are the same for the whole workgroup, kept in scalar registers.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+template <int N> struct Const { static constexpr int value = N; };
+
 // The sums' way out: four columns of a row a lane, the same four for all rows, so what belongs to columns is loaded once.
 template <class O, bool GATED> struct Columns
 {
@@ -532,38 +533,45 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                     if (GATED) *reinterpret_cast<float4*>(at + a.ldpart / 2) = *reinterpret_cast<const float4*>(from + 128);
                 }
             }
-            else if (quick)
+            else if (n < f.cols)
             {
-                #pragma unroll
-                for (int t = 0; t < kTurns; t++)
+                const Place<O> at(f, m1, n, GATED);
+                const unsigned char* const from = out + (lane / kLanes) * kOutPitch + c * 4;
+                auto turn = [&](int t, auto act)
                 {
                     const int64_t m = m1 + t * kRows;
-                    const float4 v4 = *reinterpret_cast<const float4*>(out + (lane / kLanes + t * kRows) * kOutPitch + c * 4);
-                    if (m >= f.rows || n >= f.cols) continue;
-                    float v[4] = {v4.x, v4.y, v4.z, v4.w}, u[4];
-                    cols.apply(f, m, v, u);
-                    #pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] = v[k] * f.gain + (add ? row_load(res[t].v[k]) : 0.f);
-                    quad_store(static_cast<O*>(f.out) + m * f.ldo + n, 4, true, v);
-                }
-            }
-            else
-            {
-                #pragma unroll 1
-                for (int t = 0; t < kTurns; t++)
-                {
-                    const int64_t m = m1 + t * kRows;
-                    const unsigned char* from = out + (lane / kLanes + t * kRows) * kOutPitch + c * 4;
-                    const float4 v4 = *reinterpret_cast<const float4*>(from);
+                    const float4 v4 = *reinterpret_cast<const float4*>(from + t * kRows * kOutPitch);
                     float v[4] = {v4.x, v4.y, v4.z, v4.w}, u[4] = {0.f, 0.f, 0.f, 0.f};
                     if (GATED)
                     {
-                        const float4 u4 = *reinterpret_cast<const float4*>(from + 128);
+                        const float4 u4 = *reinterpret_cast<const float4*>(from + t * kRows * kOutPitch + 128);
                         u[0] = u4.x; u[1] = u4.y; u[2] = u4.z; u[3] = u4.w;
                     }
-                    if (m >= f.rows || n >= f.cols) continue;
+                    if (m >= f.rows) return;
                     cols.apply(f, m, v, u);
-                    finish4<O, GATED>(f, m, n, v, u);
+                    if constexpr (decltype(act)::value < 0)
+                    {
+                        #pragma unroll
+                        for (int k = 0; k < 4; k++) v[k] = v[k] * f.gain + (add ? row_load(res[t].v[k]) : 0.f);
+                        quad_store(at.down(f, t * kRows, GATED).out, 4, true, v);
+                    }
+                    else finish4<O, GATED, decltype(act)::value>(f, at.down(f, t * kRows, GATED), v, u);
+                };
+                // the usual ones unrolled, the others one turn at a time
+                if (quick)
+                {
+                    #pragma unroll
+                    for (int t = 0; t < kTurns; t++) turn(t, Const<-1>());
+                }
+                else if (f.act == (GATED ? LVG_ACT_SWISH : LVG_ACT_LRELU))
+                {
+                    #pragma unroll
+                    for (int t = 0; t < kTurns; t++) turn(t, Const<GATED ? LVG_ACT_SWISH : LVG_ACT_LRELU>());
+                }
+                else
+                {
+                    #pragma unroll 1
+                    for (int t = 0; t < kTurns; t++) turn(t, Const<0>());
                 }
             }
         }

@@ -1,5 +1,6 @@
 """What the operators on matrices of token rows (linear_act, gated_ff, rms_norm) share: views of a tensor as rows, and types."""
 
+import functools
 import math
 
 import torch
@@ -14,8 +15,9 @@ ROW_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
     """[..., width] -> [rows, width] with unit element stride: a view where the strides allow it, a copy otherwise."""
-    t = t.reshape(math.prod(t.shape[:-1]), width)
-    return t if t.stride(1) == 1 or width <= 1 else t.contiguous()
+    if t.ndim != 2:
+        t = t.reshape(math.prod(t.shape[:-1]), width)
+    return t if t.is_contiguous() or t.stride(1) == 1 or width <= 1 else t.contiguous()
 
 
 def row_stride(t: torch.Tensor) -> int:
@@ -23,12 +25,39 @@ def row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+_CODES = {torch.float32: _hip.F32, torch.float16: _hip.F16, torch.bfloat16: _hip.BF16, torch.float8_e4m3fn: E4M3}
+
+
 def type_code(dtype: torch.dtype) -> int:
-    return E4M3 if dtype == torch.float8_e4m3fn else _hip.dtype_code(dtype)
+    return _CODES[dtype]
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+@functools.lru_cache(maxsize=4096)
+def query(name: str, *args) -> int:
+    """A planning query of the library (a function of its arguments alone: workspace bytes, slot counts)."""
+    return _hip.check(getattr(_hip.lib(), name)(*args), name)
+
+
+def launch(device: torch.device, name: str, *args):
+    """The entry point `name` on the device's current stream; the launch goes to the CURRENT HIP device, so that is made the tensors' first. One
+    token's worth of work takes the GPU a few microseconds: this path avoids what costs the host as much (context managers, stream objects)."""
+    fn = getattr(_hip.lib(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():                      # pylint: disable=protected-access
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _hip.check(rc, name)
 
 
 def work_of(size: int, device: torch.device):
@@ -38,7 +67,7 @@ def work_of(size: int, device: torch.device):
 
 def column_sum(part: torch.Tensor, dtype: torch.dtype, gain: float = 1.0) -> torch.Tensor:
     """gain * part.sum(dim=0), part [slots, width] float32, on part's device and the current stream."""
-    out = torch.empty(part.shape[1], dtype=dtype, device=part.device)
-    _hip.check(_hip.lib().lvg_column_sum(part.data_ptr(), out.data_ptr(), part.shape[0], part.shape[1], gain, _hip.dtype_code(dtype), _hip.stream(part.device)),
-               'lvg_column_sum')
+    slots, width = part.shape
+    out = torch.empty(width, dtype=dtype, device=part.device)
+    launch(part.device, 'lvg_column_sum', part.data_ptr(), out.data_ptr(), slots, width, gain, _CODES[dtype])
     return out

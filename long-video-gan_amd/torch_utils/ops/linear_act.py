@@ -9,7 +9,6 @@ plain-PyTorch definition."""
 
 import torch
 
-from . import _hip
 from . import _rows
 from .bias_act import _resolve, activation_funcs
 
@@ -36,7 +35,7 @@ def linear_act(x, weight, b=None, residual=None, act='linear', alpha=None, gain=
     assert impl in ['ref', 'cuda']
     out_dtype = _check(x, weight, b, x_scale, weight_scale, out_dtype, halves=1)
     if residual is not None:
-        assert residual.shape == x.shape[:-1] + weight.shape[:1] and residual.dtype == out_dtype and residual.device == x.device
+        assert residual.shape == (*x.shape[:-1], weight.shape[0]) and residual.dtype == out_dtype and residual.device == x.device
         _no_grad_with_8bit(x, residual)
     assert act in activation_funcs
     _, alpha, gain, clamp = _resolve(act, alpha, gain, clamp)
@@ -54,23 +53,24 @@ def _no_grad_with_8bit(x, *others):
 def _check(x, weight, b, x_scale, weight_scale, out_dtype, halves):
     """Checks what the dense products share; returns the result's dtype. halves: 2 = the weight holds two projections."""
     assert isinstance(x, torch.Tensor) and isinstance(weight, torch.Tensor)
-    assert x.ndim >= 1 and weight.ndim == 2 and x.shape[-1] == weight.shape[1], f'rows of {tuple(x.shape)} do not fit a weight of {tuple(weight.shape)}'
-    assert weight.shape[0] % halves == 0
-    assert weight.dtype == x.dtype and weight.device == x.device
-    if x.dtype == torch.float8_e4m3fn:
+    assert x.ndim >= 1 and weight.ndim == 2, 'x holds rows, weight is a matrix'
+    dtype, device, (total, inner) = x.dtype, x.device, weight.shape
+    assert x.shape[-1] == inner and total % halves == 0, f'rows of {tuple(x.shape)} do not fit a weight of {tuple(weight.shape)}'
+    assert weight.dtype == dtype and weight.device == device
+    if dtype == torch.float8_e4m3fn:
         out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
         assert out_dtype in (torch.float16, torch.bfloat16), '8-bit operands give a float16 or bfloat16 result'
         assert x_scale is not None and weight_scale is not None, '8-bit operands come with their scales'
-        assert x_scale.dtype == weight_scale.dtype == torch.float32 and x_scale.device == weight_scale.device == x.device
-        assert x_scale.shape == x.shape[:-1] and weight_scale.shape == weight.shape[:1]
+        assert x_scale.dtype == weight_scale.dtype == torch.float32 and x_scale.device == weight_scale.device == device
+        assert x_scale.shape == x.shape[:-1] and weight_scale.shape == (total,)
         _no_grad_with_8bit(x, b, x_scale, weight_scale)
     else:
-        assert x.dtype in _rows.ROW_DTYPES, f'dtype {x.dtype} is not supported'
-        assert out_dtype in (None, x.dtype), 'the result has the operands\' dtype'
+        assert dtype in _rows.ROW_DTYPES, f'dtype {dtype} is not supported'
+        assert out_dtype is None or out_dtype == dtype, 'the result has the operands\' dtype'
         assert x_scale is None and weight_scale is None, 'scales belong to 8-bit operands'
-        out_dtype = x.dtype
+        out_dtype = dtype
     if b is not None:
-        assert b.shape == weight.shape[:1] and b.dtype == out_dtype and b.device == x.device
+        assert b.shape == (total,) and b.dtype == out_dtype and b.device == device
     return out_dtype
 
 
@@ -102,76 +102,80 @@ def slope_kind(act, gated):
 
 def _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype, gated, kind):
     """One product on x's device and the current stream: (y, slopes or None)."""
-    inner, halves = weight.shape[1], 2 if gated else 1
-    outer = weight.shape[0] // halves
-    y = torch.empty(x.shape[:-1] + (outer,), dtype=out_dtype, device=x.device)
+    total, inner = weight.shape
+    outer = total // 2 if gated else total
+    device = x.device
     x2, w2 = _rows.rows_of(x, inner), _rows.rows_of(weight, inner)
     rows = x2.shape[0]
+    y = torch.empty((rows, outer) if x.ndim == 2 else (*x.shape[:-1], outer), dtype=out_dtype, device=device)
     slopes = None
     if kind != SLOPE_NONE:
-        slopes = torch.empty((rows, halves * outer), dtype=torch.float32 if kind == SLOPE_F32 else torch.uint8, device=x.device)
-    if y.numel() == 0:
+        slopes = torch.empty((rows, total), dtype=torch.float32 if kind == SLOPE_F32 else torch.uint8, device=device)
+    if rows == 0 or outer == 0:
         return y, slopes
     r2 = None if residual is None else _rows.rows_of(residual, outer)
-    b = None if b is None else b.contiguous()
+    if b is not None:
+        b = b.contiguous()
     if x_scale is not None:
         x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
     code = _rows.type_code(x.dtype)
-    lib = _hip.lib()
-    with torch.cuda.device(x.device):
-        size = _hip.check(lib.lvg_linear_act_work(rows, outer, inner, code, int(gated)), 'lvg_linear_act')
-        work = _rows.work_of(size, x.device)
-        _hip.check(lib.lvg_linear_act(
-            _hip.ptr(x2), _hip.ptr(w2), _hip.ptr(b), _hip.ptr(r2), _hip.ptr(x_scale), _hip.ptr(weight_scale), y.data_ptr(), _hip.ptr(slopes), _hip.ptr(work), size,
-            rows, outer, inner, _rows.row_stride(x2), _rows.row_stride(w2), 0 if r2 is None else _rows.row_stride(r2), outer,
-            code, _hip.dtype_code(out_dtype), int(gated), activation_funcs[act].cuda_idx, kind, alpha, gain, clamp, _hip.stream(x.device)), 'lvg_linear_act')
+    size = _rows.query('lvg_linear_act_work', rows, outer, inner, code, int(gated))
+    work = _rows.work_of(size, device)
+    _rows.launch(device, 'lvg_linear_act',
+                 x2.data_ptr(), w2.data_ptr(), None if b is None else b.data_ptr(), None if r2 is None else r2.data_ptr(),
+                 None if x_scale is None else x_scale.data_ptr(), None if x_scale is None else weight_scale.data_ptr(), y.data_ptr(),
+                 None if slopes is None else slopes.data_ptr(), None if work is None else work.data_ptr(), size,
+                 rows, outer, inner, _rows.row_stride(x2), _rows.row_stride(w2), 0 if r2 is None else _rows.row_stride(r2), outer,
+                 code, _rows.type_code(out_dtype), int(gated), activation_funcs[act].cuda_idx, kind, alpha, gain, clamp)
     return y, slopes
 
 
-def _grad_product(dz, other, rows, outer, inner, weight, gain, dtype):
+def _grad_product(dz, dz_stride, other, rows, outer, inner, weight, gain, dtype):
     """dz [rows, outer] against the weight [outer, inner] (weight False) or the rows [rows, inner] (True)."""
-    grad = torch.empty((outer if weight else rows, inner), dtype=dtype, device=dz.device)
-    if grad.numel() == 0:
+    device = other.device
+    grad = torch.empty((outer if weight else rows, inner), dtype=dtype, device=device)
+    if inner == 0:
         return grad
-    lib, code = _hip.lib(), _hip.dtype_code(dtype)
-    size = _hip.check(lib.lvg_linear_grad_work(rows, outer, inner, int(weight), code), 'lvg_linear_grad')
-    work = _rows.work_of(size, dz.device)
-    _hip.check(lib.lvg_linear_grad(_hip.ptr(dz), _hip.ptr(other), grad.data_ptr(), _hip.ptr(work), size, rows, outer, inner, dz.stride(0) if rows > 1 else outer,
-                                   _rows.row_stride(other), int(weight), gain, code, _hip.stream(dz.device)), 'lvg_linear_grad')
+    code = _rows.type_code(dtype)
+    size = _rows.query('lvg_linear_grad_work', rows, outer, inner, int(weight), code)
+    work = _rows.work_of(size, device)
+    _rows.launch(device, 'lvg_linear_grad', dz.data_ptr(), other.data_ptr(), grad.data_ptr(), None if work is None else work.data_ptr(), size,
+                 rows, outer, inner, dz_stride, _rows.row_stride(other), int(weight), gain, code)
     return grad
 
 
 def _backward(dy, x, weight, slopes, kind, halves, alpha, gain, need_x, need_w, need_b):
     """Gradients of x, weight and b from dy [..., outer]; kind SLOPE_NONE: dy itself times the gain is the gradient of the sums."""
-    inner, total = weight.shape[1], weight.shape[0]
+    total, inner = weight.shape
     outer = total // halves
-    x2, w2, dy2 = _rows.rows_of(x, inner), _rows.rows_of(weight, inner), _rows.rows_of(dy, outer)
-    rows, dtype, dev = x2.shape[0], x.dtype, x.device
+    x2, w2, dz = _rows.rows_of(x, inner), _rows.rows_of(weight, inner), _rows.rows_of(dy, outer)
+    rows, dtype, device = x2.shape[0], x.dtype, x.device
+    if rows == 0 or outer == 0:
+        # nothing to sum over
+        return (x2.new_zeros(x.shape) if need_x else None, w2.new_zeros(weight.shape) if need_w else None, w2.new_zeros(total) if need_b else None)
     dx = dw = db = None
-    with torch.cuda.device(dev):
-        if rows == 0 or outer == 0:
-            # nothing to sum over
-            return (x2.new_zeros(x.shape) if need_x else None, w2.new_zeros(weight.shape) if need_w else None, w2.new_zeros(total) if need_b else None)
-        lib, code = _hip.lib(), _hip.dtype_code(dtype)
-        plain = kind == SLOPE_NONE
-        dz, part = dy2, None
+    plain, dz_stride = kind == SLOPE_NONE, _rows.row_stride(dz)
+    if not plain or need_b:
+        code = _rows.type_code(dtype)
+        slots = _rows.query('lvg_linear_slope_slots', rows, outer, halves, code)
+        part = torch.empty((slots, total), dtype=torch.float32, device=device) if need_b else None
+        into, stride = None, total
         if not plain:
             # rows of dz start at multiples of 16 bytes whatever the width: both products read them as they like it best
             each = 16 // dtype.itemsize
-            dz = torch.empty((rows, -(-total // each) * each), dtype=dtype, device=dev)
-        if not plain or need_b:
-            slots = lib.lvg_linear_slope_slots(rows, outer, halves, code)
-            if need_b:
-                part = torch.empty((slots, total), dtype=torch.float32, device=dev)
-            _hip.check(lib.lvg_linear_slope(dy2.data_ptr(), _hip.ptr(slopes), None if plain else dz.data_ptr(), _hip.ptr(part), rows, outer, _rows.row_stride(dy2),
-                                            total if plain else dz.shape[1], halves, kind, slots, alpha, 1.0 if plain else gain, code, _hip.stream(dev)), 'lvg_linear_slope')
+            stride = -(-total // each) * each
+            into = torch.empty((rows, stride), dtype=dtype, device=device)
+        _rows.launch(device, 'lvg_linear_slope', dz.data_ptr(), None if plain else slopes.data_ptr(), None if plain else into.data_ptr(),
+                     None if part is None else part.data_ptr(), rows, outer, dz_stride, stride, halves, kind, slots, alpha, 1.0 if plain else gain, code)
+        if not plain:
+            dz, dz_stride = into, stride
         if need_b:
             db = _rows.column_sum(part, dtype, gain if plain else 1.0)
-        scale = gain if plain else 1.0
-        if need_x:
-            dx = _grad_product(dz, w2, rows, total, inner, False, scale, dtype).reshape(x.shape)
-        if need_w:
-            dw = _grad_product(dz, x2, rows, total, inner, True, scale, dtype)
+    scale = gain if plain else 1.0
+    if need_x:
+        dx = _grad_product(dz, dz_stride, w2, rows, total, inner, False, scale, dtype).view(x.shape)
+    if need_w:
+        dw = _grad_product(dz, dz_stride, x2, rows, total, inner, True, scale, dtype)
     return dx, dw, db
 
 

@@ -8,7 +8,6 @@ Without weight and residual it is what the reference's mapping networks do to th
 
 import torch
 
-from . import _hip
 from . import _rows
 
 
@@ -55,11 +54,9 @@ def quantize_rows(x, impl='cuda'):
     width = x.shape[-1]
     q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    if x.numel():
-        x2 = _rows.rows_of(x, width)
-        with torch.cuda.device(x.device):
-            _hip.check(_hip.lib().lvg_quantize_rows(x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], width, _rows.row_stride(x2),
-                                                    _hip.dtype_code(x.dtype), _hip.stream(x.device)), 'lvg_quantize_rows')
+    x2 = _rows.rows_of(x, width)
+    if x2.shape[0]:
+        _rows.launch(x.device, 'lvg_quantize_rows', x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], width, _rows.row_stride(x2), _rows.type_code(x.dtype))
     return q, scale
 
 
@@ -94,11 +91,11 @@ def _forward(x, weight, residual, eps, quantize, keep):
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep else None
     if rows:
         r2 = None if residual is None else _rows.rows_of(residual, width)
-        weight = None if weight is None else weight.contiguous()
-        with torch.cuda.device(x.device):
-            _hip.check(_hip.lib().lvg_rms_norm(x2.data_ptr(), _hip.ptr(r2), _hip.ptr(weight), y.data_ptr(), _hip.ptr(total), _hip.ptr(rstd), _hip.ptr(scale),
-                                               rows, width, _rows.row_stride(x2), 0 if r2 is None else _rows.row_stride(r2), eps, _hip.dtype_code(x.dtype),
-                                               int(quantize), _hip.stream(x.device)), 'lvg_rms_norm')
+        if weight is not None:
+            weight = weight.contiguous()
+        _rows.launch(x.device, 'lvg_rms_norm', x2.data_ptr(), None if r2 is None else r2.data_ptr(), None if weight is None else weight.data_ptr(), y.data_ptr(),
+                     None if total is None else total.data_ptr(), None if rstd is None else rstd.data_ptr(), None if scale is None else scale.data_ptr(),
+                     rows, width, _rows.row_stride(x2), 0 if r2 is None else _rows.row_stride(r2), eps, _rows.type_code(x.dtype), int(quantize))
     return y, scale, total, rstd
 
 
@@ -129,15 +126,15 @@ class _RmsNorm(torch.autograd.Function):
             dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
             if rows == 0:
                 return dx, torch.zeros_like(weight) if need_w else None, dx if need_r else None, None
-            lib, code = _hip.lib(), _hip.dtype_code(s.dtype)
-            with torch.cuda.device(dev):
-                slots = lib.lvg_rms_norm_backward_slots(rows, width, code)
-                part = torch.empty((slots, width), dtype=torch.float32, device=dev) if need_w else None
-                row_work = torch.empty(rows, dtype=torch.float32, device=dev)
-                weight = None if weight is None else weight.contiguous()
-                _hip.check(lib.lvg_rms_norm_backward(dy2.data_ptr(), _hip.ptr(ds2), s2.data_ptr(), _hip.ptr(weight), rstd.data_ptr(), dx.data_ptr(), _hip.ptr(part),
-                                                     row_work.data_ptr(), rows, width, _rows.row_stride(dy2), 0 if ds2 is None else _rows.row_stride(ds2),
-                                                     _rows.row_stride(s2), slots, code, _hip.stream(dev)), 'lvg_rms_norm_backward')
-                if need_w:
-                    dw = _rows.column_sum(part, s.dtype)
+            code = _rows.type_code(s.dtype)
+            slots = _rows.query('lvg_rms_norm_backward_slots', rows, width, code)
+            part = torch.empty((slots, width), dtype=torch.float32, device=dev) if need_w else None
+            row_work = torch.empty(rows, dtype=torch.float32, device=dev)
+            if weight is not None:
+                weight = weight.contiguous()
+            _rows.launch(dev, 'lvg_rms_norm_backward', dy2.data_ptr(), None if ds2 is None else ds2.data_ptr(), s2.data_ptr(), None if weight is None else weight.data_ptr(),
+                         rstd.data_ptr(), dx.data_ptr(), None if part is None else part.data_ptr(), row_work.data_ptr(), rows, width, _rows.row_stride(dy2),
+                         0 if ds2 is None else _rows.row_stride(ds2), _rows.row_stride(s2), slots, code)
+            if need_w:
+                dw = _rows.column_sum(part, s.dtype)
         return dx if need_x else None, dw, dx if need_r else None, None

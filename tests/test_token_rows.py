@@ -262,7 +262,7 @@ def test_refusals_of_the_c_entries_cpu():
 
 # rows, inner, outer: single values, less than a fragment, odd widths, one more than a tile, a summed index of one and of many steps (split over
 # the chip), and results of several tiles of every size
-SIZES = [(1, 1, 1), (1, 64, 64), (2, 7, 3), (3, 515, 5), (16, 1024, 96), (17, 130, 67), (33, 256, 128), (64, 2048, 16), (65, 63, 129), (129, 257, 515), (300, 64, 1000), (20, 9000, 40)]
+SIZES = [(1, 1, 1), (1, 64, 64), (2, 7, 3), (3, 515, 5), (16, 1024, 96), (17, 130, 67), (33, 256, 128), (64, 2048, 16), (65, 63, 129), (129, 257, 515), (300, 64, 1000), (20, 9000, 40), (40, 9000, 40)]
 BIG = [(2100, 192, 2304), (1025, 200, 4113)]
 
 
@@ -288,7 +288,7 @@ def test_linear_activations_gpu(act, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('size', [(1, 1, 1), (1, 64, 64), (3, 515, 5), (17, 130, 67), (33, 256, 128), (129, 257, 260), (20, 9000, 40), (1030, 136, 2100)])
+@pytest.mark.parametrize('size', [(1, 1, 1), (1, 64, 64), (3, 515, 5), (17, 130, 67), (33, 256, 128), (129, 257, 260), (20, 9000, 40), (40, 9000, 40), (1030, 136, 2100)])
 def test_gated_forward_and_gradients_gpu(size, dtype):
     m, k, n = size
     x, w = rand(m, k, seed=1, dtype=dtype), rand(2 * n, k, seed=2, dtype=dtype, scale=k ** -0.5)
