@@ -238,48 +238,66 @@ __global__ __launch_bounds__(256) void rms_norm_wide_kernel(NormArgs p)
 }
 
 // Gradient: a workgroup takes rows blockIdx.x, + gridDim.x, ... (W == 1: its four waves a row each) and keeps the weight's gradient of its
-// rows in registers; the four waves' sums meet in LDS in wave order and go to part[blockIdx.x][width].
+// rows in registers; the four waves' sums meet in LDS in wave order and go to part[blockIdx.x][width]. The next row's three vectors are asked
+// for before this one's are used (NV <= 4: they fit the registers), so that memory does not wait for the row's reduction.
 template <class T, int W, int NV>
 __global__ __launch_bounds__(256) void rms_norm_back_kernel(NormBackArgs p)
 {
     constexpr int V = Elem<T>::kVec;
+    constexpr bool kAhead = NV <= 4;
     __shared__ float sums[2][4];
     __shared__ float cols[W == 1 ? 64 * V : 1];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int t = W == 1 ? lane : (int)threadIdx.x;
-    float dw[NV][V];
+    float dw[NV][V], w[NV][V];
     #pragma unroll
     for (int j = 0; j < NV; j++)
+    {
+        const int64_t at = (int64_t)(j * 64 * W + t) * V;
         #pragma unroll
-        for (int i = 0; i < V; i++) dw[j][i] = 0.f;
-    const int64_t step = (int64_t)gridDim.x * (W == 1 ? 4 : 1);
-    int turn = 0;
-    for (int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x; row < p.rows; row += step, turn ^= 1)
+        for (int i = 0; i < V; i++) { dw[j][i] = 0.f; w[j][i] = 1.f; }
+        if (kAhead && p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w[j]);
+    }
+    struct Row { RawRow<T> g[NV], s[NV], d[NV]; float r; };
+    auto load = [&](Row& x, int64_t row)
     {
         const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
         const T* s = static_cast<const T*>(p.s) + row * p.lds;
-        const float r = p.rstd[row];
-        float g[NV][V], sv[NV][V];
+        const T* ds = static_cast<const T*>(p.ds) + row * p.ldds;
+        x.r = p.rstd[row];
         #pragma unroll
         for (int j = 0; j < NV; j++)
         {
             const int64_t at = (int64_t)(j * 64 * W + t) * V;
-            load_row<T>(dy + at, p.width - at, g[j]);
-            load_row<T>(s + at, p.width - at, sv[j]);
+            x.g[j] = load_raw<T>(dy + at, p.width - at);
+            x.s[j] = load_raw<T>(s + at, p.width - at);
+            if (p.ds) x.d[j] = load_raw<T>(ds + at, p.width - at);
         }
+    };
+    const int64_t step = (int64_t)gridDim.x * (W == 1 ? 4 : 1);
+    int turn = 0;
+    int64_t row = W == 1 ? (int64_t)blockIdx.x * 4 + wave : (int64_t)blockIdx.x;
+    Row now, next;
+    if (row < p.rows) load(now, row);
+    for (; row < p.rows; row += step, turn ^= 1)
+    {
+        if (kAhead && row + step < p.rows) load(next, row + step);
+        const float r = now.r;
         float dot = 0.f;
         #pragma unroll
         for (int j = 0; j < NV; j++)
         {
-            const int64_t at = (int64_t)(j * 64 * W + t) * V;
-            float w[V];
-            if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w);
+            if (!kAhead && p.weight)
+            {
+                const int64_t at = (int64_t)(j * 64 * W + t) * V;
+                load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w[j]);
+            }
             #pragma unroll
             for (int i = 0; i < V; i++)
             {
-                dw[j][i] = fmaf(g[j][i], sv[j][i] * r, dw[j][i]);
-                if (p.weight) g[j][i] *= w[i];
-                dot = fmaf(g[j][i], sv[j][i], dot);
+                const float g = row_load(now.g[j].v[i]), s = row_load(now.s[j].v[i]);
+                dw[j][i] = fmaf(g, s * r, dw[j][i]);
+                dot = fmaf(g * w[j][i], s, dot);
             }
         }
         dot = row_total<W>(dot, sums[turn], wave);         // (two sets: a wave may reach the next row's while another still reads this one's)
@@ -288,12 +306,17 @@ __global__ __launch_bounds__(256) void rms_norm_back_kernel(NormBackArgs p)
         for (int j = 0; j < NV; j++)
         {
             const int64_t at = (int64_t)(j * 64 * W + t) * V;
-            float d[V];
-            if (p.ds) load_row<T>(static_cast<const T*>(p.ds) + row * p.ldds + at, p.width - at, d);
+            float v[V];
             #pragma unroll
-            for (int i = 0; i < V; i++) g[j][i] = fmaf(g[j][i], r, -c * sv[j][i]) + (p.ds ? d[i] : 0.f);
-            store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, p.width - at, g[j]);
+            for (int i = 0; i < V; i++)
+            {
+                v[i] = fmaf(row_load(now.g[j].v[i]) * w[j][i], r, -c * row_load(now.s[j].v[i]));
+                if (p.ds) v[i] += row_load(now.d[j].v[i]);
+            }
+            store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, p.width - at, v);
         }
+        if (kAhead) now = next;
+        else if (row + step < p.rows) load(now, row + step);
     }
     if (!p.part) return;
     float* out = p.part + (int64_t)blockIdx.x * p.width;
@@ -380,22 +403,25 @@ __global__ __launch_bounds__(256) void rms_norm_back_wide_kernel(NormBackArgs p)
     }
 }
 
-// out[c] = sum over the slots of part[slot][c]: 64 columns a workgroup, its 4 waves take every fourth slot and add in wave order.
+// out[c] = sum over the slots of part[slot][c]: 32 columns a workgroup, its 8 rows of threads take every eighth slot and add in their order.
 template <class T>
 __global__ __launch_bounds__(256) void column_sum_kernel(const float* part, T* out, int slots, int64_t width, float gain)
 {
-    __shared__ float sums[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    __shared__ float sums[8][32];
+    const int group = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     float v = 0.f;
     if (c < width)
     {
-        #pragma unroll 4
-        for (int s = wave; s < slots; s += 4) v += part[(int64_t)s * width + c];
+        #pragma unroll 8
+        for (int s = group; s < slots; s += 8) v += part[(int64_t)s * width + c];
     }
-    sums[wave][lane] = v;
+    sums[group][lane] = v;
     __syncthreads();
-    if (wave == 0 && c < width) out[c] = from_acc<T>((((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]) * gain);
+    if (group != 0 || c >= width) return;
+    #pragma unroll
+    for (int g = 1; g < 8; g++) v += sums[g][lane];
+    out[c] = from_acc<T>(v * gain);
 }
 
 int esize(int dtype) { return dtype == LVG_F32 ? 4 : 2; }
@@ -439,11 +465,22 @@ template <class T, bool QUANT, bool NORM> void launch_norm(const NormArgs& a, co
     }
 }
 
+// The gradient keeps more of a row (its three vectors twice and the weight's gradient): a wave a row only as long as a lane holds it in one vector.
+Plan back_plan(int64_t width, int dtype)
+{
+    const int64_t vecs = lvg_ceil_div(width, 16 / esize(dtype));
+    if (vecs <= 64) return {1, 1};
+    for (int nv : {1, 2, 4}) if (vecs <= 256 * nv) return {4, nv};
+    // (eight vectors of 16-bit values would not fit)
+    return dtype == LVG_F32 && vecs <= 2048 ? Plan{4, 8} : Plan{0, 0};
+}
+
 template <class T> void launch_back(const NormBackArgs& a, const Plan& k, int slots, hipStream_t s)
 {
     const dim3 block(256), grid((unsigned)slots);
     #define LVG_ROW(W, NV) if (k.waves == W && k.vecs == NV) { hipLaunchKernelGGL((rms_norm_back_kernel<T, W, NV>), grid, block, 0, s, a); return; }
-    LVG_ROW(1, 1) LVG_ROW(1, 2) LVG_ROW(1, 4) LVG_ROW(1, 8) LVG_ROW(4, 4) LVG_ROW(4, 8)
+    LVG_ROW(1, 1) LVG_ROW(4, 1) LVG_ROW(4, 2) LVG_ROW(4, 4)
+    if constexpr (sizeof(T) == 4) { LVG_ROW(4, 8) }
     #undef LVG_ROW
     hipLaunchKernelGGL(rms_norm_back_coef_kernel<T>, dim3((unsigned)a.rows), block, 0, s, a);
     hipLaunchKernelGGL(rms_norm_back_wide_kernel<T>, dim3((unsigned)lvg_ceil_div(a.width, 256 * Elem<T>::kVec), (unsigned)slots), block, 0, s, a);
@@ -453,10 +490,10 @@ bool rows_ok(int64_t rows, int64_t width) { return rows >= 0 && rows <= 0x7fffff
 
 int back_slots(int64_t rows, int64_t width, int dtype)
 {
-    const Plan k = plan(width, dtype);
-    // about two workgroups for each of the 256 compute units
-    if (k.waves == 1) return (int)std::min<int64_t>(512, lvg_ceil_div(rows, 4));
-    if (k.waves == 4) return (int)std::min<int64_t>(512, rows);
+    const Plan k = back_plan(width, dtype);
+    // two or four workgroups for each of the 256 compute units: what they write of the weight's gradient is read again
+    if (k.waves == 1) return (int)std::min<int64_t>(1024, lvg_ceil_div(rows, 4));
+    if (k.waves == 4) return (int)std::min<int64_t>(k.vecs == 1 ? 1024 : 768, rows);
     return (int)std::min<int64_t>(64, rows);
 }
 
@@ -507,7 +544,7 @@ extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const voi
     LVG_REQUIRE(row_type(dtype), "lvg_rms_norm_backward: float32 / float16 / bfloat16 only (dtype %d)", dtype);
     LVG_REQUIRE(rows_ok(rows, width), "lvg_rms_norm_backward: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
     if (rows == 0) return LVG_OK;
-    const Plan k = plan(width, dtype);
+    const Plan k = back_plan(width, dtype);
     LVG_REQUIRE(dy && s_in && rstd && dx && (k.waves || row_work), "lvg_rms_norm_backward: missing pointer");
     LVG_REQUIRE(k.waves || rows <= kLaunchRows, "lvg_rms_norm_backward: more than %lld rows of %lld values", (long long)kLaunchRows, (long long)width);
     LVG_REQUIRE(dy_stride >= 0 && dsum_stride >= 0 && s_stride >= 0, "lvg_rms_norm_backward: negative row stride");
@@ -526,7 +563,7 @@ extern "C" int lvg_column_sum(const float* part, void* out, int slots, int64_t w
     LVG_REQUIRE(slots >= 0 && width >= 0 && width <= ((int64_t)1 << 36), "lvg_column_sum: bad size");
     if (width == 0) return LVG_OK;
     LVG_REQUIRE((part || slots == 0) && out, "lvg_column_sum: missing pointer");
-    const dim3 grid((unsigned)lvg_ceil_div(width, 64)), block(256);
+    const dim3 grid((unsigned)lvg_ceil_div(width, 32)), block(256);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) hipLaunchKernelGGL(column_sum_kernel<float>, grid, block, 0, s, part, static_cast<float*>(out), slots, width, gain);
     else if (dtype == LVG_F16) hipLaunchKernelGGL(column_sum_kernel<f16_t>, grid, block, 0, s, part, static_cast<f16_t*>(out), slots, width, gain);

@@ -33,6 +33,22 @@ template <class T> __device__ __forceinline__ void load_row(const T* p, int64_t 
     }
 }
 
+// The same in two steps, for loads that are to be on their way early: the raw vector, then its values.
+template <class T> struct RawRow { T v[Elem<T>::kVec]; };
+template <class T> __device__ __forceinline__ RawRow<T> load_raw(const T* p, int64_t n)
+{
+    constexpr int V = Elem<T>::kVec;
+    RawRow<T> r;
+    if (n >= V) __builtin_memcpy(&r, p, 16);
+    else
+    {
+        __builtin_memset(&r, 0, 16);
+        #pragma unroll
+        for (int i = 0; i < V; i++) if (i < n) r.v[i] = p[i];
+    }
+    return r;
+}
+
 template <class T> __device__ __forceinline__ void store_row(T* p, int64_t n, const float* v)
 {
     constexpr int V = Elem<T>::kVec;

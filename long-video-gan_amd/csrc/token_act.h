@@ -121,6 +121,13 @@ template <class T> __device__ __forceinline__ void quad_store(T* p, int64_t n, b
     }
 }
 
+template <class O> __device__ __forceinline__ void residual4(const Finish& f, int64_t m, int64_t n, float* r)
+{
+    #pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = 0.f;
+    if (f.residual) quad_load(static_cast<const O*>(f.residual) + m * f.ldr + n, f.cols - n, f.vec, r);
+}
+
 // Four neighbouring sums, row m, columns n .. n + 3 (those below cols): scales and bias. v: sums; gated: v of the gate half, u of the up half.
 template <class O, bool GATED> __device__ __forceinline__ void prepare4(const Finish& f, int64_t m, int64_t n, float* v, float* u)
 {
@@ -154,14 +161,12 @@ template <class O, bool GATED> __device__ __forceinline__ void prepare4(const Fi
 template <class O> struct Place
 {
     O*       out;
-    const O* residual;
     float*   slopes;           // (as bytes: LVG_SLOPE_CODE)
     int64_t  left;             // columns from it on
     __device__ __forceinline__ Place(const Finish& f, int64_t m, int64_t n, bool gated)
     {
         left = f.cols - n;
         out = static_cast<O*>(f.out) + m * f.ldo + n;
-        residual = f.residual ? static_cast<const O*>(f.residual) + m * f.ldr + n : nullptr;
         const int64_t s = m * (gated ? 2 : 1) * f.cols + n;
         slopes = f.slopeKind == LVG_SLOPE_F32 ? static_cast<float*>(f.slopes) + s
                : f.slopeKind == LVG_SLOPE_CODE ? reinterpret_cast<float*>(static_cast<uint8_t*>(f.slopes) + s) : nullptr;
@@ -171,7 +176,6 @@ template <class O> struct Place
     {
         Place p = *this;
         p.out += rows * f.ldo;
-        if (f.residual) p.residual += rows * f.ldr;
         const int64_t s = rows * (gated ? 2 : 1) * f.cols;
         if (f.slopeKind == LVG_SLOPE_F32) p.slopes += s;
         else if (f.slopeKind == LVG_SLOPE_CODE) p.slopes = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.slopes) + s);
@@ -179,13 +183,13 @@ template <class O> struct Place
     }
 };
 
-// The results of four such sums: activation, slopes, residual, store. ACT as in act4.
-template <class O, bool GATED, int ACT = 0> __device__ __forceinline__ void finish4(const Finish& f, const Place<O>& at, const float* v, const float* u)
+// The results of four such sums: activation, slopes, residual (four values, or NULL), store.
+template <class O, bool GATED> __device__ __forceinline__ void finish4(const Finish& f, const Place<O>& at, const float* v, const float* u, const float* residual)
 {
     const int64_t left = at.left;
     float a[4], d[4];
     const bool want = f.slopeKind != LVG_SLOPE_NONE;
-    act4<ACT, sizeof(O) == 2>(f.act, f.alpha, v, want, a, d);
+    act4<0, sizeof(O) == 2>(f.act, f.alpha, v, want, a, d);
     if (GATED)
     {
         float up[4];
@@ -229,12 +233,10 @@ template <class O, bool GATED, int ACT = 0> __device__ __forceinline__ void fini
             for (int i = 0; i < 4; i++) if (i < left) s[i] = (uint8_t)(code >> (8 * i));
         }
     }
-    if (f.residual)
+    if (residual)
     {
-        float r[4];
-        quad_load(at.residual, left, f.vec, r);
         #pragma unroll
-        for (int i = 0; i < 4; i++) a[i] += r[i];
+        for (int i = 0; i < 4; i++) a[i] += residual[i];
     }
     quad_store(at.out, left, f.vec, a);
 }

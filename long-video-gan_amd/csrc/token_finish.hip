@@ -33,7 +33,9 @@ __global__ __launch_bounds__(256) void token_finish_kernel(const float* part, in
         }
     }
     prepare4<O, GATED>(f, m, n, v, u);
-    finish4<O, GATED>(f, Place<O>(f, m, n, GATED), v, u);
+    float r[4];
+    residual4<O>(f, m, n, r);
+    finish4<O, GATED>(f, Place<O>(f, m, n, GATED), v, u, r);
 }
 
 int launch_finish(const float* part, int splits, int64_t ldpart, const Finish& f, int out_dtype, bool gated, hipStream_t s)
@@ -58,93 +60,115 @@ struct SlopeArgs
     void*       dz;            // or NULL: column sums alone
     float*      part;          // [gridDim.y][halves * cols], or NULL
     int64_t     rows, cols, lddy, lddz;
-    int         halves, kind;
+    int         kind;
     int         lanes;         // threads of a workgroup along the columns, a power of two
     float       alpha, gain;
 };
 
-template <class T>
+// A thread owns one vector of columns (gated: of both halves, dy is read once) and takes its rows four at a time, all loads first.
+template <class T, int H>
 __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
 {
-    constexpr int V = Elem<T>::kVec;
+    constexpr int V = Elem<T>::kVec, R = 4;
     __shared__ float sums[256][V + 1];
     const int tid = threadIdx.x, cl = tid & (p.lanes - 1), rl = tid / p.lanes, rstep = 256 / p.lanes;
-    const int64_t per = (p.cols + V - 1) / V;                          // vectors of one half
-    const int64_t vi = (int64_t)blockIdx.x * p.lanes + cl;
-    const int half = vi >= per ? 1 : 0;
-    const int64_t n = (vi - half * per) * V, left = vi < per * p.halves ? p.cols - n : 0;
+    const int64_t n = ((int64_t)blockIdx.x * p.lanes + cl) * V, left = p.cols - n;
     const int64_t chunk = (p.rows + gridDim.y - 1) / gridDim.y;
     const int64_t r0 = chunk * blockIdx.y, r1 = min(r0 + chunk, p.rows);
-    float db[V];
+    float db[H][V];
     #pragma unroll
-    for (int i = 0; i < V; i++) db[i] = 0.f;
-    if (left > 0)
+    for (int h = 0; h < H; h++)
+        #pragma unroll
+        for (int i = 0; i < V; i++) db[h][i] = 0.f;
+    for (int64_t m0 = r0 + rl; left > 0 && m0 < r1; m0 += R * rstep)
     {
-        for (int64_t m = r0 + rl; m < r1; m += rstep)
+        RawRow<T> g[R];
+        RawRow<float> d[R][H][V / 4];
+        uint8_t c[R][V];
+        #pragma unroll
+        for (int r = 0; r < R; r++)
         {
-            float g[V];
-            load_row<T>(static_cast<const T*>(p.dy) + m * p.lddy + n, left, g);
-            const int64_t at = (m * p.halves + half) * p.cols + n;
+            const int64_t m = m0 + r * rstep;
+            if (m >= r1) continue;
+            g[r] = load_raw<T>(static_cast<const T*>(p.dy) + m * p.lddy + n, left);
             if (p.kind == LVG_SLOPE_F32)
             {
-                const float* s = static_cast<const float*>(p.slopes) + at;
                 #pragma unroll
-                for (int k = 0; k < V; k += 4)
-                {
-                    float d[4];
-                    load_row<float>(s + k, left - k, d);
+                for (int h = 0; h < H; h++)
                     #pragma unroll
-                    for (int i = 0; i < 4; i++) g[k + i] *= d[i];
-                }
+                    for (int k = 0; k < V / 4; k++) d[r][h][k] = load_raw<float>(static_cast<const float*>(p.slopes) + (m * H + h) * p.cols + n + 4 * k, left - 4 * k);
             }
             else if (p.kind == LVG_SLOPE_CODE)
             {
-                const uint8_t* s = static_cast<const uint8_t*>(p.slopes) + at;
-                uint8_t c[V];
-                if (left >= V) __builtin_memcpy(c, s, V);
+                const uint8_t* s = static_cast<const uint8_t*>(p.slopes) + m * p.cols + n;
+                if (left >= V) __builtin_memcpy(c[r], s, V);
                 else
                 {
                     #pragma unroll
-                    for (int i = 0; i < V; i++) c[i] = i < left ? s[i] : (uint8_t)0;
+                    for (int i = 0; i < V; i++) c[r][i] = i < left ? s[i] : (uint8_t)0;
                 }
-                #pragma unroll
-                for (int i = 0; i < V; i++) g[i] = c[i] == 2 ? g[i] : c[i] == 1 ? g[i] * p.alpha : 0.f;
             }
+        }
+        #pragma unroll
+        for (int r = 0; r < R; r++)
+        {
+            const int64_t m = m0 + r * rstep;
+            if (m >= r1) continue;
             #pragma unroll
-            for (int i = 0; i < V; i++) { g[i] *= p.gain; db[i] += g[i]; }
-            if (p.dz) store_row<T>(static_cast<T*>(p.dz) + m * p.lddz + half * p.cols + n, left, g);
+            for (int h = 0; h < H; h++)
+            {
+                float v[V];
+                #pragma unroll
+                for (int i = 0; i < V; i++)
+                {
+                    v[i] = row_load(g[r].v[i]);
+                    if (p.kind == LVG_SLOPE_F32) v[i] *= d[r][h][i / 4].v[i % 4];
+                    else if (p.kind == LVG_SLOPE_CODE) v[i] = c[r][i] == 2 ? v[i] : c[r][i] == 1 ? v[i] * p.alpha : 0.f;
+                    v[i] *= p.gain;
+                    db[h][i] += v[i];
+                }
+                if (p.dz) store_row<T>(static_cast<T*>(p.dz) + m * p.lddz + h * p.cols + n, left, v);
+            }
         }
     }
     if (!p.part) return;
     #pragma unroll
-    for (int i = 0; i < V; i++) sums[tid][i] = db[i];
-    __syncthreads();
-    if (rl == 0 && left > 0)
+    for (int h = 0; h < H; h++)
     {
-        for (int k = 1; k < rstep; k++)
-        {
-            #pragma unroll
-            for (int i = 0; i < V; i++) db[i] += sums[k * p.lanes + cl][i];
-        }
-        float* out = p.part + (int64_t)blockIdx.y * p.halves * p.cols + half * p.cols + n;
+        __syncthreads();
         #pragma unroll
-        for (int i = 0; i < V; i++) if (i < left) out[i] = db[i];
+        for (int i = 0; i < V; i++) sums[tid][i] = db[h][i];
+        __syncthreads();
+        if (rl == 0 && left > 0)
+        {
+            float v[V];
+            #pragma unroll
+            for (int i = 0; i < V; i++) v[i] = db[h][i];
+            for (int k = 1; k < rstep; k++)
+            {
+                #pragma unroll
+                for (int i = 0; i < V; i++) v[i] += sums[k * p.lanes + cl][i];
+            }
+            float* out = p.part + ((int64_t)blockIdx.y * H + h) * p.cols + n;
+            #pragma unroll
+            for (int i = 0; i < V; i++) if (i < left) out[i] = v[i];
+        }
     }
 }
 
-int slope_lanes(int64_t cols, int halves, int esize)
+int slope_lanes(int64_t cols, int esize)
 {
-    const int64_t vecs = lvg_ceil_div(cols, 16 / esize) * halves;
+    const int64_t vecs = lvg_ceil_div(cols, 16 / esize);
     int lanes = 1;
     while (lanes < 256 && lanes < vecs) lanes *= 2;
     return lanes;
 }
 
 // Row chunks: about eight workgroups for each compute unit, at least four rows a thread.
-int slope_slots(int64_t rows, int64_t cols, int halves, int esize)
+int slope_slots(int64_t rows, int64_t cols, int esize)
 {
-    const int lanes = slope_lanes(cols, halves, esize);
-    const int64_t across = lvg_ceil_div(lvg_ceil_div(cols, 16 / esize) * halves, lanes);
+    const int lanes = slope_lanes(cols, esize);
+    const int64_t across = lvg_ceil_div(lvg_ceil_div(cols, 16 / esize), lanes);
     const int64_t most = lvg_ceil_div(rows, 4 * (256 / lanes));
     return (int)std::max<int64_t>(1, std::min<int64_t>(most, std::max<int64_t>(1, 2048 / across)));
 }
@@ -201,8 +225,9 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
         a.stepsPerSplit = (int)lvg_ceil_div(a.steps, k.splits);
         a.splits = splits = k.splits;
         a.tilesM = (int)lvg_ceil_div(rows, bm);
-        a.tilesN = lvg_ceil_div(cols, bn);
-        a.tiles = (int64_t)a.tilesM * a.tilesN;
+        a.tilesN = (int)lvg_ceil_div(cols, bn);
+        LVG_REQUIRE((int64_t)a.tilesM * a.tilesN <= ((int64_t)1 << 22), "%s: a result of %lld x %lld", what, (long long)rows, (long long)cols);
+        a.tiles = a.tilesM * a.tilesN;
         const int pl = form == LVG_TOKEN_ROW_GRAD || form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG, ql = form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG;
         const bool direct = direct_ok(a.p, a.ldp, cols, pl, es, gated) && direct_ok(a.q, a.ldq, rows, ql, es, false);
         if (dtype == LVG_E4M3)      rc = token_launch_8bit(form, k.tile, direct, out_dtype, a, s);
@@ -310,7 +335,7 @@ extern "C" int lvg_linear_grad(const void* dz, const void* other, void* grad, vo
 extern "C" int lvg_linear_slope_slots(int64_t rows, int64_t outer, int halves, int dtype)
 {
     if (!float_type(dtype) || !size_ok(rows) || !size_ok(outer) || rows == 0 || outer == 0 || (halves != 1 && halves != 2)) return 0;
-    return slope_slots(rows, outer, halves, esize_of(dtype));
+    return slope_slots(rows, outer, esize_of(dtype));
 }
 
 extern "C" int lvg_linear_slope(const void* dy, const void* slopes, void* dz, float* db_part, int64_t rows, int64_t outer, int64_t dy_stride, int64_t dz_stride,
@@ -322,12 +347,14 @@ extern "C" int lvg_linear_slope(const void* dy, const void* slopes, void* dz, fl
     LVG_REQUIRE(dy && (dz || db_part), "lvg_linear_slope: missing pointer");
     LVG_REQUIRE(slope_kind == LVG_SLOPE_NONE ? halves == 1 : (slopes && (slope_kind == LVG_SLOPE_F32 || (slope_kind == LVG_SLOPE_CODE && halves == 1))), "lvg_linear_slope: bad slopes");
     LVG_REQUIRE(dy_stride >= 0 && (!dz || dz_stride >= outer * halves), "lvg_linear_slope: bad row stride");
-    LVG_REQUIRE(slots == slope_slots(rows, outer, halves, esize_of(dtype)), "lvg_linear_slope: slots must be lvg_linear_slope_slots(...)");
-    SlopeArgs a = {dy, slopes, dz, db_part, rows, outer, dy_stride, dz_stride, halves, slope_kind, slope_lanes(outer, halves, esize_of(dtype)), alpha, gain};
-    const dim3 grid((unsigned)lvg_ceil_div(lvg_ceil_div(outer, 16 / esize_of(dtype)) * halves, a.lanes), (unsigned)slots), block(256);
+    LVG_REQUIRE(slots == slope_slots(rows, outer, esize_of(dtype)), "lvg_linear_slope: slots must be lvg_linear_slope_slots(...)");
+    SlopeArgs a = {dy, slopes, dz, db_part, rows, outer, dy_stride, dz_stride, slope_kind, slope_lanes(outer, esize_of(dtype)), alpha, gain};
+    const dim3 grid((unsigned)lvg_ceil_div(lvg_ceil_div(outer, 16 / esize_of(dtype)), a.lanes), (unsigned)slots), block(256);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (dtype == LVG_F32) hipLaunchKernelGGL(token_slope_kernel<float>, grid, block, 0, s, a);
-    else if (dtype == LVG_F16) hipLaunchKernelGGL(token_slope_kernel<f16_t>, grid, block, 0, s, a);
-    else hipLaunchKernelGGL(token_slope_kernel<bf16_t>, grid, block, 0, s, a);
+    #define LVG_TYPE(T) { \
+        if (halves == 2) hipLaunchKernelGGL((token_slope_kernel<T, 2>), grid, block, 0, s, a); \
+        else             hipLaunchKernelGGL((token_slope_kernel<T, 1>), grid, block, 0, s, a); }
+    if (dtype == LVG_F32) LVG_TYPE(float) else if (dtype == LVG_F16) LVG_TYPE(f16_t) else LVG_TYPE(bf16_t)
+    #undef LVG_TYPE
     return lvg_check_launch("lvg_linear_slope");
 }

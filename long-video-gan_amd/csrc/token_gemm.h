@@ -32,9 +32,7 @@ struct TokenArgs
     int64_t     inner;         // summed index
     int64_t     pRows, qRows;  // columns / rows of the result (gated: pRows of each half)
     int         steps, stepsPerSplit;
-    int64_t     tiles, tilesN;
-    int         tilesM;
-    int         splits;
+    int         tiles, tilesM, tilesN, splits;
     float*      part;          // [splits][rows][ldpart] or NULL
     int64_t     ldpart;        // gated: the up half lies ldpart / 2 behind the gate half
     Finish      fin;
@@ -338,8 +336,6 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
     static_assert((NT == 2 || NT == 4) && MT >= 1 && MT <= 4, "a wave owns 64 or 128 columns");
     constexpr int kFrags = sizeof(T) == 1 ? 2 : 1, kGroups = 4 / kFrags;    // 16-byte fragments a product takes; groups of products a step
     constexpr uint32_t kBufBytes = (uint32_t)(BM + BN) * 128u;
-    constexpr int kOutPitch = 64 * 4 + 16;                         // bytes of a row of a wave's results on their way out
-    static_assert(WR * WC * 32 * kOutPitch <= 2 * (int)kBufBytes, "the results leave through the operands' LDS");
     __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * kBufBytes];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -347,18 +343,17 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
 
     // Workgroups go to the 8 XCDs in turn; each XCD gets a contiguous run of tiles, in bands of four tile rows, so that the tiles its 32 compute
     // units work on at a time share operand rows in its L2.
-    const int64_t total = gridDim.x;
-    int64_t id = blockIdx.x;
+    const uint32_t total = gridDim.x;
+    uint32_t id = blockIdx.x;
     {
-        const int64_t each = total / 8, more = total % 8, x = id % 8;
+        const uint32_t each = total / 8, more = total % 8, x = id % 8;
         id = x * each + (x < more ? x : more) + id / 8;
     }
-    const int split = uniform((int)(id / a.tiles));
-    id -= (int64_t)split * a.tiles;
-    const int64_t band = 4 * a.tilesN, g = id / band;
-    const int64_t high = min((int64_t)4, (int64_t)a.tilesM - g * 4);
-    const int64_t tm = g * 4 + (id - g * band) % high, tn = (id - g * band) / high;
-    const int64_t m0 = (int64_t)uniform((int)tm) * BM, n0 = (int64_t)uniform((int)tn) * (GATED ? BN / 2 : BN);
+    const int split = uniform((int)(id / (uint32_t)a.tiles));
+    id -= (uint32_t)split * (uint32_t)a.tiles;
+    const uint32_t band = 4 * (uint32_t)a.tilesN, g = id / band, inBand = id - g * band;
+    const uint32_t high = min(4u, (uint32_t)a.tilesM - g * 4), across = inBand / high;
+    const int64_t m0 = (int64_t)uniform((int)(g * 4 + inBand - across * high)) * BM, n0 = (int64_t)uniform((int)across) * (GATED ? BN / 2 : BN);
 
     Loader<T, BN, PL, kThreads, GATED, DIRECT> pl;
     Loader<T, BM, QL, kThreads, false, DIRECT> ql;
@@ -480,102 +475,223 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
     }
     __syncthreads();
 
-    // 32 rows x 64 columns of a wave's sums at a time. A block's lane holds row lane & 31, columns 8 (r / 4) + 4 (lane / 32) + r % 4; read back
-    // from LDS, neighbouring lanes hold neighbouring columns, and whole rows go to memory.
-    unsigned char* const out = smem + wave * 32 * kOutPitch;
+    // 64 columns of a wave's sums at a time. A block's lane holds row lane & 31, columns 8 (r / 4) + 4 (lane / 32) + r % 4; read back from LDS
+    // (256 bytes a row, 16-byte chunks exchanged by row & 15 against bank conflicts), neighbouring lanes hold neighbouring columns, and whole rows go
+    // to memory.
+    constexpr uint32_t kOutBytes = MT * 32 * 256;
+    static_assert(WR * WC * kOutBytes <= 2 * kBufBytes, "the results leave through the operands' LDS");
+    unsigned char* const out = smem + wave * kOutBytes;
     constexpr int kLanes = GATED ? 8 : 16, kRows = 64 / kLanes, kTurns = 32 / kRows;   // lanes a row (four columns each), rows a turn
-    const int c = (lane % kLanes) * 4;
+    const int chunk = lane % kLanes, c = chunk * 4, rowIn = lane / kLanes;
     const Finish& f = a.fin;
-    const bool quick = !GATED && f.act == LVG_ACT_LINEAR && f.slopeKind == LVG_SLOPE_NONE && f.clamp < 0.f && f.vec;
-    #pragma unroll 1
-    for (int h = 0; h < NT / 2; h++)
+    auto exchange = [&](auto half)
     {
-        const int64_t n = n0 + (wc * NT / 2 + h) * (GATED ? 32 : 64) + c;
-        Columns<O, GATED> cols;
-        if (!a.part) cols.init(f, n);
-        #pragma unroll 1
+        constexpr int h = decltype(half)::value;           // (known at compile time: an index would put the accumulators in memory)
+        wave_lds_order();
+        #pragma unroll
         for (int i = 0; i < MT; i++)
-        {
-            const int64_t m1 = m0 + wr * MT * 32 + i * 32 + lane / kLanes;
-            Quad<O> res[kTurns];
-            const bool add = quick && !a.part && f.residual && n < f.cols;
-            if (add)
-            {
-                #pragma unroll
-                for (int t = 0; t < kTurns; t++)
-                    if (m1 + t * kRows < f.rows) res[t] = *reinterpret_cast<const Quad<O>*>(static_cast<const O*>(f.residual) + (m1 + t * kRows) * f.ldr + n);
-            }
-            wave_lds_order();
             #pragma unroll
-            for (int ii = 0; ii < MT; ii++)
+            for (int j = 0; j < 2; j++)
                 #pragma unroll
-                for (int hh = 0; hh < NT / 2; hh++)
-                    if (ii == i && hh == h)
-                    {
-                        #pragma unroll
-                        for (int j = 0; j < 2; j++)
-                            #pragma unroll
-                            for (int q = 0; q < 4; q++)
-                                *reinterpret_cast<float4*>(out + (lane & 31) * kOutPitch + (32 * j + 8 * q + 4 * (lane >> 5)) * 4) =
-                                    make_float4(acc[ii][2 * hh + j][4 * q], acc[ii][2 * hh + j][4 * q + 1], acc[ii][2 * hh + j][4 * q + 2], acc[ii][2 * hh + j][4 * q + 3]);
-                    }
-            wave_lds_order();
-            if (a.part)
+                for (int k = 0; k < 4; k++)
+                    *reinterpret_cast<float4*>(out + (i * 32 + (lane & 31)) * 256 + (((8 * j + 2 * k + (lane >> 5)) ^ (lane & 15)) << 4)) =
+                        make_float4(acc[i][2 * h + j][4 * k], acc[i][2 * h + j][4 * k + 1], acc[i][2 * h + j][4 * k + 2], acc[i][2 * h + j][4 * k + 3]);
+        wave_lds_order();
+    };
+    auto sumsOf = [&](int pass, int t, float* v, float* u)
+    {
+        const int row = t * kRows + rowIn;
+        const unsigned char* from = out + (pass * 32 + row) * 256;
+        const float4 v4 = *reinterpret_cast<const float4*>(from + ((chunk ^ (row & 15)) << 4));
+        v[0] = v4.x; v[1] = v4.y; v[2] = v4.z; v[3] = v4.w;
+        if (GATED)
+        {
+            const float4 u4 = *reinterpret_cast<const float4*>(from + (((chunk + 8) ^ (row & 15)) << 4));
+            u[0] = u4.x; u[1] = u4.y; u[2] = u4.z; u[3] = u4.w;
+        }
+    };
+    auto halves = [&](auto work)
+    {
+        work(Const<0>());
+        if constexpr (NT == 4) work(Const<1>());
+    };
+    auto rowOf = [&](int pass) { return m0 + wr * MT * 32 + pass * 32 + rowIn; };
+    auto colOf = [&](int h) { return n0 + (wc * NT / 2 + h) * (GATED ? 32 : 64) + c; };
+    Columns<O, GATED> cols;
+
+    if (a.part)
+    {
+        halves([&](auto h)
+        {
+            exchange(h);
+            #pragma unroll 1
+            for (int pass = 0; pass < MT; pass++)
             {
-                #pragma unroll
-                for (int t = 0; t < kTurns; t++)
+            const int64_t m = rowOf(pass), n = colOf(h.value);
+            float* at = a.part + ((int64_t)split * a.qRows + m) * a.ldpart + n;      // (ldpart, or each half of it, is a multiple of four)
+            #pragma unroll
+            for (int t = 0; t < kTurns; t++)
+            {
+                float v[4], u[4];
+                sumsOf(pass, t, v, u);
+                if (m + t * kRows < a.qRows && n < a.pRows)
                 {
-                    const int64_t m = m1 + t * kRows;
-                    const unsigned char* from = out + (lane / kLanes + t * kRows) * kOutPitch + c * 4;
-                    if (m >= a.qRows || n >= a.pRows) continue;
-                    float* at = a.part + ((int64_t)split * a.qRows + m) * a.ldpart + n;      // (ldpart, or each half of it, is a multiple of four)
-                    *reinterpret_cast<float4*>(at) = *reinterpret_cast<const float4*>(from);
-                    if (GATED) *reinterpret_cast<float4*>(at + a.ldpart / 2) = *reinterpret_cast<const float4*>(from + 128);
+                    *reinterpret_cast<float4*>(at + t * kRows * a.ldpart) = make_float4(v[0], v[1], v[2], v[3]);
+                    if (GATED) *reinterpret_cast<float4*>(at + t * kRows * a.ldpart + a.ldpart / 2) = make_float4(u[0], u[1], u[2], u[3]);
                 }
             }
-            else if (n < f.cols)
+            }
+        });
+        return;
+    }
+
+    // Whole tiles of what is used most: no bounds, and nothing in a turn that waits for memory, since that would wait for the turn's own stores too.
+    // The residual of a pass is asked for before the stores of the pass ahead of it.
+    const bool whole = f.vec && m0 + BM <= f.rows && n0 + (GATED ? BN / 2 : BN) <= f.cols;
+    auto straight = [&](auto withResidual)
+    {
+        constexpr bool kRes = decltype(withResidual)::value != 0;
+        Quad<O> res[kTurns];
+        auto ask = [&](int h, int pass)
+        {
+            const O* r = static_cast<const O*>(f.residual) + rowOf(pass) * f.ldr + colOf(h);
+            #pragma unroll
+            for (int t = 0; t < kTurns; t++) res[t] = *reinterpret_cast<const Quad<O>*>(r + t * kRows * f.ldr);
+        };
+        if (kRes) ask(0, 0);
+        halves([&](auto h)
+        {
+        cols.init(f, colOf(h.value));
+        exchange(h);
+        #pragma unroll 1
+        for (int pass = 0; pass < MT; pass++)
+        {
+            float scale[kTurns];
+            if (sizeof(T) == 1)
             {
-                const Place<O> at(f, m1, n, GATED);
-                const unsigned char* const from = out + (lane / kLanes) * kOutPitch + c * 4;
-                auto turn = [&](int t, auto act)
+                #pragma unroll
+                for (int t = 0; t < kTurns; t++) scale[t] = f.qs[rowOf(pass) + t * kRows];
+            }
+            float v[kTurns][4], u[4];
+            #pragma unroll
+            for (int t = 0; t < kTurns; t++)
+            {
+                sumsOf(pass, t, v[t], u);
+                #pragma unroll
+                for (int k = 0; k < 4; k++)
                 {
-                    const int64_t m = m1 + t * kRows;
-                    const float4 v4 = *reinterpret_cast<const float4*>(from + t * kRows * kOutPitch);
-                    float v[4] = {v4.x, v4.y, v4.z, v4.w}, u[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (GATED)
-                    {
-                        const float4 u4 = *reinterpret_cast<const float4*>(from + t * kRows * kOutPitch + 128);
-                        u[0] = u4.x; u[1] = u4.y; u[2] = u4.z; u[3] = u4.w;
-                    }
-                    if (m >= f.rows) return;
-                    cols.apply(f, m, v, u);
-                    if constexpr (decltype(act)::value < 0)
-                    {
-                        #pragma unroll
-                        for (int k = 0; k < 4; k++) v[k] = v[k] * f.gain + (add ? row_load(res[t].v[k]) : 0.f);
-                        quad_store(at.down(f, t * kRows, GATED).out, 4, true, v);
-                    }
-                    else finish4<O, GATED, decltype(act)::value>(f, at.down(f, t * kRows, GATED), v, u);
-                };
-                // the usual ones unrolled, the others one turn at a time
-                if (quick)
-                {
-                    #pragma unroll
-                    for (int t = 0; t < kTurns; t++) turn(t, Const<-1>());
+                    if (sizeof(T) == 1) v[t][k] *= scale[t] * cols.scale[k];
+                    v[t][k] = (v[t][k] + cols.bias[k]) * f.gain + (kRes ? row_load(res[t].v[k]) : 0.f);
                 }
-                else if (f.act == (GATED ? LVG_ACT_SWISH : LVG_ACT_LRELU))
+            }
+            if (kRes)
+            {
+                if (pass + 1 < MT) ask(h.value, pass + 1);
+                else if (h.value + 1 < NT / 2) ask(h.value + 1, 0);
+            }
+            O* to = static_cast<O*>(f.out) + rowOf(pass) * f.ldo + colOf(h.value);
+            #pragma unroll
+            for (int t = 0; t < kTurns; t++) quad_store(to + t * kRows * f.ldo, 4, true, v[t]);
+        }
+        });
+    };
+    auto gate = [&](auto withSlopes)
+    {
+        constexpr bool kSlopes = decltype(withSlopes)::value != 0;
+        halves([&](auto h)
+        {
+        cols.init(f, colOf(h.value));
+        exchange(h);
+        #pragma unroll 1
+        for (int pass = 0; pass < MT; pass++)
+        {
+            float scale[kTurns];
+            if (sizeof(T) == 1)
+            {
+                #pragma unroll
+                for (int t = 0; t < kTurns; t++) scale[t] = f.qs[rowOf(pass) + t * kRows];
+            }
+            O* to = static_cast<O*>(f.out) + rowOf(pass) * f.ldo + colOf(h.value);
+            float* slopes = kSlopes ? static_cast<float*>(f.slopes) + rowOf(pass) * 2 * f.cols + colOf(h.value) : nullptr;
+            float v[kTurns][4], u[kTurns][4];
+            #pragma unroll
+            for (int t = 0; t < kTurns; t++) sumsOf(pass, t, v[t], u[t]);
+            #pragma unroll
+            for (int t = 0; t < kTurns; t++)
+            {
+                float act[4], d[4];
+                #pragma unroll
+                for (int k = 0; k < 4; k++)
                 {
-                    #pragma unroll
-                    for (int t = 0; t < kTurns; t++) turn(t, Const<GATED ? LVG_ACT_SWISH : LVG_ACT_LRELU>());
+                    if (sizeof(T) == 1) { v[t][k] *= scale[t] * cols.scale[k]; u[t][k] *= scale[t] * cols.scaleUp[k]; }
+                    v[t][k] += cols.bias[k];
+                    u[t][k] += cols.biasUp[k];
                 }
-                else
+                act4<LVG_ACT_SWISH, sizeof(O) == 2>(LVG_ACT_SWISH, 0.f, v[t], kSlopes, act, d);
+                #pragma unroll
+                for (int k = 0; k < 4; k++)
                 {
-                    #pragma unroll 1
-                    for (int t = 0; t < kTurns; t++) turn(t, Const<0>());
+                    act[k] *= f.gain;               // dh/du
+                    d[k] *= u[t][k] * f.gain;       // dh/dg
+                    v[t][k] = act[k] * u[t][k];
                 }
+                if (kSlopes)
+                {
+                    quad_store(slopes + t * kRows * 2 * f.cols, 4, true, d);
+                    quad_store(slopes + t * kRows * 2 * f.cols + f.cols, 4, true, act);
+                }
+                quad_store(to + t * kRows * f.ldo, 4, true, v[t]);
             }
         }
+        });
+    };
+    if constexpr (GATED)
+    {
+        if (whole && f.act == LVG_ACT_SWISH)
+        {
+            if (f.slopeKind == LVG_SLOPE_F32) gate(Const<1>());
+            else gate(Const<0>());
+            return;
+        }
     }
+    else if (whole && f.act == LVG_ACT_LINEAR && f.slopeKind == LVG_SLOPE_NONE && f.clamp < 0.f)
+    {
+        if (f.residual) straight(Const<1>());
+        else straight(Const<0>());
+        return;
+    }
+
+    // every other activation, and the tiles at the result's edges
+    halves([&](auto h)
+    {
+    const int64_t n = colOf(h.value), left = f.cols - n;
+    cols.init(f, n);
+    exchange(h);
+    #pragma unroll 1
+    for (int pass = 0; pass < MT; pass++)
+    {
+        const int64_t m = rowOf(pass);
+        float res[kTurns][4];
+        #pragma unroll
+        for (int t = 0; t < kTurns; t++)
+        {
+            #pragma unroll
+            for (int k = 0; k < 4; k++) res[t][k] = 0.f;
+            if (!GATED && f.residual && m + t * kRows < f.rows && left > 0)
+                quad_load(static_cast<const O*>(f.residual) + (m + t * kRows) * f.ldr + n, left, f.vec, res[t]);
+        }
+        const Place<O> at(f, m, n, GATED);
+        #pragma unroll
+        for (int t = 0; t < kTurns; t++)
+        {
+            float v[4], u[4];
+            sumsOf(pass, t, v, u);
+            if (m + t * kRows >= f.rows || left <= 0) continue;
+            cols.apply(f, m + t * kRows, v, u);
+            finish4<O, GATED>(f, at.down(f, t * kRows, GATED), v, u, res[t]);
+        }
+    }
+    });
 }
 
 } // namespace
@@ -596,7 +712,7 @@ namespace {
 
 template <class T, class O, int PL, int QL, bool GATED> int token_launch_form(int tile, bool direct, const TokenArgs& a, hipStream_t s)
 {
-    const int64_t blocks = a.tiles * a.splits;
+    const int64_t blocks = (int64_t)a.tiles * a.splits;
     if (blocks > ((int64_t)1 << 22)) { lvg_set_error("token product: %lld workgroups", (long long)blocks); return LVG_ERR_INVALID; }
     const dim3 grid((unsigned)blocks);
     #define LVG_TILE(ID, BM, BN, WR, WC) if (tile == ID) { \

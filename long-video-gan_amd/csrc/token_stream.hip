@@ -212,7 +212,9 @@ __global__ __launch_bounds__(kWaves * 64) void token_stream_kernel(StreamArgs a)
         return;
     }
     prepare4<O, GATED>(a.fin, m, n, v, u);
-    finish4<O, GATED>(a.fin, Place<O>(a.fin, m, n, GATED), v, u);
+    float r[4];
+    residual4<O>(a.fin, m, n, r);
+    finish4<O, GATED>(a.fin, Place<O>(a.fin, m, n, GATED), v, u, r);
 }
 
 template <class T, class O> int launch(const StreamArgs& a, bool gated, int splits, hipStream_t s)
