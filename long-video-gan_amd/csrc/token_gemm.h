@@ -115,6 +115,7 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
     static constexpr int kDepth = 128 / (int)sizeof(T);            // summed index a step
     static constexpr int kNum = BX * 8 / NTHR;
     static constexpr int kPitchChunks = BX * (int)sizeof(T) / 16;  // down
+    static constexpr int kFirst = sizeof(T) == 1 ? kNum : kNum / 2;    // chunks a step's first sends are for (see spread)
     const char* base;          // operand at the tile's first row (along) / column (down)
     int64_t     ld, inner, left;   // left: rows / columns of the operand from the tile's first on
     int64_t     upOff;         // gated: bytes from a gate row to its up row
@@ -231,7 +232,7 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
         else if ((int64_t)(step + 1) * kDepth <= inner)
         {
             #pragma unroll
-            for (int i = 0; i < kNum; i++) if ((i < kNum / 2) == (half == 0)) send(i, step, tile, wave);
+            for (int i = 0; i < kNum; i++) if ((i < kFirst) == (half == 0)) send(i, step, tile, wave);
         }
         else if (half)
         {
@@ -419,16 +420,19 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
     if (DIRECT)
     {
         // Steps whose second next one is whole: no branches. The sends for a step lie between the products of the group behind the barrier that
-        // frees its buffer and of the group after that.
+        // frees its buffer and of the group after that, one for two products: one for each costs 16-bit products 6 % (8192^3: 805 -> 893 us). The
+        // 8-bit step has two groups of products twice as long, all its sends lie in the first of them and have a whole step to arrive (8192 x 4096
+        // -> 4096: 133 -> 121 us).
         auto spread = [&](int k, int half, int step, uint32_t pt)
         {
-            constexpr int kP = BN * 8 / kThreads / 2, kAll = kP + BM * 8 / kThreads / 2, kMma = MT * NT;
+            constexpr int kPF = decltype(pl)::kFirst, kQF = decltype(ql)::kFirst, kMma = MT * NT;
+            const int np = half ? decltype(pl)::kNum - kPF : kPF, all = np + (half ? decltype(ql)::kNum - kQF : kQF);
             #pragma unroll
-            for (int i = 0; i < kAll; i++)
-                if (i * kMma / kAll == k)
+            for (int i = 0; i < all; i++)
+                if (i * kMma / all == k)
                 {
-                    if (i < kP) pl.send(half * kP + i, step, pt, wave);
-                    else ql.send(half * (kAll - kP) + i - kP, step, pt + BN * 128, wave);
+                    if (i < np) pl.send(half * kPF + i, step, pt, wave);
+                    else ql.send(half * kQF + i - np, step, pt + BN * 128, wave);
                 }
             __builtin_amdgcn_sched_barrier(0);
         };
