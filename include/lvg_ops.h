@@ -561,11 +561,12 @@ int lvg_column_sum(const float* part, void* out, int slots, int64_t width, float
  * The two products of the backward pass; grad is dense.
  *   weight == 0: grad [rows, inner]  = gain * dz [rows, outer] . other, other = w [outer, inner]
  *   weight == 1: grad [outer, inner] = gain * dz^T . other,             other = x [rows, inner]
+ * dz_whole: every row of dz is readable for dz_stride elements (what lies behind `outer` is not used).
  * work: lvg_linear_grad_work(...) bytes, 16-byte aligned.
  */
 int64_t lvg_linear_grad_work(int64_t rows, int64_t outer, int64_t inner, int weight, int dtype);
 int lvg_linear_grad(const void* dz, const void* other, void* grad, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
-                    int64_t dz_stride, int64_t other_stride, int weight, float gain, int dtype, void* stream);
+                    int64_t dz_stride, int64_t other_stride, int dz_whole, int weight, float gain, int dtype, void* stream);
 
 /*
  * s = x + residual;  y = weight * s / sqrt(mean(s^2) + eps)   over rows [rows, width], width >= 1. residual (and then sum = s rounded to dtype),

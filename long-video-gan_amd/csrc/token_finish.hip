@@ -181,19 +181,140 @@ int64_t part_pitch(int64_t cols, bool gated) { return (cols + 3) / 4 * 4 * (gate
 
 bool streams(int64_t rows, int form) { return rows <= kStreamRows && (form == LVG_TOKEN_FORWARD || form == LVG_TOKEN_GATED); }
 
-int64_t work_bytes(int64_t rows, int64_t cols, int64_t inner, int dtype, int form)
+int layout_p(int form) { return form == LVG_TOKEN_ROW_GRAD || form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG; }
+int layout_q(int form) { return form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG; }
+
+int64_t pad16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Layout of a product over the 256 compute units, from its sizes alone: the same answer sizes the workspace and launches.
+//
+// A step of a tile costs `cycles` of a compute unit that holds as many workgroups as fit (1 / 2 / 3 of the 256 / 128 / 64-row tiles), and `alone` if
+// it has one; measured at 2.1 GHz on direct operands: 256 rows 1.45 us; 128: 0.48 and 0.7 us; 64: 0.33 and 0.57 us. Rows that go through registers
+// cost 1.8 times as much (float32: 1.25). Splitting the summed index fills the chip when there are few tiles, and costs the float32 parts' way to memory and back and
+// one more launch (about 4 us). Operands whose sizes make their rows start at odd places are repacked first, in one launch for both, where the
+// product is long enough to pay for it (3000 x 1501 -> 3000, bfloat16: 62 us, and 79 us through registers; 1237 x 771 -> 515: 19 and 14 us).
+
+struct TokenPlan { int tile, splits; bool pack; };
+
+TokenPlan token_plan(int64_t rows, int64_t cols, int64_t inner, int es, int form)
+{
+    static const struct { int bm, bn, held; double cycles[2], alone[2], more; } kTile[3] = {     // [float32]
+        {256, 256, 1, {3000., 15400.}, {3000., 15400.}, 22000.},
+        {128, 128, 2, {1000., 4000.}, {1450., 4100.}, 9000.},
+        {64, 128, 3, {700., 2050.}, {1150., 2100.}, 5000.}};
+    const bool gated = form == LVG_TOKEN_GATED, f32 = es == 4;
+    const int64_t steps = std::max<int64_t>(1, lvg_ceil_div(inner * es, 128)), width = cols * (gated ? 2 : 1);
+    const int64_t pBytes = layout_p(form) == ALONG ? inner * es : cols * es;       // of an operand's row
+    const bool odd = pBytes % 16 != 0 || (layout_q(form) == ALONG && form != LVG_TOKEN_ROW_GRAD && (inner * es) % 16 != 0);
+    TokenPlan best = {LVG_TILE_128, 1, false};
+    double least = 1e300;
+    for (int pack = 0; pack <= (odd ? 1 : 0); pack++)
+    {
+        // (bytes of the operands, read and written; bytes a cycle)
+        const double packing = pack ? 12000. + 2. * es * (double)inner * ((double)width + (layout_q(form) == ALONG && form != LVG_TOKEN_ROW_GRAD ? (double)rows : 0.)) / 1500. : 0.;
+        const double slow = odd && !pack ? (f32 ? 1.25 : 1.8) : 1.;
+        for (int t = 0; t < 3; t++)
+        {
+            if (es == 1 && odd && !pack && t == LVG_TILE_256) continue;
+            const int64_t tiles = lvg_ceil_div(rows, kTile[t].bm) * lvg_ceil_div(cols, kTile[t].bn / (gated ? 2 : 1));
+            for (int64_t splits = 1; splits <= 64 && splits <= steps; splits = splits < 4 ? splits + 1 : splits * 3 / 2)
+            {
+                if (splits > 1 && (tiles * splits > 2048 || (double)rows * (double)width > 1e9)) break;
+                const int64_t each = lvg_ceil_div(steps, splits);
+                if (lvg_ceil_div(steps, each) != splits) continue;
+                const int64_t perCu = lvg_ceil_div(tiles * splits, 256), rounds = lvg_ceil_div(perCu, kTile[t].held);
+                const double held = (double)std::min<int64_t>(perCu, kTile[t].held);
+                double cost = packing + (double)rounds * ((double)each * slow * std::max(kTile[t].alone[f32], held * kTile[t].cycles[f32]) + kTile[t].more);
+                if (splits > 1) cost += 8000. + (double)splits * (double)rows * (double)width * 8. / 3000.;
+                if (cost < least) { least = cost; best = {t, (int)splits, pack != 0}; }
+            }
+        }
+    }
+    return best;
+}
+
+// Workspace: the parts, then the repacked operands.
+struct Work { int64_t part, p, q, all; };
+
+Work work_of(const TokenPlan& k, int64_t rows, int64_t cols, int64_t inner, int es, int form)
 {
     const bool gated = form == LVG_TOKEN_GATED;
-    const int es = esize_of(dtype), splits = streams(rows, form) ? token_stream_splits(rows, cols, inner * es, gated) : token_plan(rows, cols, inner, es, gated).splits;
+    Work w = {0, 0, 0, 0};
+    if (k.splits > 1) w.part = (int64_t)k.splits * rows * part_pitch(cols, gated) * 4;
+    if (k.pack)
+    {
+        w.p = layout_p(form) == ALONG ? cols * (gated ? 2 : 1) * pad16(inner * es) : inner * pad16(cols * es);
+        if (layout_q(form) == ALONG && form != LVG_TOKEN_ROW_GRAD) w.q = rows * pad16(inner * es);
+    }
+    w.all = w.part + w.p + w.q;
+    return w;
+}
+
+int64_t work_bytes(int64_t rows, int64_t cols, int64_t inner, int dtype, int form)
+{
+    const int es = esize_of(dtype);
+    if (!streams(rows, form)) return work_of(token_plan(rows, cols, inner, es, form), rows, cols, inner, es, form).all;
+    const bool gated = form == LVG_TOKEN_GATED;
+    const int splits = token_stream_splits(rows, cols, inner * es, gated);
     return splits > 1 ? (int64_t)splits * rows * part_pitch(cols, gated) * 4 : 0;
 }
 
-// Operands that can travel to LDS without registers: 16-byte aligned rows, offsets inside a tile below 2^32, whole chunks of columns.
-bool direct_ok(const void* base, int64_t ld, int64_t count, int layout, int es, bool gated)
+// ---------------------------------------------------------------------------------------------------------------------
+// Repacking: rows of n bytes to rows that start at multiples of 16 bytes, zeros behind them. Two matrices in one launch, a thread a 16-byte chunk.
+
+struct PackArgs { const char* src[2]; char* dst[2]; int64_t ld[2], bytes[2], chunks[2]; };    // chunks: of the whole matrix
+
+template <class T>
+__global__ __launch_bounds__(256) void token_pack_kernel(PackArgs p)
+{
+    int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int which = i >= p.chunks[0] ? 1 : 0;
+    i -= which ? p.chunks[0] : 0;
+    if (i >= p.chunks[which]) return;
+    const int64_t per = (p.bytes[which] + 15) / 16, row = i / per, at = (i - row * per) * 16;
+    const char* src = p.src[which] + row * p.ld[which] + at;
+    const int64_t n = (p.bytes[which] - at) / (int64_t)sizeof(T);
+    constexpr int kE = 16 / (int)sizeof(T);
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (n >= kE) __builtin_memcpy(&v, src, 16);
+    else
+    {
+        T e[kE];
+        #pragma unroll
+        for (int j = 0; j < kE; j++)
+        {
+            if (j < n) e[j] = reinterpret_cast<const T*>(src)[j];
+            else __builtin_memset(&e[j], 0, sizeof(T));
+        }
+        __builtin_memcpy(&v, e, 16);
+    }
+    *reinterpret_cast<uint4*>(p.dst[which] + i * 16) = v;
+}
+
+int launch_pack(const PackArgs& p, int es, hipStream_t s)
+{
+    const int64_t blocks = lvg_ceil_div(p.chunks[0] + p.chunks[1], 256);
+    if (blocks == 0) return LVG_OK;
+    if (blocks > ((int64_t)1 << 23)) { lvg_set_error("token product: operands of %lld bytes to repack", (long long)blocks * 4096); return LVG_ERR_INVALID; }
+    const dim3 grid((unsigned)blocks), block(256);
+    if (es == 4) hipLaunchKernelGGL(token_pack_kernel<float>, grid, block, 0, s, p);
+    else if (es == 2) hipLaunchKernelGGL(token_pack_kernel<bf16_t>, grid, block, 0, s, p);
+    else hipLaunchKernelGGL(token_pack_kernel<e4m3_t>, grid, block, 0, s, p);
+    return lvg_check_launch("token product, repacking its operands");
+}
+
+// Offsets inside an operand's tile fit 32 bits.
+bool near_ok(int64_t ld, int64_t count, int layout, int es, bool gated)
+{
+    return (layout == ALONG ? 256 * ld + (gated ? count * ld : 0) : (128 / es) * ld + 1024) < ((int64_t)1 << 32);
+}
+
+// Operands that can travel to LDS without registers: 16-byte aligned rows, whole chunks of columns.
+bool direct_ok(const void* base, int64_t ld, int64_t stored, int layout, int es)
 {
     if (!lvg_aligned16(base) || ld % 16 != 0) return false;
-    if (layout == ALONG) return 256 * ld + (gated ? count * ld : 0) < ((int64_t)1 << 32);
-    return (128 / es) * ld + 1024 < ((int64_t)1 << 32) && (count * es) % 16 == 0 && count * es >= 16;
+    return layout == ALONG || ((stored * es) % 16 == 0 && stored * es >= 16);
 }
 
 // The product itself: rows x cols results over `inner`, args with operands and finish filled in.
@@ -203,7 +324,6 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
     const bool gated = form == LVG_TOKEN_GATED;
     const int64_t rows = a.qRows, cols = a.pRows, need = work_bytes(rows, cols, a.inner, dtype, form);
     LVG_REQUIRE(need == 0 || (work && lvg_aligned16(work) && work_size >= need), "%s: the workspace must be 16-byte aligned and hold %lld bytes", what, (long long)need);
-    a.part = need ? static_cast<float*>(work) : nullptr;
     a.ldpart = part_pitch(cols, gated);
     Finish& f = a.fin;
     auto whole = [&](const void* p, int64_t ld) { return !p || (((uintptr_t)p) % (4 * os) == 0 && ld % 4 == 0); };
@@ -212,6 +332,7 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
     if (streams(rows, form))
     {
         splits = token_stream_splits(rows, cols, a.inner * es, gated);
+        a.part = splits > 1 ? static_cast<float*>(work) : nullptr;
         StreamArgs t = {a.p, a.q, a.ldp, a.ldq, a.inner * es, rows, cols, 0, 0, a.part, a.ldpart, f};
         t.spans = (int)lvg_ceil_div(t.bytes, 256);
         t.spansPerSplit = (int)lvg_ceil_div(t.spans, splits);
@@ -219,17 +340,46 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
     }
     else
     {
-        const TokenPlan k = token_plan(rows, cols, a.inner, es, gated);
+        TokenPlan k = token_plan(rows, cols, a.inner, es, form);
+        const Work w = work_of(k, rows, cols, a.inner, es, form);
+        const int pl = layout_p(form), ql = layout_q(form);
+        splits = k.splits;
+        a.part = splits > 1 ? static_cast<float*>(work) : nullptr;
+        if (!a.pStored) a.pStored = cols;
+        if (!a.qStored) a.qStored = rows;
+        if (k.pack && a.inner > 0)
+        {
+            PackArgs g;
+            memset(&g, 0, sizeof(g));
+            char* at = static_cast<char*>(work) + w.part;
+            if (w.p && !direct_ok(a.p, a.ldp, a.pStored, pl, es))
+            {
+                const int64_t n = pl == ALONG ? a.inner * es : cols * es, ld = pad16(n);
+                g.src[0] = static_cast<const char*>(a.p); g.dst[0] = at; g.ld[0] = a.ldp; g.bytes[0] = n; g.chunks[0] = w.p / 16;
+                a.p = at; a.ldp = ld;
+                if (pl == DOWN) a.pStored = ld / es;
+            }
+            if (w.q && !direct_ok(a.q, a.ldq, a.qStored, ql, es))
+            {
+                at += w.p;
+                g.src[1] = static_cast<const char*>(a.q); g.dst[1] = at; g.ld[1] = a.ldq; g.bytes[1] = a.inner * es; g.chunks[1] = w.q / 16;
+                a.q = at; a.ldq = pad16(a.inner * es);
+            }
+            rc = launch_pack(g, es, s);
+            if (rc != LVG_OK) return rc;
+        }
+        a.near = near_ok(a.ldp, cols, pl, es, gated) && near_ok(a.ldq, rows, ql, es, false);
+        const bool direct = a.near && direct_ok(a.p, a.ldp, a.pStored, pl, es) && direct_ok(a.q, a.ldq, a.qStored, ql, es);
+        // (8-bit steps through registers hold twice the fragments: the largest tile would not fit)
+        if (es == 1 && !direct && k.tile == LVG_TILE_256) k.tile = LVG_TILE_128;
         const int bm = k.tile == LVG_TILE_256 ? 256 : k.tile == LVG_TILE_128 ? 128 : 64, bn = (k.tile == LVG_TILE_256 ? 256 : 128) / (gated ? 2 : 1);
         a.steps = (int)lvg_ceil_div(a.inner * es, 128);
-        a.stepsPerSplit = (int)lvg_ceil_div(a.steps, k.splits);
-        a.splits = splits = k.splits;
+        a.stepsPerSplit = (int)lvg_ceil_div(a.steps, splits);
+        a.splits = splits;
         a.tilesM = (int)lvg_ceil_div(rows, bm);
         a.tilesN = (int)lvg_ceil_div(cols, bn);
         LVG_REQUIRE((int64_t)a.tilesM * a.tilesN <= ((int64_t)1 << 22), "%s: a result of %lld x %lld", what, (long long)rows, (long long)cols);
         a.tiles = a.tilesM * a.tilesN;
-        const int pl = form == LVG_TOKEN_ROW_GRAD || form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG, ql = form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG;
-        const bool direct = direct_ok(a.p, a.ldp, cols, pl, es, gated) && direct_ok(a.q, a.ldq, rows, ql, es, false);
         if (dtype == LVG_E4M3)      rc = token_launch_8bit(form, k.tile, direct, out_dtype, a, s);
         else if (dtype == LVG_F32)  rc = token_launch_f32(form, k.tile, direct, a, s);
         else if (dtype == LVG_F16)  rc = token_launch_f16(form, k.tile, direct, a, s);
@@ -240,33 +390,6 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
 }
 
 } // namespace
-
-// Layout of a product over the 256 compute units. A tile's step costs its matrix instructions (in cycles, with what the K loop reaches of the
-// peak) and at least the latency of the operands' way to LDS; a compute unit holds 1 / 2 / 3 workgroups of the 256 / 128 / 64-row tiles. Splitting
-// the summed index fills the chip when there are few tiles, and costs the float32 parts' way to memory and back and one more launch.
-TokenPlan token_plan(int64_t rows, int64_t cols, int64_t inner, int esize, bool gated)
-{
-    static const struct { int bm, bn, held; double cycles; } kTile[3] = {{256, 256, 1, 3000.}, {128, 128, 2, 900.}, {64, 128, 3, 600.}};
-    const int64_t steps = std::max<int64_t>(1, lvg_ceil_div(inner * esize, 128));
-    TokenPlan best = {LVG_TILE_128, 1};
-    double least = 1e300;
-    for (int t = 0; t < 3; t++)
-    {
-        const double step = kTile[t].cycles * (esize == 4 ? 8. : 1.);
-        const int64_t tiles = lvg_ceil_div(rows, kTile[t].bm) * lvg_ceil_div(cols, kTile[t].bn / (gated ? 2 : 1));
-        for (int64_t splits = 1; splits <= 64 && splits <= steps; splits = splits < 4 ? splits + 1 : splits * 3 / 2)
-        {
-            const int64_t each = lvg_ceil_div(steps, splits);
-            if (lvg_ceil_div(steps, each) != splits) continue;
-            const int64_t perCu = lvg_ceil_div(tiles * splits, 256), rounds = lvg_ceil_div(perCu, kTile[t].held);
-            const double held = (double)std::min<int64_t>(perCu, kTile[t].held);
-            double cost = (double)rounds * ((double)each * std::max(1500., held * step) + 5000.);
-            if (splits > 1) cost += 8000. + (double)splits * (double)rows * (double)cols * (gated ? 2 : 1) * 8. / 1800.;   // bytes / (bytes a cycle)
-            if (cost < least) { least = cost; best = {t, (int)splits}; }
-        }
-    }
-    return best;
-}
 
 extern "C" int64_t lvg_linear_act_work(int64_t rows, int64_t outer, int64_t inner, int dtype, int gated)
 {
@@ -313,19 +436,20 @@ extern "C" int64_t lvg_linear_grad_work(int64_t rows, int64_t outer, int64_t inn
 }
 
 extern "C" int lvg_linear_grad(const void* dz, const void* other, void* grad, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
-                               int64_t dz_stride, int64_t other_stride, int weight, float gain, int dtype, void* stream)
+                               int64_t dz_stride, int64_t other_stride, int dz_whole, int weight, float gain, int dtype, void* stream)
 {
     LVG_REQUIRE(float_type(dtype), "lvg_linear_grad: float32 / float16 / bfloat16 only (dtype %d)", dtype);
     LVG_REQUIRE(size_ok(rows) && size_ok(outer) && size_ok(inner), "lvg_linear_grad: bad size");
     if (inner == 0 || (weight ? outer : rows) == 0) return LVG_OK;
     LVG_REQUIRE(grad && ((weight ? rows : outer) == 0 || (dz && other)), "lvg_linear_grad: missing pointer");
-    LVG_REQUIRE(dz_stride >= 0 && other_stride >= 0, "lvg_linear_grad: negative row stride");
+    LVG_REQUIRE(dz_stride >= 0 && other_stride >= 0 && (!dz_whole || dz_stride >= outer), "lvg_linear_grad: bad row stride");
     TokenArgs a;
     memset(&a, 0, sizeof(a));
     const int es = esize_of(dtype);
     a.p = other; a.q = dz;
     a.ldp = other_stride * es; a.ldq = dz_stride * es;
     a.inner = weight ? rows : outer; a.pRows = inner; a.qRows = weight ? outer : rows;
+    if (weight && dz_whole) a.qStored = dz_stride;
     Finish& f = a.fin;
     f.out = grad; f.ldo = inner; f.rows = a.qRows; f.cols = inner;
     f.act = LVG_ACT_LINEAR; f.gain = gain; f.clamp = -1.f;

@@ -31,8 +31,10 @@ struct TokenArgs
     int64_t     ldp, ldq;      // bytes between stored rows
     int64_t     inner;         // summed index
     int64_t     pRows, qRows;  // columns / rows of the result (gated: pRows of each half)
+    int64_t     pStored, qStored;   // columns / rows of them that the operands hold: more where their rows are padded
     int         steps, stepsPerSplit;
     int         tiles, tilesM, tilesN, splits;
+    bool        near;          // offsets inside a tile fit 32 bits
     float*      part;          // [splits][rows][ldpart] or NULL
     int64_t     ldpart;        // gated: the up half lies ldpart / 2 behind the gate half
     Finish      fin;
@@ -120,8 +122,9 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
     int64_t     ld, inner, left;   // left: rows / columns of the operand from the tile's first on
     int64_t     upOff;         // gated: bytes from a gate row to its up row
     int         tid;
-    uint32_t    off[DIRECT ? kNum : 1];
+    uint32_t    off[kNum];     // of the chunks, from the tile's place in the operand on
     uint4       hold[DIRECT ? 1 : kNum];
+    uint32_t    edge;          // through registers: chunks that are never whole (bits); all of them where offsets pass 32 bits
 
     // row of the tile -> row of the operand behind the tile's first one; gated tiles alternate 32 gate rows and 32 up rows
     __device__ __forceinline__ int64_t place(int row, bool& up) const
@@ -145,30 +148,32 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
             if (sizeof(T) == 2) chunk ^= kPitchChunks >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2;
         }
     }
-    __device__ __forceinline__ void init(const void* operand, int64_t ld_, int64_t inner_, int64_t first, int64_t count, int tid_)
+    __device__ __forceinline__ void init(const void* operand, int64_t ld_, int64_t inner_, int64_t first, int64_t count, int tid_, bool near)
     {
         ld = ld_; inner = inner_; left = count - first; tid = tid_;
         base = static_cast<const char*>(operand) + (LAYOUT == ALONG ? first * ld : first * (int64_t)sizeof(T));
         upOff = GATED ? count * ld : 0;
-        if (DIRECT)
+        edge = near ? 0u : ~0u;
+        #pragma unroll
+        for (int i = 0; i < kNum; i++)
         {
-            #pragma unroll
-            for (int i = 0; i < kNum; i++)
+            int row, chunk;
+            chunk_of(i, row, chunk);
+            if (LAYOUT == ALONG)
             {
-                int row, chunk;
-                chunk_of(i, row, chunk);
-                if (LAYOUT == ALONG)
+                bool up;
+                const int64_t r = place(row, up);
+                off[i] = (uint32_t)(r * ld + (up ? upOff : 0) + chunk * 16);
+            }
+            else
+            {
+                int64_t col = (int64_t)chunk * kE;
+                if (col > left - kE)
                 {
-                    bool up;
-                    const int64_t r = place(row, up);
-                    off[i] = (uint32_t)(r * ld + (up ? upOff : 0) + chunk * 16);
+                    if (!DIRECT) edge |= 1u << i;
+                    col = left - kE;
                 }
-                else
-                {
-                    int64_t col = (int64_t)chunk * kE;
-                    if (col > left - kE) col = left - kE;
-                    off[i] = (uint32_t)(row * ld + col * (int64_t)sizeof(T));
-                }
+                off[i] = (uint32_t)(row * ld + col * (int64_t)sizeof(T));
             }
         }
     }
@@ -217,7 +222,7 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
     __device__ __forceinline__ void send(int i, int step, uint32_t tile, int wave) const
     {
         const char* b = base + (int64_t)step * (LAYOUT == ALONG ? 128 : kDepth * ld);
-        wdma16(reinterpret_cast<const unsigned char*>(b), off[DIRECT ? i : 0], tile + (uint32_t)(i * NTHR + wave * 64) * 16u);
+        wdma16(reinterpret_cast<const unsigned char*>(b), off[i], tile + (uint32_t)(i * NTHR + wave * 64) * 16u);
     }
     // A step's tile is started in two halves (0, 1). Rows that go through registers are all loaded in the first, masked steps of direct ones are
     // written in the second.
@@ -226,8 +231,27 @@ template <class T, int BX, int LAYOUT, int NTHR, bool GATED, bool DIRECT> struct
         if (!DIRECT)
         {
             if (half) return;
-            #pragma unroll
-            for (int i = 0; i < kNum; i++) hold[i] = masked(step, i);
+            if ((int64_t)(step + 1) * kDepth <= inner)
+            {
+                const char* b = base + (int64_t)step * (LAYOUT == ALONG ? 128 : kDepth * ld);
+                if (edge == 0)
+                {
+                    #pragma unroll
+                    for (int i = 0; i < kNum; i++) __builtin_memcpy(&hold[i], b + off[i], 16);
+                    return;
+                }
+                #pragma unroll
+                for (int i = 0; i < kNum; i++)
+                {
+                    if (edge >> i & 1) hold[i] = masked(step, i);
+                    else __builtin_memcpy(&hold[i], b + off[i], 16);
+                }
+            }
+            else
+            {
+                #pragma unroll
+                for (int i = 0; i < kNum; i++) hold[i] = masked(step, i);
+            }
         }
         else if ((int64_t)(step + 1) * kDepth <= inner)
         {
@@ -358,8 +382,8 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
 
     Loader<T, BN, PL, kThreads, GATED, DIRECT> pl;
     Loader<T, BM, QL, kThreads, false, DIRECT> ql;
-    pl.init(a.p, a.ldp, a.inner, n0, a.pRows, tid);
-    ql.init(a.q, a.ldq, a.inner, m0, a.qRows, tid);
+    pl.init(a.p, a.ldp, a.inner, n0, a.pStored, tid, a.near);
+    ql.init(a.q, a.ldq, a.inner, m0, a.qStored, tid, a.near);
     Fragments<T, BN, PL> pf;
     Fragments<T, BM, QL> qf;
     pf.init(lane, wc * NT * 32);
@@ -549,161 +573,179 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
         return;
     }
 
-    // Whole tiles of what is used most: no bounds, and nothing in a turn that waits for memory, since that would wait for the turn's own stores too.
-    // The residual of a pass is asked for before the stores of the pass ahead of it.
-    const bool whole = f.vec && m0 + BM <= f.rows && n0 + (GATED ? BN / 2 : BN) <= f.cols;
-    auto straight = [&](auto withResidual)
+    // What is used most: nothing in a turn waits for memory, since that would wait for the turn's own stores too (the residual of a pass is asked
+    // for before the stores of the pass ahead of it), and little code: each workgroup runs through it once, from a cold instruction cache. Tiles
+    // inside the result know no bounds.
+    const bool inside = f.vec && m0 + BM <= f.rows && n0 + (GATED ? BN / 2 : BN) <= f.cols;
+    auto straight = [&](auto withResidual, auto atEdge)
     {
-        constexpr bool kRes = decltype(withResidual)::value != 0;
+        constexpr bool kRes = decltype(withResidual)::value != 0, kEdge = decltype(atEdge)::value != 0;
         Quad<O> res[kTurns];
         auto ask = [&](int h, int pass)
         {
-            const O* r = static_cast<const O*>(f.residual) + rowOf(pass) * f.ldr + colOf(h);
+            const int64_t m = rowOf(pass), n = colOf(h), left = f.cols - n;
+            const O* r = static_cast<const O*>(f.residual) + m * f.ldr + n;
             #pragma unroll
-            for (int t = 0; t < kTurns; t++) res[t] = *reinterpret_cast<const Quad<O>*>(r + t * kRows * f.ldr);
+            for (int t = 0; t < kTurns; t++)
+            {
+                if (!kEdge) res[t] = *reinterpret_cast<const Quad<O>*>(r + t * kRows * f.ldr);
+                else if (m + t * kRows < f.rows)
+                {
+                    if (f.vec && left >= 4) res[t] = *reinterpret_cast<const Quad<O>*>(r + t * kRows * f.ldr);
+                    else
+                    {
+                        #pragma unroll
+                        for (int k = 0; k < 4; k++) if (k < left) res[t].v[k] = r[t * kRows * f.ldr + k];
+                    }
+                }
+            }
         };
         if (kRes) ask(0, 0);
         halves([&](auto h)
         {
-        cols.init(f, colOf(h.value));
-        exchange(h);
-        #pragma unroll 1
-        for (int pass = 0; pass < MT; pass++)
-        {
-            float scale[kTurns];
-            if (sizeof(T) == 1)
+            const int64_t n = colOf(h.value), left = f.cols - n;
+            cols.init(f, n);
+            exchange(h);
+            #pragma unroll 1
+            for (int pass = 0; pass < MT; pass++)
             {
-                #pragma unroll
-                for (int t = 0; t < kTurns; t++) scale[t] = f.qs[rowOf(pass) + t * kRows];
-            }
-            float v[kTurns][4], u[4];
-            #pragma unroll
-            for (int t = 0; t < kTurns; t++)
-            {
-                sumsOf(pass, t, v[t], u);
-                #pragma unroll
-                for (int k = 0; k < 4; k++)
+                const int64_t m = rowOf(pass);
+                float scale[kTurns];
+                if (sizeof(T) == 1)
                 {
-                    if (sizeof(T) == 1) v[t][k] *= scale[t] * cols.scale[k];
-                    v[t][k] = (v[t][k] + cols.bias[k]) * f.gain + (kRes ? row_load(res[t].v[k]) : 0.f);
+                    #pragma unroll
+                    for (int t = 0; t < kTurns; t++) scale[t] = !kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f;
                 }
+                float v[kTurns][4], u[4];
+                #pragma unroll
+                for (int t = 0; t < kTurns; t++)
+                {
+                    sumsOf(pass, t, v[t], u);
+                    #pragma unroll
+                    for (int k = 0; k < 4; k++)
+                    {
+                        if (sizeof(T) == 1) v[t][k] *= scale[t] * cols.scale[k];
+                        v[t][k] = (v[t][k] + cols.bias[k]) * f.gain + (kRes ? row_load(res[t].v[k]) : 0.f);
+                    }
+                }
+                if (kRes)
+                {
+                    if (pass + 1 < MT) ask(h.value, pass + 1);
+                    else if (h.value + 1 < NT / 2) ask(h.value + 1, 0);
+                }
+                O* to = static_cast<O*>(f.out) + m * f.ldo + n;
+                #pragma unroll
+                for (int t = 0; t < kTurns; t++)
+                    if (!kEdge || (m + t * kRows < f.rows && left > 0)) quad_store(to + t * kRows * f.ldo, kEdge ? left : 4, kEdge ? f.vec : true, v[t]);
             }
-            if (kRes)
-            {
-                if (pass + 1 < MT) ask(h.value, pass + 1);
-                else if (h.value + 1 < NT / 2) ask(h.value + 1, 0);
-            }
-            O* to = static_cast<O*>(f.out) + rowOf(pass) * f.ldo + colOf(h.value);
-            #pragma unroll
-            for (int t = 0; t < kTurns; t++) quad_store(to + t * kRows * f.ldo, 4, true, v[t]);
-        }
         });
     };
-    auto gate = [&](auto withSlopes)
+    auto gate = [&](auto withSlopes, auto atEdge)
     {
-        constexpr bool kSlopes = decltype(withSlopes)::value != 0;
+        constexpr bool kSlopes = decltype(withSlopes)::value != 0, kEdge = decltype(atEdge)::value != 0;
         halves([&](auto h)
         {
-        cols.init(f, colOf(h.value));
-        exchange(h);
-        #pragma unroll 1
-        for (int pass = 0; pass < MT; pass++)
-        {
-            float scale[kTurns];
-            if (sizeof(T) == 1)
+            const int64_t n = colOf(h.value), left = f.cols - n;
+            cols.init(f, n);
+            exchange(h);
+            #pragma unroll 1
+            for (int pass = 0; pass < MT; pass++)
             {
+                const int64_t m = rowOf(pass);
+                float scale[kTurns];
+                if (sizeof(T) == 1)
+                {
+                    #pragma unroll
+                    for (int t = 0; t < kTurns; t++) scale[t] = !kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f;
+                }
+                O* to = static_cast<O*>(f.out) + m * f.ldo + n;
+                float* slopes = kSlopes ? static_cast<float*>(f.slopes) + m * 2 * f.cols + n : nullptr;
+                float v[kTurns][4], u[kTurns][4];
                 #pragma unroll
-                for (int t = 0; t < kTurns; t++) scale[t] = f.qs[rowOf(pass) + t * kRows];
+                for (int t = 0; t < kTurns; t++) sumsOf(pass, t, v[t], u[t]);
+                #pragma unroll
+                for (int t = 0; t < kTurns; t++)
+                {
+                    float act[4], d[4];
+                    #pragma unroll
+                    for (int k = 0; k < 4; k++)
+                    {
+                        if (sizeof(T) == 1) { v[t][k] *= scale[t] * cols.scale[k]; u[t][k] *= scale[t] * cols.scaleUp[k]; }
+                        v[t][k] += cols.bias[k];
+                        u[t][k] += cols.biasUp[k];
+                    }
+                    act4<LVG_ACT_SWISH, sizeof(O) == 2>(LVG_ACT_SWISH, 0.f, v[t], kSlopes, act, d);
+                    #pragma unroll
+                    for (int k = 0; k < 4; k++)
+                    {
+                        act[k] *= f.gain;               // dh/du
+                        d[k] *= u[t][k] * f.gain;       // dh/dg
+                        v[t][k] = act[k] * u[t][k];
+                    }
+                    if (kEdge && (m + t * kRows >= f.rows || left <= 0)) continue;
+                    if (kSlopes)
+                    {
+                        quad_store(slopes + t * kRows * 2 * f.cols, kEdge ? left : 4, kEdge ? f.vec : true, d);
+                        quad_store(slopes + t * kRows * 2 * f.cols + f.cols, kEdge ? left : 4, kEdge ? f.vec : true, act);
+                    }
+                    quad_store(to + t * kRows * f.ldo, kEdge ? left : 4, kEdge ? f.vec : true, v[t]);
+                }
             }
-            O* to = static_cast<O*>(f.out) + rowOf(pass) * f.ldo + colOf(h.value);
-            float* slopes = kSlopes ? static_cast<float*>(f.slopes) + rowOf(pass) * 2 * f.cols + colOf(h.value) : nullptr;
-            float v[kTurns][4], u[kTurns][4];
-            #pragma unroll
-            for (int t = 0; t < kTurns; t++) sumsOf(pass, t, v[t], u[t]);
-            #pragma unroll
-            for (int t = 0; t < kTurns; t++)
-            {
-                float act[4], d[4];
-                #pragma unroll
-                for (int k = 0; k < 4; k++)
-                {
-                    if (sizeof(T) == 1) { v[t][k] *= scale[t] * cols.scale[k]; u[t][k] *= scale[t] * cols.scaleUp[k]; }
-                    v[t][k] += cols.bias[k];
-                    u[t][k] += cols.biasUp[k];
-                }
-                act4<LVG_ACT_SWISH, sizeof(O) == 2>(LVG_ACT_SWISH, 0.f, v[t], kSlopes, act, d);
-                #pragma unroll
-                for (int k = 0; k < 4; k++)
-                {
-                    act[k] *= f.gain;               // dh/du
-                    d[k] *= u[t][k] * f.gain;       // dh/dg
-                    v[t][k] = act[k] * u[t][k];
-                }
-                if (kSlopes)
-                {
-                    quad_store(slopes + t * kRows * 2 * f.cols, 4, true, d);
-                    quad_store(slopes + t * kRows * 2 * f.cols + f.cols, 4, true, act);
-                }
-                quad_store(to + t * kRows * f.ldo, 4, true, v[t]);
-            }
-        }
         });
     };
     if constexpr (GATED)
     {
-        if (whole && f.act == LVG_ACT_SWISH)
+        if (f.act == LVG_ACT_SWISH)
         {
-            if (f.slopeKind == LVG_SLOPE_F32) gate(Const<1>());
-            else gate(Const<0>());
+            if (f.slopeKind == LVG_SLOPE_F32) { if (inside) gate(Const<1>(), Const<0>()); else gate(Const<1>(), Const<1>()); }
+            else                              { if (inside) gate(Const<0>(), Const<0>()); else gate(Const<0>(), Const<1>()); }
             return;
         }
     }
-    else if (whole && f.act == LVG_ACT_LINEAR && f.slopeKind == LVG_SLOPE_NONE && f.clamp < 0.f)
+    else if (f.act == LVG_ACT_LINEAR && f.slopeKind == LVG_SLOPE_NONE && f.clamp < 0.f)
     {
-        if (f.residual) straight(Const<1>());
-        else straight(Const<0>());
+        if (f.residual) { if (inside) straight(Const<1>(), Const<0>()); else straight(Const<1>(), Const<1>()); }
+        else            { if (inside) straight(Const<0>(), Const<0>()); else straight(Const<0>(), Const<1>()); }
         return;
     }
 
-    // every other activation, and the tiles at the result's edges
+    // Every other activation, one turn at a time; a turn's residual is asked for before the turn ahead of it stores.
     halves([&](auto h)
     {
-    const int64_t n = colOf(h.value), left = f.cols - n;
-    cols.init(f, n);
-    exchange(h);
-    #pragma unroll 1
-    for (int pass = 0; pass < MT; pass++)
-    {
-        const int64_t m = rowOf(pass);
-        float res[kTurns][4];
-        #pragma unroll
-        for (int t = 0; t < kTurns; t++)
+        const int64_t n = colOf(h.value), left = f.cols - n;
+        cols.init(f, n);
+        exchange(h);
+        #pragma unroll 1
+        for (int pass = 0; pass < MT; pass++)
         {
-            #pragma unroll
-            for (int k = 0; k < 4; k++) res[t][k] = 0.f;
-            if (!GATED && f.residual && m + t * kRows < f.rows && left > 0)
-                quad_load(static_cast<const O*>(f.residual) + (m + t * kRows) * f.ldr + n, left, f.vec, res[t]);
+            const int64_t m = rowOf(pass);
+            const Place<O> at(f, m, n, GATED);
+            float next[4] = {0.f, 0.f, 0.f, 0.f};
+            auto ask = [&](int t)
+            {
+                if (!GATED && f.residual && m + t * kRows < f.rows && left > 0)
+                    quad_load(static_cast<const O*>(f.residual) + (m + t * kRows) * f.ldr + n, left, f.vec, next);
+            };
+            ask(0);
+            #pragma unroll 1
+            for (int t = 0; t < kTurns; t++)
+            {
+                float v[4], u[4], res[4];
+                sumsOf(pass, t, v, u);
+                #pragma unroll
+                for (int k = 0; k < 4; k++) res[k] = next[k];
+                if (t + 1 < kTurns) ask(t + 1);
+                if (m + t * kRows >= f.rows || left <= 0) continue;
+                cols.apply(f, m + t * kRows, v, u);
+                finish4<O, GATED>(f, at.down(f, t * kRows, GATED), v, u, res);
+            }
         }
-        const Place<O> at(f, m, n, GATED);
-        #pragma unroll
-        for (int t = 0; t < kTurns; t++)
-        {
-            float v[4], u[4];
-            sumsOf(pass, t, v, u);
-            if (m + t * kRows >= f.rows || left <= 0) continue;
-            cols.apply(f, m + t * kRows, v, u);
-            finish4<O, GATED>(f, at.down(f, t * kRows, GATED), v, u, res[t]);
-        }
-    }
     });
 }
 
 } // namespace
 
-// How a product is laid out over the chip (token_finish.hip); the same answer sizes the workspace and launches.
-struct TokenPlan { int tile, splits; };
 enum { LVG_TILE_256 = 0, LVG_TILE_128 = 1, LVG_TILE_64 = 2 };
-TokenPlan token_plan(int64_t rows, int64_t cols, int64_t inner, int esize, bool gated);
 
 // One launcher per operand type and kind of product, each in a file of its own (they are compiled side by side).
 enum { LVG_TOKEN_FORWARD = 0, LVG_TOKEN_GATED = 1, LVG_TOKEN_ROW_GRAD = 2, LVG_TOKEN_WEIGHT_GRAD = 3 };
@@ -719,12 +761,13 @@ template <class T, class O, int PL, int QL, bool GATED> int token_launch_form(in
     const int64_t blocks = (int64_t)a.tiles * a.splits;
     if (blocks > ((int64_t)1 << 22)) { lvg_set_error("token product: %lld workgroups", (long long)blocks); return LVG_ERR_INVALID; }
     const dim3 grid((unsigned)blocks);
-    #define LVG_TILE(ID, BM, BN, WR, WC) if (tile == ID) { \
+    #define LVG_TILE(ID, BM, BN, WR, WC, STAGED) if (tile == ID) { \
         if (direct) hipLaunchKernelGGL((token_gemm_kernel<T, O, BM, BN, WR, WC, PL, QL, GATED, true>), grid, dim3(WR * WC * 64), 0, s, a); \
-        else        hipLaunchKernelGGL((token_gemm_kernel<T, O, BM, BN, WR, WC, PL, QL, GATED, false>), grid, dim3(WR * WC * 64), 0, s, a); }
-    LVG_TILE(LVG_TILE_256, 256, 256, 2, 2)
-    LVG_TILE(LVG_TILE_128, 128, 128, 2, 2)
-    LVG_TILE(LVG_TILE_64, 64, 128, 2, 2)
+        else if constexpr (STAGED) hipLaunchKernelGGL((token_gemm_kernel<T, O, BM, BN, WR, WC, PL, QL, GATED, false>), grid, dim3(WR * WC * 64), 0, s, a); \
+        else { lvg_set_error("token product: no such kernel"); return LVG_ERR_INVALID; } }
+    LVG_TILE(LVG_TILE_256, 256, 256, 2, 2, sizeof(T) != 1)
+    LVG_TILE(LVG_TILE_128, 128, 128, 2, 2, true)
+    LVG_TILE(LVG_TILE_64, 64, 128, 2, 2, true)
     #undef LVG_TILE
     return lvg_check_launch("token product");
 }

@@ -86,7 +86,7 @@ _SIGNATURES = {
     'lvg_linear_slope': [_vp] * 4 + [_i64] * 4 + [_i32] * 3 + [_f32] * 2 + [_i32, _vp],
     'lvg_column_sum': [_vp, _vp, _i32, _i64, _f32, _i32, _vp],
     'lvg_linear_grad_work': [_i64] * 3 + [_i32] * 2,
-    'lvg_linear_grad': [_vp] * 4 + [_i64] * 6 + [_i32, _f32, _i32, _vp],
+    'lvg_linear_grad': [_vp] * 4 + [_i64] * 6 + [_i32, _i32, _f32, _i32, _vp],
     'lvg_rms_norm': [_vp] * 7 + [_i64] * 4 + [_f32, _i32, _i32, _vp],
     'lvg_rms_norm_backward_slots': [_i64] * 2 + [_i32],
     'lvg_rms_norm_backward': [_vp] * 8 + [_i64] * 5 + [_i32, _i32, _vp],

@@ -130,8 +130,9 @@ def _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_sc
     return y, slopes
 
 
-def _grad_product(dz, dz_stride, other, rows, outer, inner, weight, gain, dtype):
-    """dz [rows, outer] against the weight [outer, inner] (weight False) or the rows [rows, inner] (True)."""
+def _grad_product(dz, dz_stride, dz_whole, other, rows, outer, inner, weight, gain, dtype):
+    """dz [rows, outer] against the weight [outer, inner] (weight False) or the rows [rows, inner] (True); dz_whole: dz's rows are readable up to
+    their stride."""
     device = other.device
     grad = torch.empty((outer if weight else rows, inner), dtype=dtype, device=device)
     if inner == 0:
@@ -140,7 +141,7 @@ def _grad_product(dz, dz_stride, other, rows, outer, inner, weight, gain, dtype)
     size = _rows.query('lvg_linear_grad_work', rows, outer, inner, int(weight), code)
     work = _rows.work_of(size, device)
     _rows.launch(device, 'lvg_linear_grad', dz.data_ptr(), other.data_ptr(), grad.data_ptr(), None if work is None else work.data_ptr(), size,
-                 rows, outer, inner, dz_stride, _rows.row_stride(other), int(weight), gain, code)
+                 rows, outer, inner, dz_stride, _rows.row_stride(other), int(dz_whole), int(weight), gain, code)
     return grad
 
 
@@ -173,9 +174,9 @@ def _backward(dy, x, weight, slopes, kind, halves, alpha, gain, need_x, need_w, 
             db = _rows.column_sum(part, dtype, gain if plain else 1.0)
     scale = gain if plain else 1.0
     if need_x:
-        dx = _grad_product(dz, dz_stride, w2, rows, total, inner, False, scale, dtype).view(x.shape)
+        dx = _grad_product(dz, dz_stride, not plain, w2, rows, total, inner, False, scale, dtype).view(x.shape)
     if need_w:
-        dw = _grad_product(dz, dz_stride, x2, rows, total, inner, True, scale, dtype)
+        dw = _grad_product(dz, dz_stride, not plain, x2, rows, total, inner, True, scale, dtype)
     return dx, dw, db
 
 

@@ -239,8 +239,8 @@ def test_refusals_of_the_c_entries_cpu():
         assert lib.lvg_last_error()
     assert linear(rows=0) == 0 and linear(outer=0) == 0
     assert lib.lvg_linear_act_work(-1, 4, 4, 2, 0) == -1 and lib.lvg_linear_act_work(4, 4, 4, 3, 0) == -1 and lib.lvg_linear_grad_work(4, 4, 4, 0, 4) == -1
-    grad = dict(dz=p, o=p, g=p, work=None, size=0, rows=4, outer=4, inner=4, ldz=4, ldo=4, weight=0, gain=1.0, dtype=2)
-    for kw in (dict(dtype=4), dict(dz=None), dict(o=None), dict(g=None), dict(rows=-1), dict(ldz=-1)):
+    grad = dict(dz=p, o=p, g=p, work=None, size=0, rows=4, outer=4, inner=4, ldz=4, ldo=4, whole=0, weight=0, gain=1.0, dtype=2)
+    for kw in (dict(dtype=4), dict(dz=None), dict(o=None), dict(g=None), dict(rows=-1), dict(ldz=-1), dict(ldz=3, whole=1)):
         assert lib.lvg_linear_grad(*{**grad, **kw}.values(), None) == -1, kw
     slots = lib.lvg_linear_slope_slots(4, 4, 1, 2)
     slope = dict(dy=p, s=p, dz=p, part=p, rows=4, outer=4, ldy=4, ldz=4, halves=1, kind=1, slots=slots, alpha=0.0, gain=1.0, dtype=2)
@@ -263,7 +263,7 @@ def test_refusals_of_the_c_entries_cpu():
 # rows, inner, outer: single values, less than a fragment, odd widths, one more than a tile, a summed index of one and of many steps (split over
 # the chip), and results of several tiles of every size
 SIZES = [(1, 1, 1), (1, 64, 64), (2, 7, 3), (3, 515, 5), (16, 1024, 96), (17, 130, 67), (33, 256, 128), (64, 2048, 16), (65, 63, 129), (129, 257, 515), (300, 64, 1000), (20, 9000, 40), (40, 9000, 40)]
-BIG = [(2100, 192, 2304), (1025, 200, 4113)]
+BIG = [(2100, 192, 2304), (1025, 200, 4113), (2100, 1021, 2311)]
 
 
 @pytest.mark.gpu
@@ -288,7 +288,7 @@ def test_linear_activations_gpu(act, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES)
-@pytest.mark.parametrize('size', [(1, 1, 1), (1, 64, 64), (3, 515, 5), (17, 130, 67), (33, 256, 128), (129, 257, 260), (20, 9000, 40), (40, 9000, 40), (1030, 136, 2100)])
+@pytest.mark.parametrize('size', [(1, 1, 1), (1, 64, 64), (3, 515, 5), (17, 130, 67), (33, 256, 128), (129, 257, 260), (20, 9000, 40), (40, 9000, 40), (1030, 136, 2100), (1530, 1037, 1301)])
 def test_gated_forward_and_gradients_gpu(size, dtype):
     m, k, n = size
     x, w = rand(m, k, seed=1, dtype=dtype), rand(2 * n, k, seed=2, dtype=dtype, scale=k ** -0.5)
@@ -397,7 +397,7 @@ def test_rows_behind_the_result_stay_as_they_are_gpu():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('out', [BF16, F16])
-@pytest.mark.parametrize('size', [(1, 1, 1), (1, 64, 64), (2, 7, 3), (3, 515, 5), (16, 1024, 96), (17, 130, 67), (65, 63, 129), (64, 4096, 16), (300, 128, 1000), (1030, 320, 2304)])
+@pytest.mark.parametrize('size', [(1, 1, 1), (1, 64, 64), (2, 7, 3), (3, 515, 5), (16, 1024, 96), (17, 130, 67), (65, 63, 129), (64, 4096, 16), (300, 128, 1000), (1030, 320, 2304), (1030, 2051, 1501)])
 def test_8bit_products_gpu(size, out):
     m, k, n = size
     (q, s), (qw, sw) = rn.quantize_rows(rand(m, k, seed=1)), rn.quantize_rows(rand(2 * n, k, seed=2, scale=k ** -0.5))
