@@ -535,7 +535,7 @@ int lvg_split32_stack(const float* x, void* out, int64_t pixels, int channels, i
  * act / alpha / gain / clamp as in lvg_bias_act (clamp < 0: none; a NaN stays a NaN). b, residual and y have type out_dtype, which is dtype,
  * or float16 / bfloat16 for LVG_E4M3 operands; those come with x_scale [rows] and w_scale [outer] (gated: [2 outer]) float32: the value of an
  * element is itself times its row's scale. b, residual, slopes may be NULL.
- * slopes receives what lvg_linear_slope multiplies gradients with: slope_kind 1: float32 [rows, outer] (gated [rows, 2 outer]: the derivatives
+ * slopes receives what lvg_linear_backward multiplies gradients with: slope_kind 1: float32 [rows, outer] (gated [rows, 2 outer]: the derivatives
  * with respect to the gate's and the up half's sums), 2: one byte an element (0: clamped, 1: alpha, 2: one; linear, relu and lrelu only), 0: none.
  * work: lvg_linear_act_work(...) bytes, 16-byte aligned (0 bytes: NULL will do); nothing in it outlives the call.
  */
@@ -546,27 +546,16 @@ int lvg_linear_act(const void* x, const void* w, const void* b, const void* resi
                    int dtype, int out_dtype, int gated, int act, int slope_kind, float alpha, float gain, float clamp, void* stream);
 
 /*
- * dz [rows, halves * outer] = dy [rows, outer] * slopes * gain   (slope_kind 0: dy * gain; 2: alpha stands for code 1), and the column sums of
- * dz by row ranges: db_part [slots, halves * outer] float32, slots = lvg_linear_slope_slots(...); lvg_column_sum adds them. dz may be NULL (sums
- * alone) and so may db_part.
+ * Gradients of lvg_linear_act from dy [rows, outer] and the slopes it left (halves: 1, or 2 for a gated unit; w has halves * outer rows):
+ *   dz = dy * slopes * gain  (slope_kind 0: dy * gain; 2: alpha stands for code 1),
+ *   dx [rows, inner] = dz . w,   dw [halves * outer, inner] = dz^T . x,   db [halves * outer] = column sums of dz.
+ * dx, dw, db are dense and have type dtype; those that are NULL are not computed. A gated unit's slopes hold its gain: pass gain 1.
+ * work: lvg_linear_backward_work(...) bytes, 16-byte aligned; grads: 1 (dx) | 2 (dw) | 4 (db) of those asked for.
  */
-int lvg_linear_slope_slots(int64_t rows, int64_t outer, int halves, int dtype);
-int lvg_linear_slope(const void* dy, const void* slopes, void* dz, float* db_part, int64_t rows, int64_t outer, int64_t dy_stride, int64_t dz_stride,
-                     int halves, int slope_kind, int slots, float alpha, float gain, int dtype, void* stream);
-
-/* out [width] (type dtype) = gain * sum over slots of part [slots, width] float32, in slot order within four interleaved runs. */
-int lvg_column_sum(const float* part, void* out, int slots, int64_t width, float gain, int dtype, void* stream);
-
-/*
- * The two products of the backward pass; grad is dense.
- *   weight == 0: grad [rows, inner]  = gain * dz [rows, outer] . other, other = w [outer, inner]
- *   weight == 1: grad [outer, inner] = gain * dz^T . other,             other = x [rows, inner]
- * dz_whole: every row of dz is readable for dz_stride elements (what lies behind `outer` is not used).
- * work: lvg_linear_grad_work(...) bytes, 16-byte aligned.
- */
-int64_t lvg_linear_grad_work(int64_t rows, int64_t outer, int64_t inner, int weight, int dtype);
-int lvg_linear_grad(const void* dz, const void* other, void* grad, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
-                    int64_t dz_stride, int64_t other_stride, int dz_whole, int weight, float gain, int dtype, void* stream);
+int64_t lvg_linear_backward_work(int64_t rows, int64_t outer, int64_t inner, int halves, int slope_kind, int grads, int dtype);
+int lvg_linear_backward(const void* dy, const void* slopes, const void* x, const void* w, void* dx, void* dw, void* db, void* work, int64_t work_size,
+                        int64_t rows, int64_t outer, int64_t inner, int64_t dy_stride, int64_t x_stride, int64_t w_stride,
+                        int halves, int slope_kind, float alpha, float gain, int dtype, void* stream);
 
 /*
  * s = x + residual;  y = weight * s / sqrt(mean(s^2) + eps)   over rows [rows, width], width >= 1. residual (and then sum = s rounded to dtype),
@@ -578,13 +567,13 @@ int lvg_rms_norm(const void* x, const void* residual, const void* weight, void* 
 
 /*
  * Gradient of lvg_rms_norm: with g = weight * dy, dx = rstd g - s rstd^3 mean(g s) + dsum (dsum: gradient of sum's other uses, or NULL); dx is also
- * the residual's gradient. dw_part [slots, width] float32 (or NULL), slots = lvg_rms_norm_backward_slots(...): the weight's gradient by row ranges,
- * added by lvg_column_sum. row_work: [rows] floats, used for rows of more than 32 KiB (NULL otherwise will do). dx is dense.
+ * the residual's gradient. dw [width] = sum over rows of dy s rstd (or NULL). dx and dw are dense, of type dtype.
+ * work: lvg_rms_norm_backward_work(...) bytes, 16-byte aligned; weight: whether dw is asked for.
  */
-int lvg_rms_norm_backward_slots(int64_t rows, int64_t width, int dtype);
-int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* rstd, void* dx, float* dw_part,
-                          float* row_work, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
-                          int slots, int dtype, void* stream);
+int64_t lvg_rms_norm_backward_work(int64_t rows, int64_t width, int weight, int dtype);
+int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* rstd, void* dx, void* dw,
+                          void* work, int64_t work_size, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
+                          int dtype, void* stream);
 
 /* q [rows, width] e4m3 = x / scale, scale [rows] = max |x| of the row / 448 (2^-64 at least). q is dense. */
 int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t width, int64_t x_stride, int dtype, void* stream);

@@ -532,41 +532,42 @@ extern "C" int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t r
     return lvg_check_launch("lvg_quantize_rows");
 }
 
-extern "C" int lvg_rms_norm_backward_slots(int64_t rows, int64_t width, int dtype)
+extern "C" int64_t lvg_rms_norm_backward_work(int64_t rows, int64_t width, int weight, int dtype)
 {
-    return row_type(dtype) && rows_ok(rows, width) && rows > 0 ? back_slots(rows, width, dtype) : 0;
+    if (!row_type(dtype) || !rows_ok(rows, width)) return LVG_ERR_INVALID;
+    if (rows == 0) return 0;
+    return (back_plan(width, dtype).waves ? 0 : (rows + 3) / 4 * 16) + (weight ? (int64_t)back_slots(rows, width, dtype) * width * 4 : 0);
 }
 
-extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s_in, const void* weight, const float* rstd, void* dx, float* dw_part,
-                                     float* row_work, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
-                                     int slots, int dtype, void* stream)
+extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s_in, const void* weight, const float* rstd, void* dx, void* dw,
+                                     void* work, int64_t work_size, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
+                                     int dtype, void* stream)
 {
     LVG_REQUIRE(row_type(dtype), "lvg_rms_norm_backward: float32 / float16 / bfloat16 only (dtype %d)", dtype);
     LVG_REQUIRE(rows_ok(rows, width), "lvg_rms_norm_backward: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
     if (rows == 0) return LVG_OK;
     const Plan k = back_plan(width, dtype);
-    LVG_REQUIRE(dy && s_in && rstd && dx && (k.waves || row_work), "lvg_rms_norm_backward: missing pointer");
+    const int64_t need = lvg_rms_norm_backward_work(rows, width, dw != nullptr, dtype);
+    LVG_REQUIRE(dy && s_in && rstd && dx, "lvg_rms_norm_backward: missing pointer");
+    LVG_REQUIRE(need == 0 || (work && lvg_aligned16(work) && work_size >= need), "lvg_rms_norm_backward: the workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
     LVG_REQUIRE(k.waves || rows <= kLaunchRows, "lvg_rms_norm_backward: more than %lld rows of %lld values", (long long)kLaunchRows, (long long)width);
     LVG_REQUIRE(dy_stride >= 0 && dsum_stride >= 0 && s_stride >= 0, "lvg_rms_norm_backward: negative row stride");
-    LVG_REQUIRE(slots == back_slots(rows, width, dtype), "lvg_rms_norm_backward: slots must be lvg_rms_norm_backward_slots(...) (= %d)", back_slots(rows, width, dtype));
-    NormBackArgs a = {dy, dsum, s_in, weight, rstd, dx, dw_part, row_work, rows, width, dy_stride, dsum_stride, s_stride};
+    const int slots = back_slots(rows, width, dtype);
+    float* const coef = k.waves ? nullptr : static_cast<float*>(work);
+    float* const part = dw ? static_cast<float*>(work) + (k.waves ? 0 : (rows + 3) / 4 * 4) : nullptr;
+    NormBackArgs a = {dy, dsum, s_in, weight, rstd, dx, part, coef, rows, width, dy_stride, dsum_stride, s_stride};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) launch_back<float>(a, k, slots, s);
     else if (dtype == LVG_F16) launch_back<f16_t>(a, k, slots, s);
     else launch_back<bf16_t>(a, k, slots, s);
+    if (dw) row_column_sum(part, dw, slots, width, 1.f, dtype, s);
     return lvg_check_launch("lvg_rms_norm_backward");
 }
 
-extern "C" int lvg_column_sum(const float* part, void* out, int slots, int64_t width, float gain, int dtype, void* stream)
+void row_column_sum(const float* part, void* out, int slots, int64_t width, float gain, int dtype, hipStream_t s)
 {
-    LVG_REQUIRE(row_type(dtype), "lvg_column_sum: float32 / float16 / bfloat16 only (dtype %d)", dtype);
-    LVG_REQUIRE(slots >= 0 && width >= 0 && width <= ((int64_t)1 << 36), "lvg_column_sum: bad size");
-    if (width == 0) return LVG_OK;
-    LVG_REQUIRE((part || slots == 0) && out, "lvg_column_sum: missing pointer");
     const dim3 grid((unsigned)lvg_ceil_div(width, 32)), block(256);
-    hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) hipLaunchKernelGGL(column_sum_kernel<float>, grid, block, 0, s, part, static_cast<float*>(out), slots, width, gain);
     else if (dtype == LVG_F16) hipLaunchKernelGGL(column_sum_kernel<f16_t>, grid, block, 0, s, part, static_cast<f16_t*>(out), slots, width, gain);
     else hipLaunchKernelGGL(column_sum_kernel<bf16_t>, grid, block, 0, s, part, static_cast<bf16_t*>(out), slots, width, gain);
-    return lvg_check_launch("lvg_column_sum");
 }

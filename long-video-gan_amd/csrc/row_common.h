@@ -96,3 +96,6 @@ __device__ __forceinline__ float row_scale(uint32_t largest)
 }
 
 } // namespace
+
+// out [width] (type dtype) = gain * sum over the slots of part [slots][width] (rms_norm.hip).
+void row_column_sum(const float* part, void* out, int slots, int64_t width, float gain, int dtype, hipStream_t s);

@@ -428,21 +428,14 @@ extern "C" int lvg_linear_act(const void* x, const void* w, const void* b, const
     return run_product(a, gated ? LVG_TOKEN_GATED : LVG_TOKEN_FORWARD, dtype, out_dtype, work, work_size, static_cast<hipStream_t>(stream), "lvg_linear_act");
 }
 
-extern "C" int64_t lvg_linear_grad_work(int64_t rows, int64_t outer, int64_t inner, int weight, int dtype)
-{
-    if (!float_type(dtype) || !size_ok(rows) || !size_ok(outer) || !size_ok(inner)) return LVG_ERR_INVALID;
-    if (inner == 0 || (weight ? outer : rows) == 0) return 0;
-    return weight ? work_bytes(outer, inner, rows, dtype, LVG_TOKEN_WEIGHT_GRAD) : work_bytes(rows, inner, outer, dtype, LVG_TOKEN_ROW_GRAD);
-}
+namespace {
 
-extern "C" int lvg_linear_grad(const void* dz, const void* other, void* grad, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
-                               int64_t dz_stride, int64_t other_stride, int dz_whole, int weight, float gain, int dtype, void* stream)
+// One of the two products of the backward pass: grad = gain * dz . w (weight false) or gain * dz^T . x. dz_whole: dz's rows are readable up to
+// their stride.
+int grad_product(const void* dz, int64_t dz_stride, bool dz_whole, const void* other, int64_t other_stride, void* grad, void* work, int64_t work_size,
+                 int64_t rows, int64_t outer, int64_t inner, bool weight, float gain, int dtype, hipStream_t s)
 {
-    LVG_REQUIRE(float_type(dtype), "lvg_linear_grad: float32 / float16 / bfloat16 only (dtype %d)", dtype);
-    LVG_REQUIRE(size_ok(rows) && size_ok(outer) && size_ok(inner), "lvg_linear_grad: bad size");
-    if (inner == 0 || (weight ? outer : rows) == 0) return LVG_OK;
-    LVG_REQUIRE(grad && ((weight ? rows : outer) == 0 || (dz && other)), "lvg_linear_grad: missing pointer");
-    LVG_REQUIRE(dz_stride >= 0 && other_stride >= 0 && (!dz_whole || dz_stride >= outer), "lvg_linear_grad: bad row stride");
+    if (inner == 0) return LVG_OK;
     TokenArgs a;
     memset(&a, 0, sizeof(a));
     const int es = esize_of(dtype);
@@ -453,32 +446,75 @@ extern "C" int lvg_linear_grad(const void* dz, const void* other, void* grad, vo
     Finish& f = a.fin;
     f.out = grad; f.ldo = inner; f.rows = a.qRows; f.cols = inner;
     f.act = LVG_ACT_LINEAR; f.gain = gain; f.clamp = -1.f;
-    return run_product(a, weight ? LVG_TOKEN_WEIGHT_GRAD : LVG_TOKEN_ROW_GRAD, dtype, dtype, work, work_size, static_cast<hipStream_t>(stream), "lvg_linear_grad");
+    return run_product(a, weight ? LVG_TOKEN_WEIGHT_GRAD : LVG_TOKEN_ROW_GRAD, dtype, dtype, work, work_size, s, "lvg_linear_backward");
 }
 
-extern "C" int lvg_linear_slope_slots(int64_t rows, int64_t outer, int halves, int dtype)
+// Workspace of a backward pass: dz (rows that start at multiples of 16 bytes whatever the width: both products read them as they like it best),
+// the column sums by row ranges, and what the larger of the two products needs (they follow one another on the stream).
+struct BackWork { int64_t dz, dzStride, part, product, all; int slots; };
+
+BackWork back_work(int64_t rows, int64_t outer, int64_t inner, int halves, int kind, bool dx, bool dw, bool db, int dtype)
 {
-    if (!float_type(dtype) || !size_ok(rows) || !size_ok(outer) || rows == 0 || outer == 0 || (halves != 1 && halves != 2)) return 0;
-    return slope_slots(rows, outer, esize_of(dtype));
+    const int es = esize_of(dtype);
+    BackWork w = {0, pad16(outer * halves * es) / es, 0, 0, 0, 0};
+    w.slots = slope_slots(rows, outer, es);
+    if (kind != LVG_SLOPE_NONE) w.dz = rows * w.dzStride * es;
+    if (db) w.part = pad16((int64_t)w.slots * halves * outer * 4);
+    if (dx && inner) w.product = work_bytes(rows, inner, outer * halves, dtype, LVG_TOKEN_ROW_GRAD);
+    if (dw && inner) w.product = std::max(w.product, work_bytes(outer * halves, inner, rows, dtype, LVG_TOKEN_WEIGHT_GRAD));
+    w.all = w.dz + w.part + w.product;
+    return w;
 }
 
-extern "C" int lvg_linear_slope(const void* dy, const void* slopes, void* dz, float* db_part, int64_t rows, int64_t outer, int64_t dy_stride, int64_t dz_stride,
-                                int halves, int slope_kind, int slots, float alpha, float gain, int dtype, void* stream)
+bool back_sizes(int64_t rows, int64_t outer, int64_t inner, int halves, int kind, int dtype)
 {
-    LVG_REQUIRE(float_type(dtype), "lvg_linear_slope: float32 / float16 / bfloat16 only (dtype %d)", dtype);
-    LVG_REQUIRE(size_ok(rows) && size_ok(outer) && (halves == 1 || halves == 2), "lvg_linear_slope: bad size");
+    return float_type(dtype) && size_ok(rows) && size_ok(outer) && size_ok(inner) && (halves == 1 || halves == 2) && size_ok(outer * halves) &&
+           (kind == LVG_SLOPE_NONE || kind == LVG_SLOPE_F32 || kind == LVG_SLOPE_CODE) && (halves == 1 || kind == LVG_SLOPE_F32);
+}
+
+} // namespace
+
+extern "C" int64_t lvg_linear_backward_work(int64_t rows, int64_t outer, int64_t inner, int halves, int slope_kind, int grads, int dtype)
+{
+    if (!back_sizes(rows, outer, inner, halves, slope_kind, dtype)) return LVG_ERR_INVALID;
+    return rows && outer ? back_work(rows, outer, inner, halves, slope_kind, grads & 1, grads & 2, grads & 4, dtype).all : 0;
+}
+
+extern "C" int lvg_linear_backward(const void* dy, const void* slopes, const void* x, const void* w, void* dx, void* dw, void* db, void* work, int64_t work_size,
+                                   int64_t rows, int64_t outer, int64_t inner, int64_t dy_stride, int64_t x_stride, int64_t w_stride,
+                                   int halves, int slope_kind, float alpha, float gain, int dtype, void* stream)
+{
+    LVG_REQUIRE(back_sizes(rows, outer, inner, halves, slope_kind, dtype), "lvg_linear_backward: bad size, type or slopes");
     if (rows == 0 || outer == 0) return LVG_OK;
-    LVG_REQUIRE(dy && (dz || db_part), "lvg_linear_slope: missing pointer");
-    LVG_REQUIRE(slope_kind == LVG_SLOPE_NONE ? halves == 1 : (slopes && (slope_kind == LVG_SLOPE_F32 || (slope_kind == LVG_SLOPE_CODE && halves == 1))), "lvg_linear_slope: bad slopes");
-    LVG_REQUIRE(dy_stride >= 0 && (!dz || dz_stride >= outer * halves), "lvg_linear_slope: bad row stride");
-    LVG_REQUIRE(slots == slope_slots(rows, outer, esize_of(dtype)), "lvg_linear_slope: slots must be lvg_linear_slope_slots(...)");
-    SlopeArgs a = {dy, slopes, dz, db_part, rows, outer, dy_stride, dz_stride, slope_kind, slope_lanes(outer, esize_of(dtype)), alpha, gain};
-    const dim3 grid((unsigned)lvg_ceil_div(lvg_ceil_div(outer, 16 / esize_of(dtype)), a.lanes), (unsigned)slots), block(256);
+    LVG_REQUIRE(dy && (slope_kind == LVG_SLOPE_NONE || slopes) && (!dx || inner == 0 || w) && (!dw || inner == 0 || x), "lvg_linear_backward: missing pointer");
+    LVG_REQUIRE(dy_stride >= 0 && x_stride >= 0 && w_stride >= 0, "lvg_linear_backward: negative row stride");
+    const BackWork k = back_work(rows, outer, inner, halves, slope_kind, dx != nullptr, dw != nullptr, db != nullptr, dtype);
+    LVG_REQUIRE(k.all == 0 || (work && lvg_aligned16(work) && work_size >= k.all), "lvg_linear_backward: the workspace must be 16-byte aligned and hold %lld bytes", (long long)k.all);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    #define LVG_TYPE(T) { \
-        if (halves == 2) hipLaunchKernelGGL((token_slope_kernel<T, 2>), grid, block, 0, s, a); \
-        else             hipLaunchKernelGGL((token_slope_kernel<T, 1>), grid, block, 0, s, a); }
-    if (dtype == LVG_F32) LVG_TYPE(float) else if (dtype == LVG_F16) LVG_TYPE(f16_t) else LVG_TYPE(bf16_t)
-    #undef LVG_TYPE
-    return lvg_check_launch("lvg_linear_slope");
+    const bool plain = slope_kind == LVG_SLOPE_NONE;               // dy times the gain is the gradient of the sums
+    char* const mem = static_cast<char*>(work);
+    const void* dz = plain ? dy : mem;
+    const int64_t dzStride = plain ? dy_stride : k.dzStride, total = outer * halves;
+    if (!plain || db)
+    {
+        float* part = db ? reinterpret_cast<float*>(mem + k.dz) : nullptr;
+        SlopeArgs a = {dy, slopes, plain ? nullptr : mem, part, rows, outer, dy_stride, k.dzStride, slope_kind, slope_lanes(outer, esize_of(dtype)), alpha, plain ? 1.f : gain};
+        const dim3 grid((unsigned)lvg_ceil_div(lvg_ceil_div(outer, 16 / esize_of(dtype)), a.lanes), (unsigned)k.slots), block(256);
+        #define LVG_TYPE(T) { \
+            if (halves == 2) hipLaunchKernelGGL((token_slope_kernel<T, 2>), grid, block, 0, s, a); \
+            else             hipLaunchKernelGGL((token_slope_kernel<T, 1>), grid, block, 0, s, a); }
+        if (dtype == LVG_F32) LVG_TYPE(float) else if (dtype == LVG_F16) LVG_TYPE(f16_t) else LVG_TYPE(bf16_t)
+        #undef LVG_TYPE
+        if (db) row_column_sum(part, db, k.slots, total, plain ? gain : 1.f, dtype, s);
+        const int rc = lvg_check_launch("lvg_linear_backward");
+        if (rc != LVG_OK) return rc;
+    }
+    void* const pw = mem + k.dz + k.part;
+    if (dx)
+    {
+        const int rc = grad_product(dz, dzStride, !plain, w, w_stride, dx, pw, k.product, rows, total, inner, false, plain ? gain : 1.f, dtype, s);
+        if (rc != LVG_OK) return rc;
+    }
+    if (dw) return grad_product(dz, dzStride, !plain, x, x_stride, dw, pw, k.product, rows, total, inner, true, plain ? gain : 1.f, dtype, s);
+    return LVG_OK;
 }

@@ -63,11 +63,3 @@ def launch(device: torch.device, name: str, *args):
 def work_of(size: int, device: torch.device):
     """Workspace of a call, from the current stream's pool (a captured graph gets its own)."""
     return torch.empty(size, dtype=torch.uint8, device=device) if size > 0 else None
-
-
-def column_sum(part: torch.Tensor, dtype: torch.dtype, gain: float = 1.0) -> torch.Tensor:
-    """gain * part.sum(dim=0), part [slots, width] float32, on part's device and the current stream."""
-    slots, width = part.shape
-    out = torch.empty(width, dtype=dtype, device=part.device)
-    launch(part.device, 'lvg_column_sum', part.data_ptr(), out.data_ptr(), slots, width, gain, _CODES[dtype])
-    return out

@@ -130,53 +130,25 @@ def _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_sc
     return y, slopes
 
 
-def _grad_product(dz, dz_stride, dz_whole, other, rows, outer, inner, weight, gain, dtype):
-    """dz [rows, outer] against the weight [outer, inner] (weight False) or the rows [rows, inner] (True); dz_whole: dz's rows are readable up to
-    their stride."""
-    device = other.device
-    grad = torch.empty((outer if weight else rows, inner), dtype=dtype, device=device)
-    if inner == 0:
-        return grad
-    code = _rows.type_code(dtype)
-    size = _rows.query('lvg_linear_grad_work', rows, outer, inner, int(weight), code)
-    work = _rows.work_of(size, device)
-    _rows.launch(device, 'lvg_linear_grad', dz.data_ptr(), other.data_ptr(), grad.data_ptr(), None if work is None else work.data_ptr(), size,
-                 rows, outer, inner, dz_stride, _rows.row_stride(other), int(dz_whole), int(weight), gain, code)
-    return grad
-
-
 def _backward(dy, x, weight, slopes, kind, halves, alpha, gain, need_x, need_w, need_b):
     """Gradients of x, weight and b from dy [..., outer]; kind SLOPE_NONE: dy itself times the gain is the gradient of the sums."""
     total, inner = weight.shape
     outer = total // halves
-    x2, w2, dz = _rows.rows_of(x, inner), _rows.rows_of(weight, inner), _rows.rows_of(dy, outer)
+    x2, w2, dy2 = _rows.rows_of(x, inner), _rows.rows_of(weight, inner), _rows.rows_of(dy, outer)
     rows, dtype, device = x2.shape[0], x.dtype, x.device
     if rows == 0 or outer == 0:
         # nothing to sum over
         return (x2.new_zeros(x.shape) if need_x else None, w2.new_zeros(weight.shape) if need_w else None, w2.new_zeros(total) if need_b else None)
-    dx = dw = db = None
-    plain, dz_stride = kind == SLOPE_NONE, _rows.row_stride(dz)
-    if not plain or need_b:
-        code = _rows.type_code(dtype)
-        slots = _rows.query('lvg_linear_slope_slots', rows, outer, halves, code)
-        part = torch.empty((slots, total), dtype=torch.float32, device=device) if need_b else None
-        into, stride = None, total
-        if not plain:
-            # rows of dz start at multiples of 16 bytes whatever the width: both products read them as they like it best
-            each = 16 // dtype.itemsize
-            stride = -(-total // each) * each
-            into = torch.empty((rows, stride), dtype=dtype, device=device)
-        _rows.launch(device, 'lvg_linear_slope', dz.data_ptr(), None if plain else slopes.data_ptr(), None if plain else into.data_ptr(),
-                     None if part is None else part.data_ptr(), rows, outer, dz_stride, stride, halves, kind, slots, alpha, 1.0 if plain else gain, code)
-        if not plain:
-            dz, dz_stride = into, stride
-        if need_b:
-            db = _rows.column_sum(part, dtype, gain if plain else 1.0)
-    scale = gain if plain else 1.0
-    if need_x:
-        dx = _grad_product(dz, dz_stride, not plain, w2, rows, total, inner, False, scale, dtype).view(x.shape)
-    if need_w:
-        dw = _grad_product(dz, dz_stride, not plain, x2, rows, total, inner, True, scale, dtype)
+    dx = torch.empty(x.shape, dtype=dtype, device=device) if need_x else None
+    dw = torch.empty((total, inner), dtype=dtype, device=device) if need_w else None
+    db = torch.empty(total, dtype=dtype, device=device) if need_b else None
+    code = _rows.type_code(dtype)
+    size = _rows.query('lvg_linear_backward_work', rows, outer, inner, halves, kind, need_x + 2 * need_w + 4 * need_b, code)
+    work = _rows.work_of(size, device)
+    _rows.launch(device, 'lvg_linear_backward', dy2.data_ptr(), None if slopes is None else slopes.data_ptr(), x2.data_ptr(), w2.data_ptr(),
+                 None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
+                 None if work is None else work.data_ptr(), size, rows, outer, inner, _rows.row_stride(dy2), _rows.row_stride(x2), _rows.row_stride(w2),
+                 halves, kind, alpha, gain, code)
     return dx, dw, db
 
 

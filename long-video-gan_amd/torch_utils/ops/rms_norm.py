@@ -127,14 +127,13 @@ class _RmsNorm(torch.autograd.Function):
             if rows == 0:
                 return dx, torch.zeros_like(weight) if need_w else None, dx if need_r else None, None
             code = _rows.type_code(s.dtype)
-            slots = _rows.query('lvg_rms_norm_backward_slots', rows, width, code)
-            part = torch.empty((slots, width), dtype=torch.float32, device=dev) if need_w else None
-            row_work = torch.empty(rows, dtype=torch.float32, device=dev)
+            if need_w:
+                dw = torch.empty(width, dtype=s.dtype, device=dev)
+            size = _rows.query('lvg_rms_norm_backward_work', rows, width, int(need_w), code)
+            work = _rows.work_of(size, dev)
             if weight is not None:
                 weight = weight.contiguous()
             _rows.launch(dev, 'lvg_rms_norm_backward', dy2.data_ptr(), None if ds2 is None else ds2.data_ptr(), s2.data_ptr(), None if weight is None else weight.data_ptr(),
-                         rstd.data_ptr(), dx.data_ptr(), None if part is None else part.data_ptr(), row_work.data_ptr(), rows, width, _rows.row_stride(dy2),
-                         0 if ds2 is None else _rows.row_stride(ds2), _rows.row_stride(s2), slots, code)
-            if need_w:
-                dw = _rows.column_sum(part, s.dtype)
+                         rstd.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(), None if work is None else work.data_ptr(), size, rows, width,
+                         _rows.row_stride(dy2), 0 if ds2 is None else _rows.row_stride(ds2), _rows.row_stride(s2), code)
         return dx if need_x else None, dw, dx if need_r else None, None

@@ -238,23 +238,24 @@ def test_refusals_of_the_c_entries_cpu():
         assert linear(**kw) == -1, kw
         assert lib.lvg_last_error()
     assert linear(rows=0) == 0 and linear(outer=0) == 0
-    assert lib.lvg_linear_act_work(-1, 4, 4, 2, 0) == -1 and lib.lvg_linear_act_work(4, 4, 4, 3, 0) == -1 and lib.lvg_linear_grad_work(4, 4, 4, 0, 4) == -1
-    grad = dict(dz=p, o=p, g=p, work=None, size=0, rows=4, outer=4, inner=4, ldz=4, ldo=4, whole=0, weight=0, gain=1.0, dtype=2)
-    for kw in (dict(dtype=4), dict(dz=None), dict(o=None), dict(g=None), dict(rows=-1), dict(ldz=-1), dict(ldz=3, whole=1)):
-        assert lib.lvg_linear_grad(*{**grad, **kw}.values(), None) == -1, kw
-    slots = lib.lvg_linear_slope_slots(4, 4, 1, 2)
-    slope = dict(dy=p, s=p, dz=p, part=p, rows=4, outer=4, ldy=4, ldz=4, halves=1, kind=1, slots=slots, alpha=0.0, gain=1.0, dtype=2)
-    for kw in (dict(dtype=4), dict(dy=None), dict(s=None), dict(halves=3), dict(halves=2, kind=0, ldz=8), dict(halves=2, kind=2, ldz=8), dict(dz=None, part=None), dict(ldz=3), dict(slots=slots + 1)):
-        assert lib.lvg_linear_slope(*{**slope, **kw}.values(), None) == -1, kw
+    assert lib.lvg_linear_act_work(-1, 4, 4, 2, 0) == -1 and lib.lvg_linear_act_work(4, 4, 4, 3, 0) == -1
+    for bad in ((-1, 4, 4, 1, 0, 7, 2), (4, 4, 4, 3, 0, 7, 2), (4, 4, 4, 1, 3, 7, 2), (4, 4, 4, 2, 2, 7, 2), (4, 4, 4, 1, 0, 7, 4), (4, 1 << 30, 4, 2, 1, 7, 2)):
+        assert lib.lvg_linear_backward_work(*bad) == -1, bad
+    size = lib.lvg_linear_backward_work(4, 4, 4, 1, 1, 7, 2)
+    back = dict(dy=p, s=p, x=p, w=p, dx=p, dw=p, db=p, work=p, size=size, rows=4, outer=4, inner=4, ldy=4, ldx=4, ldw=4, halves=1, kind=1, alpha=0.0, gain=1.0, dtype=2)
+    for kw in (dict(dtype=4), dict(dy=None), dict(s=None), dict(x=None), dict(w=None), dict(work=None), dict(work=p + 8), dict(size=size - 1), dict(rows=-1), dict(halves=3),
+               dict(halves=2, kind=0), dict(halves=2, kind=2), dict(kind=5), dict(ldy=-1), dict(ldx=-1), dict(ldw=-1)):
+        assert lib.lvg_linear_backward(*{**back, **kw}.values(), None) == -1, kw
+    assert lib.lvg_linear_backward(*{**back, 'rows': 0}.values(), None) == 0
     norm = dict(x=p, r=None, w=None, y=p, s=None, rstd=None, scale=None, rows=4, width=4, ldx=4, ldr=0, eps=0.0, dtype=2, quant=0)
     for kw in (dict(dtype=3), dict(x=None), dict(y=None), dict(quant=1), dict(s=p), dict(rows=-1), dict(width=0), dict(ldx=-1), dict(eps=-1.0), dict(eps=math.nan)):
         assert lib.lvg_rms_norm(*{**norm, **kw}.values(), None) == -1, kw
-    slots = lib.lvg_rms_norm_backward_slots(4, 4, 2)
-    back = dict(dy=p, ds=None, s=p, w=None, rstd=p, dx=p, part=p, work=None, rows=4, width=4, lddy=4, ldds=0, lds=4, slots=slots, dtype=2)
-    for kw in (dict(dtype=4), dict(dy=None), dict(rstd=None), dict(dx=None), dict(slots=slots + 1), dict(lds=-1)):
+    assert lib.lvg_rms_norm_backward_work(4, 0, 1, 2) == -1 and lib.lvg_rms_norm_backward_work(-1, 4, 1, 2) == -1 and lib.lvg_rms_norm_backward_work(4, 4, 1, 4) == -1
+    size = lib.lvg_rms_norm_backward_work(4, 4, 1, 2)
+    back = dict(dy=p, ds=None, s=p, w=None, rstd=p, dx=p, dw=p, work=p, size=size, rows=4, width=4, lddy=4, ldds=0, lds=4, dtype=2)
+    for kw in (dict(dtype=4), dict(dy=None), dict(rstd=None), dict(dx=None), dict(s=None), dict(work=None), dict(work=p + 4), dict(size=size - 1), dict(lds=-1), dict(lddy=-1)):
         assert lib.lvg_rms_norm_backward(*{**back, **kw}.values(), None) == -1, kw
     assert lib.lvg_quantize_rows(p, p, None, 4, 4, 4, 2, None) == -1 and lib.lvg_quantize_rows(p, p, p, 4, 0, 4, 2, None) == -1
-    assert lib.lvg_column_sum(None, p, 2, 4, 1.0, 2, None) == -1 and lib.lvg_column_sum(p, p, 2, 4, 1.0, 3, None) == -1
 
 
 # --------------------------------------------------------------------------------------------------------------------
