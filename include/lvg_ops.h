@@ -560,18 +560,20 @@ int lvg_linear_backward(const void* dy, const void* slopes, const void* x, const
 /*
  * s = x + residual;  y = weight * s / sqrt(mean(s^2) + eps)   over rows [rows, width], width >= 1. residual (and then sum = s rounded to dtype),
  * weight, rstd [rows] (the reciprocal root) may be NULL. quantize == 0: y has type dtype; 1: y is e4m3 bytes and scale [rows] = max |y| / 448 of the
- * row (2^-64 at least; a row with a NaN has a NaN scale), y = result / scale. y and sum are dense.
+ * row (2^-64 at least; a row with a NaN has a NaN scale), y = result / scale. y and sum are dense. rest [rows, ceil(width / 8)] uint16 (or NULL; not used
+ * for float32) keeps two bits of what each value of sum lost in its rounding, for the backward pass.
  */
-int lvg_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* sum, float* rstd, float* scale,
+int lvg_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* sum, void* rest, float* rstd, float* scale,
                  int64_t rows, int64_t width, int64_t x_stride, int64_t residual_stride, float eps, int dtype, int quantize, void* stream);
 
 /*
  * Gradient of lvg_rms_norm: with g = weight * dy, dx = rstd g - s rstd^3 mean(g s) + dsum (dsum: gradient of sum's other uses, or NULL); dx is also
- * the residual's gradient. dw [width] = sum over rows of dy s rstd (or NULL). dx and dw are dense, of type dtype.
+ * the residual's gradient. dw [width] = sum over rows of dy s rstd (or NULL). s, rest: the forward pass's sum and
+ * rest; x and NULL where it had no residual. dx and dw are dense, of type dtype.
  * work: lvg_rms_norm_backward_work(...) bytes, 16-byte aligned; weight: whether dw is asked for.
  */
 int64_t lvg_rms_norm_backward_work(int64_t rows, int64_t width, int weight, int dtype);
-int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s, const void* weight, const float* rstd, void* dx, void* dw,
+int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s, const void* rest, const void* weight, const float* rstd, void* dx, void* dw,
                           void* work, int64_t work_size, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
                           int dtype, void* stream);
 

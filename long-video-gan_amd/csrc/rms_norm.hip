@@ -5,7 +5,9 @@
 //   ds_in = r g - s r^3 mean(g s) + ds,   g = weight * dy,   dweight = sum over rows of dy s r
 //
 // What a program otherwise spells as add, square, mean, rsqrt, two products, an absolute maximum and a cast: eight passes over the rows where
-// one has to read x and residual and write s and y. One row is held in the registers of one wave (up to 8 vectors a lane) or of a workgroup of
+// one has to read x and residual and write s and y. The gradient reads the sum as it was stored, rounded; two bits a value that the forward pass
+// keeps beside it (a third of the rounding's half step up, down, or neither) bring it three times closer to what the norm was taken of, for 3 % of
+// the traffic: without them the weight's gradient is 1.5 times as far from the exact one as its own rounding makes it. One row is held in the registers of one wave (up to 8 vectors a lane) or of a workgroup of
 // four, so each value is read once and written once; the sums are float32 and their order is fixed. Rows of more than 4 x 64 x 8 vectors take
 // two passes over the row, the second of which finds it in L2.
 #include "row_common.h"
@@ -19,6 +21,7 @@ struct NormArgs
     const void*  weight;       // [width] or NULL
     void*        y;            // T, or e4m3 bytes
     void*        sum;          // T: x + residual, or NULL
+    uint16_t*    rest;         // [rows][ceil(width / 8)], 2 bits a value: what the sum's rounding left (16-bit T), or NULL
     float*       rstd;         // [rows] or NULL
     float*       scale;        // [rows], 8-bit results
     int64_t      rows, width, ldx, ldr, ldy;
@@ -30,6 +33,7 @@ struct NormBackArgs
     const void*  dy;
     const void*  ds;           // gradient of the sum's other uses, or NULL
     const void*  s;
+    const uint16_t* rest;      // as in NormArgs
     const void*  weight;
     const float* rstd;
     void*        dx;
@@ -37,6 +41,43 @@ struct NormBackArgs
     float*       coef;         // [rows]: wide rows only
     int64_t      rows, width, lddy, ldds, lds;
 };
+
+// What rounding v to T left, in units of two thirds of half a step: -1, 0 or 1 (+ 1). A half step is 2^(exponent - 8) (bfloat16) or - 11 (float16).
+template <class T> __device__ __forceinline__ float half_step(float rounded)
+{
+    return __uint_as_float(__float_as_uint(rounded) & 0x7f800000u) * (sizeof(T) == 4 ? 0.f : __is_same(T, bf16_t) ? 0.00390625f : 0.00048828125f);
+}
+template <class T> __device__ __forceinline__ uint32_t rest_code(float v)
+{
+    const float r = to_acc(from_acc<T>(v)), left = v - r, third = half_step<T>(r) * (1.f / 3.f);
+    return left > third ? 2u : left < -third ? 0u : 1u;
+}
+template <class T> __device__ __forceinline__ float with_rest(float rounded, uint32_t code)
+{
+    return code == 1u ? rounded : fmaf((float)(int)(code - 1u), half_step<T>(rounded) * (2.f / 3.f), rounded);
+}
+template <class T> __device__ __forceinline__ void store_rest(const NormArgs& p, int64_t row, int64_t at, const float* v)
+{
+    if constexpr (sizeof(T) == 2)
+    {
+        if (!p.rest || at >= p.width) return;
+        uint32_t w = 0;
+        #pragma unroll
+        for (int i = 0; i < 8; i++) w |= rest_code<T>(v[i]) << (2 * i);
+        p.rest[row * ((p.width + 7) / 8) + at / 8] = (uint16_t)w;
+    }
+}
+// the sum's values at `at` (a multiple of the vector), as close as they are kept
+template <class T> __device__ __forceinline__ void kept_sum(const NormBackArgs& p, int64_t row, int64_t at, float* v)
+{
+    if constexpr (sizeof(T) == 2)
+    {
+        if (!p.rest || at >= p.width) return;
+        const uint32_t w = p.rest[row * ((p.width + 7) / 8) + at / 8];
+        #pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = with_rest<T>(v[i], w >> (2 * i) & 3u);
+    }
+}
 
 template <int W> __device__ __forceinline__ float row_total(float v, float* lds, int wave)
 {
@@ -96,6 +137,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
                 #pragma unroll
                 for (int i = 0; i < V; i++) v[j][i] += o[i];
                 if (p.sum) store_row<T>(static_cast<T*>(p.sum) + row * p.width + at, p.width - at, v[j]);
+                store_rest<T>(p, row, at, v[j]);
             }
         }
         float ss = 0.f;
@@ -189,6 +231,7 @@ __global__ __launch_bounds__(256) void rms_norm_wide_kernel(NormArgs p)
             #pragma unroll
             for (int i = 0; i < V; i++) ss = fmaf(v[i], v[i], ss);
             if (res && p.sum) store_row<T>(static_cast<T*>(p.sum) + row * p.width + at, p.width - at, v);
+            if (res) store_rest<T>(p, row, at, v);
         }
         ss = row_total<4>(ss, sums, wave);
         r = 1.f / sqrtf(ss / (float)p.width + p.eps);
@@ -258,7 +301,7 @@ __global__ __launch_bounds__(256) void rms_norm_back_kernel(NormBackArgs p)
         for (int i = 0; i < V; i++) { dw[j][i] = 0.f; w[j][i] = 1.f; }
         if (kAhead && p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w[j]);
     }
-    struct Row { RawRow<T> g[NV], s[NV], d[NV]; float r; };
+    struct Row { RawRow<T> g[NV], s[NV], d[NV]; uint32_t rest[NV]; float r; };
     auto load = [&](Row& x, int64_t row)
     {
         const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
@@ -272,7 +315,14 @@ __global__ __launch_bounds__(256) void rms_norm_back_kernel(NormBackArgs p)
             x.g[j] = load_raw<T>(dy + at, p.width - at);
             x.s[j] = load_raw<T>(s + at, p.width - at);
             if (p.ds) x.d[j] = load_raw<T>(ds + at, p.width - at);
+            x.rest[j] = sizeof(T) == 2 && p.rest && at < p.width ? p.rest[row * ((p.width + 7) / 8) + at / 8] : 0x5555u;     // (0x5555: nothing left)
         }
+    };
+    auto sum_at = [](const Row& x, int j, int i)
+    {
+        const float s = row_load(x.s[j].v[i]);
+        if constexpr (sizeof(T) == 2) return with_rest<T>(s, x.rest[j] >> (2 * i) & 3u);
+        else return s;
     };
     const int64_t step = (int64_t)gridDim.x * (W == 1 ? 4 : 1);
     int turn = 0;
@@ -295,7 +345,7 @@ __global__ __launch_bounds__(256) void rms_norm_back_kernel(NormBackArgs p)
             #pragma unroll
             for (int i = 0; i < V; i++)
             {
-                const float g = row_load(now.g[j].v[i]), s = row_load(now.s[j].v[i]);
+                const float g = row_load(now.g[j].v[i]), s = sum_at(now, j, i);
                 dw[j][i] = fmaf(g, s * r, dw[j][i]);
                 dot = fmaf(g * w[j][i], s, dot);
             }
@@ -310,7 +360,7 @@ __global__ __launch_bounds__(256) void rms_norm_back_kernel(NormBackArgs p)
             #pragma unroll
             for (int i = 0; i < V; i++)
             {
-                v[i] = fmaf(row_load(now.g[j].v[i]) * w[j][i], r, -c * row_load(now.s[j].v[i]));
+                v[i] = fmaf(row_load(now.g[j].v[i]) * w[j][i], r, -c * sum_at(now, j, i));
                 if (p.ds) v[i] += row_load(now.d[j].v[i]);
             }
             store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, p.width - at, v);
@@ -362,6 +412,7 @@ __global__ __launch_bounds__(256) void rms_norm_back_coef_kernel(NormBackArgs p)
         float g[V], sv[V], w[V];
         load_row<T>(dy + at, p.width - at, g);
         load_row<T>(s + at, p.width - at, sv);
+        kept_sum<T>(p, row, at, sv);
         if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w);
         #pragma unroll
         for (int i = 0; i < V; i++) dot = fmaf(p.weight ? g[i] * w[i] : g[i], sv[i], dot);
@@ -386,6 +437,7 @@ __global__ __launch_bounds__(256) void rms_norm_back_wide_kernel(NormBackArgs p)
         float g[V], sv[V], d[V];
         load_row<T>(static_cast<const T*>(p.dy) + row * p.lddy + at, left, g);
         load_row<T>(static_cast<const T*>(p.s) + row * p.lds + at, left, sv);
+        kept_sum<T>(p, row, at, sv);
         if (p.ds) load_row<T>(static_cast<const T*>(p.ds) + row * p.ldds + at, left, d);
         const float r = p.rstd[row], c = p.coef[row];
         #pragma unroll
@@ -459,6 +511,7 @@ template <class T, bool QUANT, bool NORM> void launch_norm(const NormArgs& a, co
         if (a.residual) b.residual = static_cast<const T*>(a.residual) + r * a.ldr;
         b.y = static_cast<char*>(a.y) + r * a.ldy * (QUANT ? 1 : (int64_t)sizeof(T));
         if (a.sum) b.sum = static_cast<T*>(a.sum) + r * a.width;
+        if (a.rest) b.rest = a.rest + r * ((a.width + 7) / 8);
         if (a.rstd) b.rstd = a.rstd + r;
         if (a.scale) b.scale = a.scale + r;
         launch_norm_rows<T, QUANT, NORM>(b, k, s);
@@ -499,16 +552,16 @@ int back_slots(int64_t rows, int64_t width, int dtype)
 
 } // namespace
 
-extern "C" int lvg_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* sum, float* rstd, float* scale,
+extern "C" int lvg_rms_norm(const void* x, const void* residual, const void* weight, void* y, void* sum, void* rest, float* rstd, float* scale,
                             int64_t rows, int64_t width, int64_t x_stride, int64_t residual_stride, float eps, int dtype, int quantize, void* stream)
 {
     LVG_REQUIRE(row_type(dtype), "lvg_rms_norm: float32 / float16 / bfloat16 only (dtype %d)", dtype);
     LVG_REQUIRE(rows_ok(rows, width), "lvg_rms_norm: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
     if (rows == 0) return LVG_OK;
-    LVG_REQUIRE(x && y && (!quantize || scale) && (!sum || residual), "lvg_rms_norm: missing pointer");
+    LVG_REQUIRE(x && y && (!quantize || scale) && (!sum || residual) && (!rest || sum), "lvg_rms_norm: missing pointer");
     LVG_REQUIRE(x_stride >= 0 && residual_stride >= 0, "lvg_rms_norm: negative row stride");
     LVG_REQUIRE(eps >= 0.f, "lvg_rms_norm: eps must not be negative");
-    NormArgs a = {x, residual, weight, y, sum, rstd, scale, rows, width, x_stride, residual_stride, width, eps};
+    NormArgs a = {x, residual, weight, y, sum, dtype == LVG_F32 ? nullptr : static_cast<uint16_t*>(rest), rstd, scale, rows, width, x_stride, residual_stride, width, eps};
     const Plan k = plan(width, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     #define LVG_TYPE(T) { if (quantize) launch_norm<T, true, true>(a, k, s); else launch_norm<T, false, true>(a, k, s); }
@@ -523,7 +576,7 @@ extern "C" int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t r
     LVG_REQUIRE(rows_ok(rows, width), "lvg_quantize_rows: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
     if (rows == 0) return LVG_OK;
     LVG_REQUIRE(x && q && scale && x_stride >= 0, "lvg_quantize_rows: missing pointer or negative row stride");
-    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f};
+    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f};
     const Plan k = plan(width, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) launch_norm<float, true, false>(a, k, s);
@@ -539,7 +592,7 @@ extern "C" int64_t lvg_rms_norm_backward_work(int64_t rows, int64_t width, int w
     return (back_plan(width, dtype).waves ? 0 : (rows + 3) / 4 * 16) + (weight ? (int64_t)back_slots(rows, width, dtype) * width * 4 : 0);
 }
 
-extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s_in, const void* weight, const float* rstd, void* dx, void* dw,
+extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s_in, const void* rest, const void* weight, const float* rstd, void* dx, void* dw,
                                      void* work, int64_t work_size, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
                                      int dtype, void* stream)
 {
@@ -555,7 +608,7 @@ extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const voi
     const int slots = back_slots(rows, width, dtype);
     float* const coef = k.waves ? nullptr : static_cast<float*>(work);
     float* const part = dw ? static_cast<float*>(work) + (k.waves ? 0 : (rows + 3) / 4 * 4) : nullptr;
-    NormBackArgs a = {dy, dsum, s_in, weight, rstd, dx, part, coef, rows, width, dy_stride, dsum_stride, s_stride};
+    NormBackArgs a = {dy, dsum, s_in, dtype == LVG_F32 ? nullptr : static_cast<const uint16_t*>(rest), weight, rstd, dx, part, coef, rows, width, dy_stride, dsum_stride, s_stride};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) launch_back<float>(a, k, slots, s);
     else if (dtype == LVG_F16) launch_back<f16_t>(a, k, slots, s);

@@ -84,9 +84,9 @@ _SIGNATURES = {
     'lvg_linear_act': [_vp] * 9 + [_i64] * 8 + [_i32] * 5 + [_f32] * 3 + [_vp],
     'lvg_linear_backward_work': [_i64] * 3 + [_i32] * 4,
     'lvg_linear_backward': [_vp] * 8 + [_i64] * 7 + [_i32] * 2 + [_f32] * 2 + [_i32, _vp],
-    'lvg_rms_norm': [_vp] * 7 + [_i64] * 4 + [_f32, _i32, _i32, _vp],
+    'lvg_rms_norm': [_vp] * 8 + [_i64] * 4 + [_f32, _i32, _i32, _vp],
     'lvg_rms_norm_backward_work': [_i64] * 2 + [_i32] * 2,
-    'lvg_rms_norm_backward': [_vp] * 8 + [_i64] * 6 + [_i32, _vp],
+    'lvg_rms_norm_backward': [_vp] * 9 + [_i64] * 6 + [_i32, _vp],
     'lvg_quantize_rows': [_vp] * 3 + [_i64] * 3 + [_i32, _vp],
     'lvg_tapconv_epilogue_backward': [_vp] * 10 + [_i64, _i32, _i32, _i32, _i64, _i32, _i32, _f32, _f32, _f32, _vp],
 }

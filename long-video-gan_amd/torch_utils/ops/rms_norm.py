@@ -38,7 +38,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-8, quantize=False, impl='cuda
     elif grad:
         out = _RmsNorm.apply(x, weight, residual, eps)
     else:
-        y, scale, total, _ = _forward(x, weight, residual, eps, quantize, False)
+        y, scale, total, _, _ = _forward(x, weight, residual, eps, quantize, False)
         out = tuple(t for t in (y, scale, total) if t is not None)
     return out[0] if len(out) == 1 else out
 
@@ -81,7 +81,8 @@ def _rms_norm_ref(x, weight, residual, eps, quantize):
 # HIP path.
 
 def _forward(x, weight, residual, eps, quantize, keep):
-    """(y or q, scale or None, s or None, rstd or None) on x's device and the current stream."""
+    """(y or q, scale or None, s or None, rstd or None, rest or None) on x's device and the current stream; keep: for a backward pass, with the
+    reciprocal roots and what the 16-bit sum lost in its rounding."""
     width = x.shape[-1]
     y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if quantize else x.dtype, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quantize else None
@@ -89,28 +90,29 @@ def _forward(x, weight, residual, eps, quantize, keep):
     x2 = _rows.rows_of(x, width)
     rows = x2.shape[0]
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep else None
+    rest = torch.empty((rows, -(-width // 8)), dtype=torch.int16, device=x.device) if keep and total is not None and x.dtype != torch.float32 else None
     if rows:
         r2 = None if residual is None else _rows.rows_of(residual, width)
         if weight is not None:
             weight = weight.contiguous()
         _rows.launch(x.device, 'lvg_rms_norm', x2.data_ptr(), None if r2 is None else r2.data_ptr(), None if weight is None else weight.data_ptr(), y.data_ptr(),
-                     None if total is None else total.data_ptr(), None if rstd is None else rstd.data_ptr(), None if scale is None else scale.data_ptr(),
+                     None if total is None else total.data_ptr(), None if rest is None else rest.data_ptr(), None if rstd is None else rstd.data_ptr(), None if scale is None else scale.data_ptr(),
                      rows, width, _rows.row_stride(x2), 0 if r2 is None else _rows.row_stride(r2), eps, _rows.type_code(x.dtype), int(quantize))
-    return y, scale, total, rstd
+    return y, scale, total, rstd, rest
 
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        y, _, total, rstd = _forward(x, weight, residual, eps, False, True)
+        y, _, total, rstd, rest = _forward(x, weight, residual, eps, False, True)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if total is None else total, weight, rstd)
+        ctx.save_for_backward(x if total is None else total, weight, rstd, rest)
         return (y,) if total is None else (y, total)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, ds=None):
-        s, weight, rstd = ctx.saved_tensors
+        s, weight, rstd, rest = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         dw = None
         if dy is None:
@@ -133,7 +135,7 @@ class _RmsNorm(torch.autograd.Function):
             work = _rows.work_of(size, dev)
             if weight is not None:
                 weight = weight.contiguous()
-            _rows.launch(dev, 'lvg_rms_norm_backward', dy2.data_ptr(), None if ds2 is None else ds2.data_ptr(), s2.data_ptr(), None if weight is None else weight.data_ptr(),
-                         rstd.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(), None if work is None else work.data_ptr(), size, rows, width,
+            _rows.launch(dev, 'lvg_rms_norm_backward', dy2.data_ptr(), None if ds2 is None else ds2.data_ptr(), s2.data_ptr(), None if rest is None else rest.data_ptr(),
+                         None if weight is None else weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(), None if work is None else work.data_ptr(), size, rows, width,
                          _rows.row_stride(dy2), 0 if ds2 is None else _rows.row_stride(ds2), _rows.row_stride(s2), code)
         return dx if need_x else None, dw, dx if need_r else None, None

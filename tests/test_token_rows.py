@@ -121,8 +121,8 @@ def check_norm(x, w, r, eps=1e-6, dy=None, ds=None):
     dot = (g * s).mean(dim=-1, keepdim=True)
     big = (g * s).abs().mean(dim=-1, keepdim=True)
     want = inv * g - s * inv ** 3 * dot + (0 if ds is None or r is None else ds.double())
-    # the kernel reads the sum as it was stored, rounded once
-    su = (tr.u(dt) if r is not None else 0) + tr.F32_ULP
+    # the kernel reads the sum as it was stored, rounded once, with two bits of what the rounding left: within a third of half a step
+    su = (tr.u(dt) / 3 if r is not None and x.is_cuda else tr.u(dt) if r is not None else 0) + 3 * tr.F32_ULP
     off = rel * (inv * g).abs() * 2 + (s * inv ** 3).abs() * big * (2 * su + 4 * rel) + 4 * tr.F32_ULP * want.abs()
     bound = tr.rounded(want, off, dt)
     tr.assert_within(grads[0], want, bound, 'dx')
@@ -247,12 +247,12 @@ def test_refusals_of_the_c_entries_cpu():
                dict(halves=2, kind=0), dict(halves=2, kind=2), dict(kind=5), dict(ldy=-1), dict(ldx=-1), dict(ldw=-1)):
         assert lib.lvg_linear_backward(*{**back, **kw}.values(), None) == -1, kw
     assert lib.lvg_linear_backward(*{**back, 'rows': 0}.values(), None) == 0
-    norm = dict(x=p, r=None, w=None, y=p, s=None, rstd=None, scale=None, rows=4, width=4, ldx=4, ldr=0, eps=0.0, dtype=2, quant=0)
-    for kw in (dict(dtype=3), dict(x=None), dict(y=None), dict(quant=1), dict(s=p), dict(rows=-1), dict(width=0), dict(ldx=-1), dict(eps=-1.0), dict(eps=math.nan)):
+    norm = dict(x=p, r=None, w=None, y=p, s=None, rest=None, rstd=None, scale=None, rows=4, width=4, ldx=4, ldr=0, eps=0.0, dtype=2, quant=0)
+    for kw in (dict(dtype=3), dict(x=None), dict(y=None), dict(quant=1), dict(s=p), dict(rest=p), dict(rows=-1), dict(width=0), dict(ldx=-1), dict(eps=-1.0), dict(eps=math.nan)):
         assert lib.lvg_rms_norm(*{**norm, **kw}.values(), None) == -1, kw
     assert lib.lvg_rms_norm_backward_work(4, 0, 1, 2) == -1 and lib.lvg_rms_norm_backward_work(-1, 4, 1, 2) == -1 and lib.lvg_rms_norm_backward_work(4, 4, 1, 4) == -1
     size = lib.lvg_rms_norm_backward_work(4, 4, 1, 2)
-    back = dict(dy=p, ds=None, s=p, w=None, rstd=p, dx=p, dw=p, work=p, size=size, rows=4, width=4, lddy=4, ldds=0, lds=4, dtype=2)
+    back = dict(dy=p, ds=None, s=p, rest=None, w=None, rstd=p, dx=p, dw=p, work=p, size=size, rows=4, width=4, lddy=4, ldds=0, lds=4, dtype=2)
     for kw in (dict(dtype=4), dict(dy=None), dict(rstd=None), dict(dx=None), dict(s=None), dict(work=None), dict(work=p + 4), dict(size=size - 1), dict(lds=-1), dict(lddy=-1)):
         assert lib.lvg_rms_norm_backward(*{**back, **kw}.values(), None) == -1, kw
     assert lib.lvg_quantize_rows(p, p, None, 4, 4, 4, 2, None) == -1 and lib.lvg_quantize_rows(p, p, p, 4, 0, 4, 2, None) == -1
