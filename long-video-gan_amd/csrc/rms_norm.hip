@@ -289,11 +289,11 @@ __global__ __launch_bounds__(256) void rms_norm_wide_kernel(NormArgs p)
 // rows in registers; the four waves' sums meet in LDS in wave order and go to part[blockIdx.x][width]. The next row's three vectors are asked
 // for before this one's are used (NV <= 4: they fit the registers), so that memory does not wait for the row's reduction.
 template <class T, int W, int NV>
-__global__ __launch_bounds__(256) void rms_norm_back_kernel(NormBackArgs p)
+__global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormBackArgs p)
 {
     constexpr int V = Elem<T>::kVec;
     constexpr bool kAhead = NV <= 4;
-    __shared__ float sums[2][4];
+    __shared__ float sums[2][W == 1 ? 4 : W];
     __shared__ float cols[W == 1 ? 64 * V : 1];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int t = W == 1 ? lane : (int)threadIdx.x;
@@ -529,17 +529,17 @@ Plan back_plan(int64_t width, int dtype)
 {
     const int64_t vecs = lvg_ceil_div(width, 16 / esize(dtype));
     if (vecs <= 64) return {1, 1};
-    for (int nv : {1, 2, 4}) if (vecs <= 256 * nv) return {4, nv};
-    // (eight vectors of 16-bit values would not fit)
-    return dtype == LVG_F32 && vecs <= 2048 ? Plan{4, 8} : Plan{0, 0};
+    if (vecs <= 256) return {4, 1};
+    for (int nv : {1, 2, 4}) if (vecs <= 512 * nv && (nv < 4 || dtype == LVG_F32)) return {8, nv};
+    return {0, 0};
 }
 
 template <class T> void launch_back(const NormBackArgs& a, const Plan& k, int slots, hipStream_t s)
 {
     const dim3 block(256), grid((unsigned)slots);
-    #define LVG_ROW(W, NV) if (k.waves == W && k.vecs == NV) { hipLaunchKernelGGL((rms_norm_back_kernel<T, W, NV>), grid, block, 0, s, a); return; }
-    LVG_ROW(1, 1) LVG_ROW(4, 1) LVG_ROW(4, 2) LVG_ROW(4, 4)
-    if constexpr (sizeof(T) == 4) { LVG_ROW(4, 8) }
+    #define LVG_ROW(W, NV) if (k.waves == W && k.vecs == NV) { hipLaunchKernelGGL((rms_norm_back_kernel<T, W, NV>), grid, dim3(W == 8 ? 512 : 256), 0, s, a); return; }
+    LVG_ROW(1, 1) LVG_ROW(4, 1) LVG_ROW(8, 1) LVG_ROW(8, 2)
+    if constexpr (sizeof(T) == 4) { LVG_ROW(8, 4) }
     #undef LVG_ROW
     hipLaunchKernelGGL(rms_norm_back_coef_kernel<T>, dim3((unsigned)a.rows), block, 0, s, a);
     hipLaunchKernelGGL(rms_norm_back_wide_kernel<T>, dim3((unsigned)lvg_ceil_div(a.width, 256 * Elem<T>::kVec), (unsigned)slots), block, 0, s, a);
@@ -552,7 +552,7 @@ int back_slots(int64_t rows, int64_t width, int dtype)
     const Plan k = back_plan(width, dtype);
     // two or four workgroups for each of the 256 compute units: what they write of the weight's gradient is read again
     if (k.waves == 1) return (int)std::min<int64_t>(1024, lvg_ceil_div(rows, 4));
-    if (k.waves == 4) return (int)std::min<int64_t>(k.vecs == 1 ? 1024 : 768, rows);
+    if (k.waves) return (int)std::min<int64_t>(k.waves == 4 ? 1024 : 512, rows);
     return (int)std::min<int64_t>(64, rows);
 }
 
