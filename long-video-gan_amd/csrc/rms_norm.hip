@@ -604,7 +604,11 @@ extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const voi
 {
     LVG_REQUIRE(row_type(dtype), "lvg_rms_norm_backward: float32 / float16 / bfloat16 only (dtype %d)", dtype);
     LVG_REQUIRE(rows_ok(rows, width), "lvg_rms_norm_backward: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
-    if (rows == 0) return LVG_OK;
+    if (rows == 0)
+    {
+        if (dw) row_column_sum(nullptr, dw, 0, width, 0.f, dtype, static_cast<hipStream_t>(stream));
+        return lvg_check_launch("lvg_rms_norm_backward");
+    }
     const Plan k = back_plan(width, dtype);
     const int64_t need = lvg_rms_norm_backward_work(rows, width, dw != nullptr, dtype);
     LVG_REQUIRE(dy && s_in && rstd && dx, "lvg_rms_norm_backward: missing pointer");

@@ -457,6 +457,7 @@ BackWork back_work(int64_t rows, int64_t outer, int64_t inner, int halves, int k
 {
     const int es = esize_of(dtype);
     BackWork w = {0, pad16(outer * halves * es) / es, 0, 0, 0, 0};
+    if (rows == 0 || outer == 0) return w;
     w.slots = slope_slots(rows, outer, es);
     if (kind != LVG_SLOPE_NONE) w.dz = rows * w.dzStride * es;
     if (db) w.part = pad16((int64_t)w.slots * halves * outer * 4);
@@ -477,7 +478,7 @@ bool back_sizes(int64_t rows, int64_t outer, int64_t inner, int halves, int kind
 extern "C" int64_t lvg_linear_backward_work(int64_t rows, int64_t outer, int64_t inner, int halves, int slope_kind, int grads, int dtype)
 {
     if (!back_sizes(rows, outer, inner, halves, slope_kind, dtype)) return LVG_ERR_INVALID;
-    return rows && outer ? back_work(rows, outer, inner, halves, slope_kind, grads & 1, grads & 2, grads & 4, dtype).all : 0;
+    return back_work(rows, outer, inner, halves, slope_kind, grads & 1, grads & 2, grads & 4, dtype).all;
 }
 
 extern "C" int lvg_linear_backward(const void* dy, const void* slopes, const void* x, const void* w, void* dx, void* dw, void* db, void* work, int64_t work_size,
@@ -485,8 +486,9 @@ extern "C" int lvg_linear_backward(const void* dy, const void* slopes, const voi
                                    int halves, int slope_kind, float alpha, float gain, int dtype, void* stream)
 {
     LVG_REQUIRE(back_sizes(rows, outer, inner, halves, slope_kind, dtype), "lvg_linear_backward: bad size, type or slopes");
-    if (rows == 0 || outer == 0) return LVG_OK;
-    LVG_REQUIRE(dy && (slope_kind == LVG_SLOPE_NONE || slopes) && (!dx || inner == 0 || w) && (!dw || inner == 0 || x), "lvg_linear_backward: missing pointer");
+    // (nothing to sum over: the gradients that have values are zeros)
+    const bool none = rows == 0 || outer == 0;
+    LVG_REQUIRE((none || (dy && (slope_kind == LVG_SLOPE_NONE || slopes))) && (!dx || inner == 0 || none || w) && (!dw || inner == 0 || none || x), "lvg_linear_backward: missing pointer");
     LVG_REQUIRE(dy_stride >= 0 && x_stride >= 0 && w_stride >= 0, "lvg_linear_backward: negative row stride");
     const BackWork k = back_work(rows, outer, inner, halves, slope_kind, dx != nullptr, dw != nullptr, db != nullptr, dtype);
     LVG_REQUIRE(k.all == 0 || (work && lvg_aligned16(work) && work_size >= k.all), "lvg_linear_backward: the workspace must be 16-byte aligned and hold %lld bytes", (long long)k.all);
@@ -495,7 +497,8 @@ extern "C" int lvg_linear_backward(const void* dy, const void* slopes, const voi
     char* const mem = static_cast<char*>(work);
     const void* dz = plain ? dy : mem;
     const int64_t dzStride = plain ? dy_stride : k.dzStride, total = outer * halves;
-    if (!plain || db)
+    if (none && db && outer) row_column_sum(nullptr, db, 0, total, 0.f, dtype, s);
+    if (!none && (!plain || db))
     {
         float* part = db ? reinterpret_cast<float*>(mem + k.dz) : nullptr;
         SlopeArgs a = {dy, slopes, plain ? nullptr : mem, part, rows, outer, dy_stride, k.dzStride, slope_kind, slope_lanes(outer, esize_of(dtype)), alpha, plain ? 1.f : gain};
@@ -510,11 +513,11 @@ extern "C" int lvg_linear_backward(const void* dy, const void* slopes, const voi
         if (rc != LVG_OK) return rc;
     }
     void* const pw = mem + k.dz + k.part;
-    if (dx)
+    if (dx && rows)
     {
         const int rc = grad_product(dz, dzStride, !plain, w, w_stride, dx, pw, k.product, rows, total, inner, false, plain ? gain : 1.f, dtype, s);
         if (rc != LVG_OK) return rc;
     }
-    if (dw) return grad_product(dz, dzStride, !plain, x, x_stride, dw, pw, k.product, rows, total, inner, true, plain ? gain : 1.f, dtype, s);
+    if (dw && outer) return grad_product(dz, dzStride, !plain, x, x_stride, dw, pw, k.product, rows, total, inner, true, plain ? gain : 1.f, dtype, s);
     return LVG_OK;
 }

@@ -63,7 +63,7 @@ def _check(x, weight, b, x_scale, weight_scale, out_dtype, halves):
         assert x_scale is not None and weight_scale is not None, '8-bit operands come with their scales'
         assert x_scale.dtype == weight_scale.dtype == torch.float32 and x_scale.device == weight_scale.device == device
         assert x_scale.shape == x.shape[:-1] and weight_scale.shape == (total,)
-        _no_grad_with_8bit(x, b, x_scale, weight_scale)
+        _no_grad_with_8bit(x, x, weight, b, x_scale, weight_scale)
     else:
         assert dtype in _rows.ROW_DTYPES, f'dtype {dtype} is not supported'
         assert out_dtype is None or out_dtype == dtype, 'the result has the operands\' dtype'
@@ -107,10 +107,10 @@ def _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_sc
     device = x.device
     x2, w2 = _rows.rows_of(x, inner), _rows.rows_of(weight, inner)
     rows = x2.shape[0]
-    y = torch.empty((rows, outer) if x.ndim == 2 else (*x.shape[:-1], outer), dtype=out_dtype, device=device)
+    y = x.new_empty((rows, outer) if x.ndim == 2 else (*x.shape[:-1], outer), dtype=out_dtype)
     slopes = None
     if kind != SLOPE_NONE:
-        slopes = torch.empty((rows, total), dtype=torch.float32 if kind == SLOPE_F32 else torch.uint8, device=device)
+        slopes = x.new_empty((rows, total), dtype=torch.float32 if kind == SLOPE_F32 else torch.uint8)
     if rows == 0 or outer == 0:
         return y, slopes
     r2 = None if residual is None else _rows.rows_of(residual, outer)
@@ -135,14 +135,11 @@ def _backward(dy, x, weight, slopes, kind, halves, alpha, gain, need_x, need_w, 
     total, inner = weight.shape
     outer = total // halves
     x2, w2, dy2 = _rows.rows_of(x, inner), _rows.rows_of(weight, inner), _rows.rows_of(dy, outer)
-    rows, dtype, device = x2.shape[0], x.dtype, x.device
-    if rows == 0 or outer == 0:
-        # nothing to sum over
-        return (x2.new_zeros(x.shape) if need_x else None, w2.new_zeros(weight.shape) if need_w else None, w2.new_zeros(total) if need_b else None)
-    dx = torch.empty(x.shape, dtype=dtype, device=device) if need_x else None
-    dw = torch.empty((total, inner), dtype=dtype, device=device) if need_w else None
-    db = torch.empty(total, dtype=dtype, device=device) if need_b else None
-    code = _rows.type_code(dtype)
+    rows, device = x2.shape[0], x.device
+    dx = x2.new_empty(x.shape) if need_x else None
+    dw = x2.new_empty((total, inner)) if need_w else None
+    db = x2.new_empty(total) if need_b else None
+    code = _rows.type_code(x.dtype)
     size = _rows.query('lvg_linear_backward_work', rows, outer, inner, halves, kind, need_x + 2 * need_w + 4 * need_b, code)
     work = _rows.work_of(size, device)
     _rows.launch(device, 'lvg_linear_backward', dy2.data_ptr(), None if slopes is None else slopes.data_ptr(), x2.data_ptr(), w2.data_ptr(),

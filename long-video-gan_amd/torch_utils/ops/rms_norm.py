@@ -52,8 +52,8 @@ def quantize_rows(x, impl='cuda'):
     if impl == 'ref' or not x.is_cuda:
         return _quantize_ref(x.float())
     width = x.shape[-1]
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
     x2 = _rows.rows_of(x, width)
     if x2.shape[0]:
         _rows.launch(x.device, 'lvg_quantize_rows', x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], width, _rows.row_stride(x2), _rows.type_code(x.dtype))
@@ -84,9 +84,9 @@ def _forward(x, weight, residual, eps, quantize, keep):
     """(y or q, scale or None, s or None, rstd or None, rest or None) on x's device and the current stream; keep: for a backward pass, with the
     reciprocal roots and what the 16-bit sum lost in its rounding."""
     width = x.shape[-1]
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if quantize else x.dtype, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quantize else None
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual is not None else None
+    y = torch.empty_like(x, dtype=torch.float8_e4m3fn if quantize else x.dtype, memory_format=torch.contiguous_format)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32) if quantize else None
+    total = torch.empty_like(x, memory_format=torch.contiguous_format) if residual is not None else None
     x2 = _rows.rows_of(x, width)
     rows = x2.shape[0]
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep else None
@@ -126,8 +126,6 @@ class _RmsNorm(torch.autograd.Function):
             ds2 = None if ds is None else _rows.rows_of(ds, width)
             rows, dev = s2.shape[0], s.device
             dx = torch.empty(s.shape, dtype=s.dtype, device=dev)
-            if rows == 0:
-                return dx, torch.zeros_like(weight) if need_w else None, dx if need_r else None, None
             code = _rows.type_code(s.dtype)
             if need_w:
                 dw = torch.empty(width, dtype=s.dtype, device=dev)

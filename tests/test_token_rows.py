@@ -211,6 +211,7 @@ def test_refusals_python_cpu():
                  lambda: la.linear_act(q, qw, x_scale=s.half(), weight_scale=sw.half()), lambda: la.linear_act(q, qw, x_scale=s, weight_scale=sw, out_dtype=F32),
                  lambda: la.linear_act(q, qw, torch.randn(6, dtype=BF16, requires_grad=True), x_scale=s, weight_scale=sw),
                  lambda: la.linear_act(q, qw, residual=torch.randn(4, 6, dtype=BF16, requires_grad=True), x_scale=s, weight_scale=sw),
+                 lambda: la.linear_act(q.clone().requires_grad_(True), qw, x_scale=s, weight_scale=sw), lambda: gf.gated_ff(q, qw.clone().requires_grad_(True), x_scale=s, weight_scale=sw),
                  lambda: la.linear_act(x, w.unsqueeze(0)), lambda: la.linear_act(x, w, impl='fast'),
                  lambda: gf.gated_ff(x, torch.randn(5, 8)), lambda: gf.gated_ff(x, w, torch.randn(3)), lambda: gf.gated_ff(x, w, act='silu'),
                  lambda: rn.rms_norm(x, torch.randn(7)), lambda: rn.rms_norm(x, torch.randn(8).half()), lambda: rn.rms_norm(x, residual=torch.randn(8)),
@@ -246,7 +247,7 @@ def test_refusals_of_the_c_entries_cpu():
     for kw in (dict(dtype=4), dict(dy=None), dict(s=None), dict(x=None), dict(w=None), dict(work=None), dict(work=p + 8), dict(size=size - 1), dict(rows=-1), dict(halves=3),
                dict(halves=2, kind=0), dict(halves=2, kind=2), dict(kind=5), dict(ldy=-1), dict(ldx=-1), dict(ldw=-1)):
         assert lib.lvg_linear_backward(*{**back, **kw}.values(), None) == -1, kw
-    assert lib.lvg_linear_backward(*{**back, 'rows': 0}.values(), None) == 0
+    assert lib.lvg_linear_backward(*{**back, 'rows': 0, 'outer': 0}.values(), None) == 0
     norm = dict(x=p, r=None, w=None, y=p, s=None, rest=None, rstd=None, scale=None, rows=4, width=4, ldx=4, ldr=0, eps=0.0, dtype=2, quant=0)
     for kw in (dict(dtype=3), dict(x=None), dict(y=None), dict(quant=1), dict(s=p), dict(rest=p), dict(rows=-1), dict(width=0), dict(ldx=-1), dict(eps=-1.0), dict(eps=math.nan)):
         assert lib.lvg_rms_norm(*{**norm, **kw}.values(), None) == -1, kw
@@ -324,6 +325,22 @@ def test_layouts_gpu(view, dtype):
     check_linear(x, w, None, r, act='tanh', dy=wide[..., 7:47])
     check_gated(x.detach(), w.detach(), rand(80, seed=3, dtype=dtype)[::2], dy=wide[..., 1:41:2])
     check_norm(x.detach(), rand(96, seed=3, dtype=dtype)[::2], x.detach(), dy=wide[..., 3:51], ds=wide[..., :1].expand(*shape, 48))
+
+
+@pytest.mark.gpu
+def test_single_rows_and_8bit_layouts_gpu():
+    """A vector is one row; 8-bit operands take any strides."""
+    x, w, b = rand(70, seed=1, dtype=BF16), rand(40, 70, seed=2, dtype=BF16), rand(40, seed=3, dtype=BF16)
+    check_linear(x, w, b, rand(40, seed=4, dtype=BF16), act='swish', dy=rand(40, seed=5, dtype=BF16))
+    check_norm(x.detach(), rand(70, seed=6, dtype=BF16), rand(70, seed=7, dtype=BF16), dy=rand(70, seed=8, dtype=BF16), ds=rand(70, seed=9, dtype=BF16))
+    q, s = rn.quantize_rows(x.detach())
+    assert q.shape == (70,) and s.shape == ()
+    (q, s), (qw, sw) = rn.quantize_rows(rand(70, 111, seed=1)), rn.quantize_rows(rand(90, 111, seed=2))
+    s2, sw2 = torch.stack([s, s], dim=1)[:, 0], torch.stack([sw, sw], dim=1)[:, 1]
+    for rows in (5, 20, 70):
+        for qx, qv in ((q[:rows, 3:83], qw[:, 7:87]), (q[:rows, :80].t().contiguous().t(), qw[:, :80].t().contiguous().t())):
+            v, off = tr.sums64(qx.float(), qv.float(), None, s[:rows], sw)
+            tr.assert_within(la.linear_act(qx, qv, x_scale=s2[:rows], weight_scale=sw2), v, tr.rounded(v, off, BF16), 'y')
 
 
 @pytest.mark.gpu
