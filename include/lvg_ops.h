@@ -535,11 +535,13 @@ int lvg_split32_stack(const float* x, void* out, int64_t pixels, int channels, i
  * act / alpha / gain / clamp as in lvg_bias_act (clamp < 0: none; a NaN stays a NaN). b, residual and y have type out_dtype, which is dtype,
  * or float16 / bfloat16 for LVG_E4M3 operands; those come with x_scale [rows] and w_scale [outer] (gated: [2 outer]) float32: the value of an
  * element is itself times its row's scale. b, residual, slopes may be NULL.
- * slopes receives what lvg_linear_backward multiplies gradients with: slope_kind 1: float32 [rows, outer] (gated [rows, 2 outer]: the derivatives
- * with respect to the gate's and the up half's sums), 2: one byte an element (0: clamped, 1: alpha, 2: one; linear, relu and lrelu only), 0: none.
+ * slopes (16-byte aligned, lvg_linear_slope_bytes(...) bytes) receives what lvg_linear_backward multiplies gradients with: slope_kind 1: the derivatives
+ * with respect to the sums, [rows, outer] (gated [rows, 2 outer]: the gate's and the up half's) in float32, or in bfloat16 with two more bits a
+ * value behind them; 2: one byte an element (0: clamped, 1: alpha, 2: one; linear, relu and lrelu only); 0: none.
  * work: lvg_linear_act_work(...) bytes, 16-byte aligned (0 bytes: NULL will do); nothing in it outlives the call.
  */
 int64_t lvg_linear_act_work(int64_t rows, int64_t outer, int64_t inner, int dtype, int gated);
+int64_t lvg_linear_slope_bytes(int64_t rows, int64_t outer, int halves, int slope_kind, int dtype);
 int lvg_linear_act(const void* x, const void* w, const void* b, const void* residual, const float* x_scale, const float* w_scale,
                    void* y, void* slopes, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
                    int64_t x_stride, int64_t w_stride, int64_t residual_stride, int64_t y_stride,

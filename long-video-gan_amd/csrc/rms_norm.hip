@@ -42,20 +42,6 @@ struct NormBackArgs
     int64_t      rows, width, lddy, ldds, lds;
 };
 
-// What rounding v to T left, in units of two thirds of half a step: -1, 0 or 1 (+ 1). A half step is 2^(exponent - 8) (bfloat16) or - 11 (float16).
-template <class T> __device__ __forceinline__ float half_step(float rounded)
-{
-    return __uint_as_float(__float_as_uint(rounded) & 0x7f800000u) * (sizeof(T) == 4 ? 0.f : __is_same(T, bf16_t) ? 0.00390625f : 0.00048828125f);
-}
-template <class T> __device__ __forceinline__ uint32_t rest_code(float v)
-{
-    const float r = to_acc(from_acc<T>(v)), left = v - r, third = half_step<T>(r) * (1.f / 3.f);
-    return left > third ? 2u : left < -third ? 0u : 1u;
-}
-template <class T> __device__ __forceinline__ float with_rest(float rounded, uint32_t code)
-{
-    return code == 1u ? rounded : fmaf((float)(int)(code - 1u), half_step<T>(rounded) * (2.f / 3.f), rounded);
-}
 template <class T> __device__ __forceinline__ void store_rest(const NormArgs& p, int64_t row, int64_t at, const float* v)
 {
     if constexpr (sizeof(T) == 2)

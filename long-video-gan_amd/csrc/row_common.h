@@ -72,6 +72,26 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
     return (uint32_t)w;
 }
 
+// Two bits beside a rounded value: what rounding v to T left, in units of two thirds of half a step: -1, 0 or 1 (+ 1), a third of it at most is lost. A half step is 2^(exponent - 8) (bfloat16) or - 11 (float16).
+// A half step is 2^(exponent - 11) of float16; bfloat16 is the upper half of a float32, a half step 0x8000 of its lower half (zeros, infinities and
+// NaNs stay what they are: nothing is left of them, or it stays within their patterns).
+__device__ __forceinline__ float half_step(float rounded) { return __uint_as_float(__float_as_uint(rounded) & 0x7f800000u) * 0.00048828125f; }
+template <class T> __device__ __forceinline__ uint32_t rest_code(float v)
+{
+    if constexpr (__is_same(T, bf16_t))
+    {
+        const int left = (int)(__float_as_uint(v) - ((uint32_t)from_acc<bf16_t>(v).bits << 16));
+        return left > 0x2aaa ? 2u : left < -0x2aaa ? 0u : 1u;
+    }
+    const float r = to_acc(from_acc<f16_t>(v)), left = v - r, third = half_step(r) * (1.f / 3.f);
+    return left > third ? 2u : left < -third ? 0u : 1u;
+}
+template <class T> __device__ __forceinline__ float with_rest(float rounded, uint32_t code)
+{
+    if constexpr (__is_same(T, bf16_t)) return __uint_as_float(__float_as_uint(rounded) + code * 0x5555u - 0x5555u);
+    return code == 1u ? rounded : fmaf((float)(int)(code - 1u), half_step(rounded) * (2.f / 3.f), rounded);
+}
+
 __device__ __forceinline__ float wave_total(float v)
 {
     #pragma unroll

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(256) void token_finish_kernel(const float* part, in
     prepare4<O, GATED>(f, m, n, v, u);
     float r[4];
     residual4<O>(f, m, n, r);
-    finish4<O, GATED>(f, Place<O>(f, m, n, GATED), v, u, r);
+    finish4<O, GATED>(f, Place<O, GATED ? 2 : 1>(f, m, n), v, u, r);
 }
 
 int launch_finish(const float* part, int splits, int64_t ldpart, const Finish& f, int out_dtype, bool gated, hipStream_t s)
@@ -56,7 +56,7 @@ int launch_finish(const float* part, int splits, int64_t ldpart, const Finish& f
 struct SlopeArgs
 {
     const void* dy;
-    const void* slopes;        // [rows][halves * cols], or NULL
+    const void* slopes;        // [rows][halves * cols] (and their bits), or NULL
     void*       dz;            // or NULL: column sums alone
     float*      part;          // [gridDim.y][halves * cols], or NULL
     int64_t     rows, cols, lddy, lddz;
@@ -69,7 +69,9 @@ struct SlopeArgs
 template <class T, int H>
 __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
 {
-    constexpr int V = Elem<T>::kVec, R = 4;
+    typedef typename Kept<T>::S S;
+    constexpr int V = Elem<T>::kVec, R = 2, kE = Elem<S>::kVec;        // kE: derivatives of a 16-byte vector
+    const int64_t quads = (p.cols + 3) / 4;
     __shared__ float sums[256][V + 1];
     const int tid = threadIdx.x, cl = tid & (p.lanes - 1), rl = tid / p.lanes, rstep = 256 / p.lanes;
     const int64_t n = ((int64_t)blockIdx.x * p.lanes + cl) * V, left = p.cols - n;
@@ -80,40 +82,52 @@ __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
     for (int h = 0; h < H; h++)
         #pragma unroll
         for (int i = 0; i < V; i++) db[h][i] = 0.f;
-    for (int64_t m0 = r0 + rl; left > 0 && m0 < r1; m0 += R * rstep)
+    // N rows from m0 on; WHOLE: the thread's vector is not cut by the last column. No branch lies between the loads.
+    auto take = [&](int64_t m0, auto count, auto isWhole)
     {
-        RawRow<T> g[R];
-        RawRow<float> d[R][H][V / 4];
-        uint8_t c[R][V];
+        constexpr int N = decltype(count)::value;
+        constexpr bool WHOLE = decltype(isWhole)::value != 0;
+        const int64_t have = WHOLE ? V : left;
+        RawRow<T> g[N];
+        RawRow<S> d[N][H][V / kE];
+        uint32_t bits[N][H];
+        uint8_t c[N][V];
         #pragma unroll
-        for (int r = 0; r < R; r++)
+        for (int r = 0; r < N; r++) g[r] = load_raw<T>(static_cast<const T*>(p.dy) + (m0 + r * rstep) * p.lddy + n, have);
+        if (p.kind == LVG_SLOPE_SMOOTH)
         {
-            const int64_t m = m0 + r * rstep;
-            if (m >= r1) continue;
-            g[r] = load_raw<T>(static_cast<const T*>(p.dy) + m * p.lddy + n, left);
-            if (p.kind == LVG_SLOPE_F32)
-            {
+            #pragma unroll
+            for (int r = 0; r < N; r++)
                 #pragma unroll
                 for (int h = 0; h < H; h++)
+                {
+                    const int64_t row = (m0 + r * rstep) * H + h;
                     #pragma unroll
-                    for (int k = 0; k < V / 4; k++) d[r][h][k] = load_raw<float>(static_cast<const float*>(p.slopes) + (m * H + h) * p.cols + n + 4 * k, left - 4 * k);
-            }
-            else if (p.kind == LVG_SLOPE_CODE)
+                    for (int k = 0; k < V / kE; k++) d[r][h][k] = load_raw<S>(static_cast<const S*>(p.slopes) + row * p.cols + n + kE * k, have - kE * k);
+                    if constexpr (Kept<T>::kBits)
+                    {
+                        const uint8_t* at = reinterpret_cast<const uint8_t*>(static_cast<const S*>(p.slopes) + p.rows * H * p.cols) + row * quads + n / 4;
+                        bits[r][h] = at[0];
+                        if (WHOLE || have > 4) bits[r][h] |= (uint32_t)at[1] << 8;
+                    }
+                }
+        }
+        else if (p.kind == LVG_SLOPE_CODE)
+        {
+            #pragma unroll
+            for (int r = 0; r < N; r++)
             {
-                const uint8_t* s = static_cast<const uint8_t*>(p.slopes) + m * p.cols + n;
-                if (left >= V) __builtin_memcpy(c[r], s, V);
+                const uint8_t* s = static_cast<const uint8_t*>(p.slopes) + (m0 + r * rstep) * p.cols + n;
+                if (WHOLE) __builtin_memcpy(c[r], s, V);
                 else
                 {
                     #pragma unroll
-                    for (int i = 0; i < V; i++) c[r][i] = i < left ? s[i] : (uint8_t)0;
+                    for (int i = 0; i < V; i++) c[r][i] = i < have ? s[i] : (uint8_t)0;
                 }
             }
         }
         #pragma unroll
-        for (int r = 0; r < R; r++)
-        {
-            const int64_t m = m0 + r * rstep;
-            if (m >= r1) continue;
+        for (int r = 0; r < N; r++)
             #pragma unroll
             for (int h = 0; h < H; h++)
             {
@@ -122,15 +136,27 @@ __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
                 for (int i = 0; i < V; i++)
                 {
                     v[i] = row_load(g[r].v[i]);
-                    if (p.kind == LVG_SLOPE_F32) v[i] *= d[r][h][i / 4].v[i % 4];
+                    if (p.kind == LVG_SLOPE_SMOOTH)
+                    {
+                        const float s = row_load(d[r][h][i / kE].v[i % kE]);
+                        if constexpr (Kept<T>::kBits) v[i] *= __uint_as_float(__float_as_uint(s) | (bits[r][h] >> (2 * i) & 3u) << 14);
+                        else v[i] *= s;
+                    }
                     else if (p.kind == LVG_SLOPE_CODE) v[i] = c[r][i] == 2 ? v[i] : c[r][i] == 1 ? v[i] * p.alpha : 0.f;
                     v[i] *= p.gain;
                     db[h][i] += v[i];
                 }
-                if (p.dz) store_row<T>(static_cast<T*>(p.dz) + m * p.lddz + h * p.cols + n, left, v);
+                if (p.dz) store_row<T>(static_cast<T*>(p.dz) + (m0 + r * rstep) * p.lddz + h * p.cols + n, have, v);
             }
-        }
-    }
+    };
+    auto run = [&](auto isWhole)
+    {
+        int64_t m0 = r0 + rl;
+        for (; m0 + (R - 1) * rstep < r1; m0 += R * rstep) take(m0, Const<R>(), isWhole);
+        for (; m0 < r1; m0 += rstep) take(m0, Const<1>(), isWhole);
+    };
+    if (left >= V) run(Const<1>());
+    else if (left > 0) run(Const<0>());
     if (!p.part) return;
     #pragma unroll
     for (int h = 0; h < H; h++)
@@ -397,6 +423,12 @@ extern "C" int64_t lvg_linear_act_work(int64_t rows, int64_t outer, int64_t inne
     return rows && outer ? work_bytes(rows, outer, inner, dtype, gated ? LVG_TOKEN_GATED : LVG_TOKEN_FORWARD) : 0;
 }
 
+extern "C" int64_t lvg_linear_slope_bytes(int64_t rows, int64_t outer, int halves, int slope_kind, int dtype)
+{
+    if (!float_type(dtype) || !size_ok(rows) || !size_ok(outer) || (halves != 1 && halves != 2) || slope_kind < LVG_SLOPE_NONE || slope_kind > LVG_SLOPE_CODE) return LVG_ERR_INVALID;
+    return slope_bytes(rows, outer, halves, slope_kind, dtype);
+}
+
 extern "C" int lvg_linear_act(const void* x, const void* w, const void* b, const void* residual, const float* x_scale, const float* w_scale,
                               void* y, void* slopes, void* work, int64_t work_size, int64_t rows, int64_t outer, int64_t inner,
                               int64_t x_stride, int64_t w_stride, int64_t residual_stride, int64_t y_stride,
@@ -413,7 +445,7 @@ extern "C" int lvg_linear_act(const void* x, const void* w, const void* b, const
     LVG_REQUIRE(y && (inner == 0 || (x && w)), "lvg_linear_act: missing pointer");
     LVG_REQUIRE(x_stride >= 0 && w_stride >= 0 && residual_stride >= 0 && y_stride >= outer, "lvg_linear_act: bad row stride");
     LVG_REQUIRE(!gated || (!residual && clamp < 0.f), "lvg_linear_act: a gated unit has neither residual nor clamp");
-    LVG_REQUIRE(slope_kind == LVG_SLOPE_NONE || (slopes && (slope_kind == LVG_SLOPE_F32 || (slope_kind == LVG_SLOPE_CODE && !gated &&
+    LVG_REQUIRE(slope_kind == LVG_SLOPE_NONE || (slopes && (slope_kind == LVG_SLOPE_SMOOTH || (slope_kind == LVG_SLOPE_CODE && !gated &&
                 (act == LVG_ACT_LINEAR || act == LVG_ACT_RELU || act == LVG_ACT_LRELU)))), "lvg_linear_act: bad slopes");
     TokenArgs a;
     memset(&a, 0, sizeof(a));
@@ -470,7 +502,7 @@ BackWork back_work(int64_t rows, int64_t outer, int64_t inner, int halves, int k
 bool back_sizes(int64_t rows, int64_t outer, int64_t inner, int halves, int kind, int dtype)
 {
     return float_type(dtype) && size_ok(rows) && size_ok(outer) && size_ok(inner) && (halves == 1 || halves == 2) && size_ok(outer * halves) &&
-           (kind == LVG_SLOPE_NONE || kind == LVG_SLOPE_F32 || kind == LVG_SLOPE_CODE) && (halves == 1 || kind == LVG_SLOPE_F32);
+           (kind == LVG_SLOPE_NONE || kind == LVG_SLOPE_SMOOTH || kind == LVG_SLOPE_CODE) && (halves == 1 || kind == LVG_SLOPE_SMOOTH);
 }
 
 } // namespace

@@ -658,8 +658,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                     #pragma unroll
                     for (int t = 0; t < kTurns; t++) scale[t] = !kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f;
                 }
-                O* to = static_cast<O*>(f.out) + m * f.ldo + n;
-                float* slopes = kSlopes ? static_cast<float*>(f.slopes) + m * 2 * f.cols + n : nullptr;
+                const Place<O, 2> at(f, m, n);
                 float v[kTurns][4], u[kTurns][4];
                 #pragma unroll
                 for (int t = 0; t < kTurns; t++) sumsOf(pass, t, v[t], u[t]);
@@ -683,12 +682,13 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                         v[t][k] = act[k] * u[t][k];
                     }
                     if (kEdge && (m + t * kRows >= f.rows || left <= 0)) continue;
+                    const Place<O, 2> here = at.down(f, t * kRows);
                     if (kSlopes)
                     {
-                        quad_store(slopes + t * kRows * 2 * f.cols, kEdge ? left : 4, kEdge ? f.vec : true, d);
-                        quad_store(slopes + t * kRows * 2 * f.cols + f.cols, kEdge ? left : 4, kEdge ? f.vec : true, act);
+                        here.keep(f, 0, kEdge ? f.vec : true, d);
+                        here.keep(f, 1, kEdge ? f.vec : true, act);
                     }
-                    quad_store(to + t * kRows * f.ldo, kEdge ? left : 4, kEdge ? f.vec : true, v[t]);
+                    quad_store(here.out, kEdge ? left : 4, kEdge ? f.vec : true, v[t]);
                 }
             }
         });
@@ -697,7 +697,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
     {
         if (f.act == LVG_ACT_SWISH)
         {
-            if (f.slopeKind == LVG_SLOPE_F32) { if (inside) gate(Const<1>(), Const<0>()); else gate(Const<1>(), Const<1>()); }
+            if (f.slopeKind == LVG_SLOPE_SMOOTH) { if (inside) gate(Const<1>(), Const<0>()); else gate(Const<1>(), Const<1>()); }
             else                              { if (inside) gate(Const<0>(), Const<0>()); else gate(Const<0>(), Const<1>()); }
             return;
         }
@@ -719,7 +719,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
         for (int pass = 0; pass < MT; pass++)
         {
             const int64_t m = rowOf(pass);
-            const Place<O> at(f, m, n, GATED);
+            const Place<O, GATED ? 2 : 1> at(f, m, n);
             float next[4] = {0.f, 0.f, 0.f, 0.f};
             auto ask = [&](int t)
             {
@@ -737,7 +737,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                 if (t + 1 < kTurns) ask(t + 1);
                 if (m + t * kRows >= f.rows || left <= 0) continue;
                 cols.apply(f, m + t * kRows, v, u);
-                finish4<O, GATED>(f, at.down(f, t * kRows, GATED), v, u, res);
+                finish4<O, GATED>(f, at.down(f, t * kRows), v, u, res);
             }
         }
     });

@@ -214,7 +214,7 @@ __global__ __launch_bounds__(kWaves * 64) void token_stream_kernel(StreamArgs a)
     prepare4<O, GATED>(a.fin, m, n, v, u);
     float r[4];
     residual4<O>(a.fin, m, n, r);
-    finish4<O, GATED>(a.fin, Place<O>(a.fin, m, n, GATED), v, u, r);
+    finish4<O, GATED>(a.fin, Place<O, GATED ? 2 : 1>(a.fin, m, n), v, u, r);
 }
 
 template <class T, class O> int launch(const StreamArgs& a, bool gated, int splits, hipStream_t s)

@@ -82,6 +82,7 @@ _SIGNATURES = {
     'lvg_noise_filter_bank': [_vp] * 5 + [_i32] * 7 + [_vp],
     'lvg_linear_act_work': [_i64] * 3 + [_i32] * 2,
     'lvg_linear_act': [_vp] * 9 + [_i64] * 8 + [_i32] * 5 + [_f32] * 3 + [_vp],
+    'lvg_linear_slope_bytes': [_i64] * 2 + [_i32] * 3,
     'lvg_linear_backward_work': [_i64] * 3 + [_i32] * 4,
     'lvg_linear_backward': [_vp] * 8 + [_i64] * 7 + [_i32] * 2 + [_f32] * 2 + [_i32, _vp],
     'lvg_rms_norm': [_vp] * 8 + [_i64] * 4 + [_f32, _i32, _i32, _vp],
@@ -103,7 +104,7 @@ def lib():
         for name, argtypes in _SIGNATURES.items():
             fn = getattr(handle, name)
             fn.argtypes = argtypes
-            fn.restype = ctypes.c_int64 if name in ('lvg_conv3d_frames_workgroups', 'lvg_conv3d_frames_workgroups_f32out', 'lvg_bias_act_grad_bias_slots', 'lvg_conv2d_frames_workgroups', 'lvg_conv2d_frames_planes_dot_rows', 'lvg_linear_act_work', 'lvg_linear_backward_work', 'lvg_rms_norm_backward_work') else ctypes.c_int
+            fn.restype = ctypes.c_int64 if name in ('lvg_conv3d_frames_workgroups', 'lvg_conv3d_frames_workgroups_f32out', 'lvg_bias_act_grad_bias_slots', 'lvg_conv2d_frames_workgroups', 'lvg_conv2d_frames_planes_dot_rows', 'lvg_linear_act_work', 'lvg_linear_slope_bytes', 'lvg_linear_backward_work', 'lvg_rms_norm_backward_work') else ctypes.c_int
         _lib = handle
     return _lib
 

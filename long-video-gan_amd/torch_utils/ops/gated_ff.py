@@ -9,7 +9,7 @@ import torch
 
 from . import _rows
 from .bias_act import _resolve, activation_funcs
-from .linear_act import SLOPE_F32, SLOPE_NONE, _backward, _check, _forward, _sums_ref
+from .linear_act import SLOPE_SMOOTH, SLOPE_NONE, _backward, _check, _forward, _sums_ref
 
 
 def gated_ff(x, weight, b=None, act='swish', alpha=None, gain=1.0, x_scale=None, weight_scale=None, out_dtype=None, impl='cuda'):
@@ -44,7 +44,7 @@ def _gated_ff_ref(x, weight, b, act, alpha, gain, x_scale, weight_scale, out_dty
 class _GatedFF(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, b, act, alpha, gain):
-        h, slopes = _forward(x, weight, b, None, act, alpha, gain, -1.0, None, None, x.dtype, True, SLOPE_F32)
+        h, slopes = _forward(x, weight, b, None, act, alpha, gain, -1.0, None, None, x.dtype, True, SLOPE_SMOOTH)
         ctx.save_for_backward(x, weight, slopes)
         return h
 
@@ -53,4 +53,4 @@ class _GatedFF(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, slopes = ctx.saved_tensors
         # (the gain is in the slopes)
-        return *_backward(dy, x, weight, slopes, SLOPE_F32, 2, 0.0, 1.0, *ctx.needs_input_grad[:3]), None, None, None
+        return *_backward(dy, x, weight, slopes, SLOPE_SMOOTH, 2, 0.0, 1.0, *ctx.needs_input_grad[:3]), None, None, None

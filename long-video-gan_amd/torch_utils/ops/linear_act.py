@@ -12,7 +12,7 @@ import torch
 from . import _rows
 from .bias_act import _resolve, activation_funcs
 
-SLOPE_NONE, SLOPE_F32, SLOPE_CODE = 0, 1, 2
+SLOPE_NONE, SLOPE_SMOOTH, SLOPE_CODE = 0, 1, 2
 
 
 def linear_act(x, weight, b=None, residual=None, act='linear', alpha=None, gain=None, clamp=None, x_scale=None, weight_scale=None,
@@ -96,8 +96,8 @@ def _linear_act_ref(x, weight, b, residual, act, alpha, gain, clamp, x_scale, we
 # HIP path.
 
 def slope_kind(act, gated):
-    """How the forward pass keeps the derivative: piecewise linear activations as one byte an element, smooth ones as float32."""
-    return SLOPE_CODE if not gated and act in ('linear', 'relu', 'lrelu') else SLOPE_F32
+    """How the forward pass keeps the derivative: piecewise linear activations as one byte an element, smooth ones as values."""
+    return SLOPE_CODE if not gated and act in ('linear', 'relu', 'lrelu') else SLOPE_SMOOTH
 
 
 def _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype, gated, kind):
@@ -110,7 +110,7 @@ def _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_sc
     y = x.new_empty((rows, outer) if x.ndim == 2 else (*x.shape[:-1], outer), dtype=out_dtype)
     slopes = None
     if kind != SLOPE_NONE:
-        slopes = x.new_empty((rows, total), dtype=torch.float32 if kind == SLOPE_F32 else torch.uint8)
+        slopes = _rows.work_of(_rows.query('lvg_linear_slope_bytes', rows, outer, total // outer if outer else 1, kind, _rows.type_code(x.dtype)), device)
     if rows == 0 or outer == 0:
         return y, slopes
     r2 = None if residual is None else _rows.rows_of(residual, outer)
