@@ -524,8 +524,8 @@ int lvg_split32_stack(const float* x, void* out, int64_t pixels, int channels, i
 
 /* --------------------------------------------------------------------------------------------------------------------
  * Operators on matrices of token rows (csrc/token_*.hip, csrc/rms_norm.hip): the dense layers, gated units and norms of
- * row-wise networks. The reference runs its dense layers as torch.addmm / matmul + bias_act (model/generator_lres.py:60-80)
- * and has no gated unit, residual norm or 8-bit rows. Sizes and row strides are in elements, rows are dense (unit element
+ * row-wise networks. No pybind counterpart: dense layers are torch.addmm / matmul + bias_act in the reference's networks, which
+ * have no gated unit, residual norm or 8-bit rows. Sizes and row strides are in elements, rows are dense (unit element
  * stride) and may start at any element; 16-byte aligned rows are faster. Sums are float32, in a fixed order.
  */
 

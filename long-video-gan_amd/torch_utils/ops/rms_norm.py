@@ -3,8 +3,8 @@
     s = x + residual,   y = weight * s / sqrt(mean(s^2) + eps)
     q = y / scale in e4m3,   scale = max |y| of the row / 448
 
-Without weight and residual it is what the reference's mapping networks do to their input in tensor expressions
-(model/generator_lres.py:444-480). GPU tensors run the HIP kernels, CPU tensors and impl='ref' the plain-PyTorch definition."""
+Without weight and residual it is what the mapping networks do to their input in tensor expressions (reference
+model/generator_lres.py:444, LatentMappingNetwork). GPU tensors run the HIP kernels, CPU tensors and impl='ref' the plain-PyTorch definition."""
 
 import torch
 
