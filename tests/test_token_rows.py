@@ -352,6 +352,108 @@ def test_single_rows_and_8bit_layouts_gpu():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('act', ['linear', 'lrelu', 'swish'])
+def test_gradients_of_some_inputs_alone_gpu(act):
+    """Each subset of inputs that asks for a gradient gets the bits it gets when all of them ask."""
+    base = [rand(70, 96, seed=1, dtype=BF16), rand(80, 96, seed=2, dtype=BF16, scale=0.1), rand(80, seed=3, dtype=BF16)]
+    extra, dy, dh = rand(70, 80, seed=4, dtype=BF16), rand(70, 80, seed=5, dtype=BF16), rand(70, 40, seed=6, dtype=BF16)
+    norm = [rand(70, 80, seed=7, dtype=BF16), rand(80, seed=8, dtype=BF16), extra]
+
+    def run(wanted, kind):
+        ts = [t.clone().requires_grad_(i in wanted) for i, t in enumerate(norm if kind == 'norm' else base + ([extra] if kind == 'linear' else []))]
+        if kind == 'linear':
+            out = la.linear_act(ts[0], ts[1], ts[2], residual=ts[3], act=act)
+        elif kind == 'gated':
+            out = gf.gated_ff(ts[0], ts[1], ts[2], act=act)
+        else:
+            out = rn.rms_norm(ts[0], ts[1], residual=ts[2])[0]
+        return dict(zip(wanted, torch.autograd.grad(out, [ts[i] for i in wanted], dh if kind == 'gated' else dy)))
+
+    for kind, n in (('linear', 4), ('gated', 3), ('norm', 3)):
+        every = run(range(n), kind)
+        for mask in range(1, 2 ** n):
+            wanted = [i for i in range(n) if mask >> i & 1]
+            for i, g in run(wanted, kind).items():
+                assert torch.equal(g, every[i]), (kind, wanted, i)
+
+
+@pytest.mark.gpu
+def test_a_graph_can_be_walked_twice_gpu():
+    x, w = rand(33, 70, seed=1, dtype=F16).requires_grad_(True), rand(60, 70, seed=2, dtype=F16, scale=0.1).requires_grad_(True)
+    y, dy = gf.gated_ff(x, w), rand(33, 30, seed=3, dtype=F16)
+    first = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(y, (x, w), dy)))
+    with torch.inference_mode():
+        assert torch.equal(gf.gated_ff(x, w), y)
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once_gpu():
+    """Calls on two streams side by side, split over the summed index so that both use workspaces, give what they give alone."""
+    xs = [rand(40, 9000, seed=i, dtype=BF16) for i in (1, 2)]
+    w = rand(96, 9000, seed=3, dtype=BF16, scale=0.01)
+    want = [la.linear_act(x, w, act='swish') for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(la.linear_act(xs[i], w, act='swish'))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits_gpu():
+    """Operands and results of more than 2^32 bytes: the last rows are what a call on them alone gives."""
+    rows, width = 36000, 65536
+    big = torch.zeros(rows, width, dtype=BF16, device='cuda')
+    big[-70:] = rand(70, width, seed=1, dtype=BF16)
+    w = rand(48, width, seed=2, dtype=BF16, scale=width ** -0.5)
+    tail = big[-64:].clone()
+    assert big.numel() * 2 > 2 ** 32
+    y, alone = la.linear_act(big, w)[-64:].double(), la.linear_act(tail, w).double()
+    v, off = tr.sums64(tail, w, None)
+    tr.assert_within(y, v, tr.rounded(v, off, BF16), 'rows past 2^32')
+    tr.assert_within(alone, v, tr.rounded(v, off, BF16), 'rows')
+    n = rn.rms_norm(big, residual=big)[0]
+    assert torch.equal(n[-64:], rn.rms_norm(tail, residual=tail)[0])
+    del n
+    q, s = rn.quantize_rows(big)
+    q2, s2 = rn.quantize_rows(tail)
+    assert torch.equal(q[-64:].float(), q2.float()) and torch.equal(s[-64:], s2)
+    del q
+    # as the weight of a product (its rows' gradient read down them), and as a result
+    x = rand(40, 64, seed=3, dtype=BF16)
+    wide = rand(rows, 64, seed=4, dtype=BF16)
+    out = la.linear_act(rand(65536, 64, seed=5, dtype=BF16), wide)
+    assert out.numel() * 2 > 2 ** 32
+    tail_rows = rand(65536, 64, seed=5, dtype=BF16)[-50:]
+    v, off = tr.sums64(tail_rows, wide, None)
+    tr.assert_within(out[-50:], v, tr.rounded(v, off, BF16), 'result past 2^32')
+    del out
+    wl = rand(36000, 64, seed=6, dtype=BF16).requires_grad_(True)
+    xl = x.requires_grad_(True)
+    dy = torch.zeros(40, 36000, dtype=BF16, device='cuda')
+    dy[:, -3:] = 1
+    dx, dw = torch.autograd.grad(la.linear_act(xl, wl), (xl, wl), dy)
+    want = wl.detach().double()[-3:].sum(dim=0).expand(40, 64)
+    tr.assert_within(dx, want, tr.rounded(want, 5 * tr.F32_ULP * want.abs() + 1e-5, BF16), 'dx')
+    want = x.detach().double().sum(dim=0).expand(3, 64)
+    tr.assert_within(dw[-3:], want, tr.rounded(want, 50 * tr.F32_ULP * x.detach().double().abs().sum(dim=0).expand(3, 64), BF16), 'dw')
+    # the summed index runs down operands of more than 2^32 bytes
+    g = torch.zeros(rows, 40, dtype=BF16, device='cuda')
+    g[-2:] = 1
+    wb = rand(40, width, seed=7, dtype=BF16, scale=0.01).requires_grad_(True)
+    dw, = torch.autograd.grad(la.linear_act(big, wb), wb, g)
+    want = big[-2:].double().sum(dim=0).expand(40, width)
+    tr.assert_within(dw, want, tr.rounded(want, 4 * tr.F32_ULP * big[-2:].double().abs().sum(dim=0).expand(40, width), BF16), 'dw down')
+
+
+@pytest.mark.gpu
 def test_results_are_reproducible_gpu():
     x, w, dy = rand(700, 1100, seed=1, dtype=BF16), rand(1000, 1100, seed=2, dtype=BF16, scale=0.03), rand(700, 500, seed=3, dtype=BF16)
     x.requires_grad_(True), w.requires_grad_(True)
