@@ -26,6 +26,7 @@ struct NormArgs
     float*       scale;        // [rows], 8-bit results
     int64_t      rows, width, ldx, ldr, ldy;
     float        eps;
+    bool         past;         // results are stored past the caches
 };
 
 struct NormBackArgs
@@ -40,6 +41,7 @@ struct NormBackArgs
     float*       part;         // [slots][width] or NULL
     float*       coef;         // [rows]: wide rows only
     int64_t      rows, width, lddy, ldds, lds;
+    bool         past;
 };
 
 template <class T> __device__ __forceinline__ void store_rest(const NormArgs& p, int64_t row, int64_t at, const float* v)
@@ -127,7 +129,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
                 const int64_t at = (int64_t)(j * 64 * W + t) * V;
                 #pragma unroll
                 for (int i = 0; i < V; i++) v[j][i] += row_load(rr[j].v[i]);
-                if (p.sum) store_row<T>(static_cast<T*>(p.sum) + row * p.width + at, p.width - at, v[j]);
+                if (p.sum) store_row<T>(static_cast<T*>(p.sum) + row * p.width + at, p.width - at, v[j], p.past);
                 store_rest<T>(p, row, at, v[j]);
             }
         }
@@ -184,7 +186,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
         for (int j = 0; j < NV; j++)
         {
             const int64_t at = (int64_t)(j * 64 * W + t) * V;
-            store_row<T>(y + at, p.width - at, v[j]);
+            store_row<T>(y + at, p.width - at, v[j], p.past);
         }
     }
 }
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormB
                 v[i] = fmaf(row_load(now.g[j].v[i]) * w[j][i], r, -c * sum_at(now, j, i));
                 if (p.ds) v[i] += row_load(now.d[j].v[i]);
             }
-            store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, p.width - at, v);
+            store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, p.width - at, v, p.past);
         }
         if (kAhead) now = next;
         else if (row + step < p.rows) load(now, row + step);
@@ -481,6 +483,14 @@ Plan plan(int64_t width, int dtype)
     return {0, 0};
 }
 
+// Results of 64 MB and more, in aligned rows, go past the caches: the next operator would not find them there, and the rows still to be read stay
+// (16384 rows of 4096 bfloat16 with residual, forward and backward: 257 -> 224 us).
+bool past_caches(const void* a, const void* b, int64_t rows, int64_t width, int arrays, int dtype)
+{
+    const int64_t row = width * esize(dtype);
+    return row % 16 == 0 && lvg_aligned16(a) && lvg_aligned16(b) && arrays * rows * row >= (int64_t)64 << 20;
+}
+
 // Rows of one launch: a grid holds fewer than 2^32 threads.
 constexpr int64_t kLaunchRows = (int64_t)1 << 23;
 
@@ -553,7 +563,7 @@ extern "C" int lvg_rms_norm(const void* x, const void* residual, const void* wei
     LVG_REQUIRE(x && y && (!quantize || scale) && (!sum || residual) && (!rest || sum), "lvg_rms_norm: missing pointer");
     LVG_REQUIRE(x_stride >= 0 && residual_stride >= 0, "lvg_rms_norm: negative row stride");
     LVG_REQUIRE(eps >= 0.f, "lvg_rms_norm: eps must not be negative");
-    NormArgs a = {x, residual, weight, y, sum, dtype == LVG_F32 ? nullptr : static_cast<uint16_t*>(rest), rstd, scale, rows, width, x_stride, residual_stride, width, eps};
+    NormArgs a = {x, residual, weight, y, sum, dtype == LVG_F32 ? nullptr : static_cast<uint16_t*>(rest), rstd, scale, rows, width, x_stride, residual_stride, width, eps, !quantize && past_caches(y, sum, rows, width, sum ? 2 : 1, dtype)};
     const Plan k = plan(width, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     #define LVG_TYPE(T) { if (quantize) launch_norm<T, true, true>(a, k, s); else launch_norm<T, false, true>(a, k, s); }
@@ -568,7 +578,7 @@ extern "C" int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t r
     LVG_REQUIRE(rows_ok(rows, width), "lvg_quantize_rows: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
     if (rows == 0) return LVG_OK;
     LVG_REQUIRE(x && q && scale && x_stride >= 0, "lvg_quantize_rows: missing pointer or negative row stride");
-    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f};
+    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f, false};
     const Plan k = plan(width, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) launch_norm<float, true, false>(a, k, s);
@@ -604,7 +614,7 @@ extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const voi
     const int slots = back_slots(rows, width, dtype);
     float* const coef = k.waves ? nullptr : static_cast<float*>(work);
     float* const part = dw ? static_cast<float*>(work) + (k.waves ? 0 : (rows + 3) / 4 * 4) : nullptr;
-    NormBackArgs a = {dy, dsum, s_in, dtype == LVG_F32 ? nullptr : static_cast<const uint16_t*>(rest), weight, rstd, dx, part, coef, rows, width, dy_stride, dsum_stride, s_stride};
+    NormBackArgs a = {dy, dsum, s_in, dtype == LVG_F32 ? nullptr : static_cast<const uint16_t*>(rest), weight, rstd, dx, part, coef, rows, width, dy_stride, dsum_stride, s_stride, past_caches(dx, nullptr, rows, width, 1, dtype)};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) launch_back<float>(a, k, slots, s);
     else if (dtype == LVG_F16) launch_back<f16_t>(a, k, slots, s);

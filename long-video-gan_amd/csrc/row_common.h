@@ -49,13 +49,21 @@ template <class T> __device__ __forceinline__ RawRow<T> load_raw(const T* p, int
     return r;
 }
 
-template <class T> __device__ __forceinline__ void store_row(T* p, int64_t n, const float* v)
+// past: 16-byte aligned rows of a result larger than the caches, stored past them.
+template <class T> __device__ __forceinline__ void store_row(T* p, int64_t n, const float* v, bool past = false)
 {
     constexpr int V = Elem<T>::kVec;
     T r[V];
     #pragma unroll
     for (int i = 0; i < V; i++) r[i] = from_acc<T>(v[i]);
-    if (n >= V) __builtin_memcpy(p, r, 16);
+    if (n >= V && past)
+    {
+        typedef uint32_t vec __attribute__((ext_vector_type(4)));
+        vec w;
+        __builtin_memcpy(&w, r, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<vec*>(p));
+    }
+    else if (n >= V) __builtin_memcpy(p, r, 16);
     else
     {
         #pragma unroll

@@ -354,6 +354,7 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
     Finish& f = a.fin;
     auto whole = [&](const void* p, int64_t ld) { return !p || (((uintptr_t)p) % (4 * os) == 0 && ld % 4 == 0); };
     f.vec = cols % 4 == 0 && whole(f.bias, 0) && whole(f.residual, f.ldr) && whole(f.out, f.ldo) && (!f.slopes || lvg_aligned16(f.slopes));
+    f.past = gated && os == 2 && rows * cols * os + slope_bytes(rows, cols, 2, f.slopeKind, out_dtype) >= (int64_t)64 << 20;
     int rc, splits;
     if (streams(rows, form))
     {

@@ -691,7 +691,14 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                         here.keep(f, 0, kEdge ? f.vec : true, d);
                         here.keep(f, 1, kEdge ? f.vec : true, act);
                     }
-                    quad_store(here.out, kEdge ? left : 4, kEdge ? f.vec : true, v[t]);
+                    if (!kEdge && sizeof(O) == 2 && f.past)
+                    {
+                        Quad<O> q;
+                        #pragma unroll
+                        for (int k = 0; k < 4; k++) q.v[k] = from_acc<O>(v[t][k]);
+                        quad_past(here.out, q);
+                    }
+                    else quad_store(here.out, kEdge ? left : 4, kEdge ? f.vec : true, v[t]);
                 }
             }
         });

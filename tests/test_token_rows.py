@@ -352,6 +352,24 @@ def test_single_rows_and_8bit_layouts_gpu():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [F16, BF16])
+def test_results_larger_than_the_caches_gpu(dtype):
+    """64 MB and more of results are stored past the caches: whole tiles and those at the edges, rows of the norm, forward and backward."""
+    x, w = rand(2600, 64, seed=1, dtype=dtype), rand(2 * 4360, 64, seed=2, dtype=dtype, scale=0.125)
+    check_gated(x, w, rand(2 * 4360, seed=3, dtype=dtype), dy=rand(2600, 4360, seed=5, dtype=dtype))
+    (q, s), (qw, sw) = rn.quantize_rows(rand(4200, 64, seed=6)), rn.quantize_rows(rand(2 * 8192, 64, seed=7, scale=0.125))
+    v, off = tr.sums64(q.float(), qw.float(), None, s, sw)
+    a, _, a_off, _ = tr.slopes64(v[:, :8192], off[:, :8192], 'swish', 0.0, 1.0, None)
+    up, up_off = v[:, 8192:], off[:, 8192:]
+    want = a * up
+    bound = a.abs() * up_off + up.abs() * a_off + a_off * up_off + tr.F32_ULP * want.abs()
+    tr.assert_within(gf.gated_ff(q, qw, x_scale=s, weight_scale=sw, out_dtype=dtype), want, tr.rounded(want, bound, dtype), 'h')
+    for shape in ((8300, 4096), (70000, 520)):
+        x, w, r, dy, ds = (rand(*sh, seed=i, dtype=dtype) for i, sh in enumerate([shape, shape[-1:], shape, shape, shape]))
+        check_norm(x, w, r, dy=dy, ds=ds)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('act', ['linear', 'lrelu', 'swish'])
 def test_gradients_of_some_inputs_alone_gpu(act):
     """Each subset of inputs that asks for a gradient gets the bits it gets when all of them ask."""
