@@ -26,7 +26,7 @@ struct NormArgs
     float*       scale;        // [rows], 8-bit results
     int64_t      rows, width, ldx, ldr, ldy;
     float        eps;
-    bool         past;         // results are stored past the caches
+    bool         past, once;   // results are stored past the caches, operands loaded past them
 };
 
 struct NormBackArgs
@@ -41,7 +41,7 @@ struct NormBackArgs
     float*       part;         // [slots][width] or NULL
     float*       coef;         // [rows]: wide rows only
     int64_t      rows, width, lddy, ldds, lds;
-    bool         past;
+    bool         past, once;
 };
 
 template <class T> __device__ __forceinline__ void store_rest(const NormArgs& p, int64_t row, int64_t at, const float* v)
@@ -111,8 +111,8 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
     for (int j = 0; j < NV; j++)
     {
         const int64_t at = (int64_t)(j * 64 * W + t) * V;
-        xr[j] = load_raw<T>(x + at, p.width - at);
-        if (res) rr[j] = load_raw<T>(res + at, p.width - at);
+        xr[j] = load_raw<T>(x + at, p.width - at, p.once);
+        if (res) rr[j] = load_raw<T>(res + at, p.width - at, p.once);
     }
     float v[NV][V];
     #pragma unroll
@@ -305,9 +305,9 @@ __global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormB
         for (int j = 0; j < NV; j++)
         {
             const int64_t at = (int64_t)(j * 64 * W + t) * V;
-            x.g[j] = load_raw<T>(dy + at, p.width - at);
-            x.s[j] = load_raw<T>(s + at, p.width - at);
-            if (p.ds) x.d[j] = load_raw<T>(ds + at, p.width - at);
+            x.g[j] = load_raw<T>(dy + at, p.width - at, p.once);
+            x.s[j] = load_raw<T>(s + at, p.width - at, p.once);
+            if (p.ds) x.d[j] = load_raw<T>(ds + at, p.width - at, p.once);
             x.rest[j] = sizeof(T) == 2 && p.rest && at < p.width ? p.rest[row * ((p.width + 7) / 8) + at / 8] : 0x5555u;     // (0x5555: nothing left)
         }
     };
@@ -483,13 +483,12 @@ Plan plan(int64_t width, int dtype)
     return {0, 0};
 }
 
-// Results of 64 MB and more, in aligned rows, go past the caches: the next operator would not find them there, and the rows still to be read stay
-// (16384 rows of 4096 bfloat16 with residual, forward and backward: 257 -> 224 us).
-bool past_caches(const void* a, const void* b, int64_t rows, int64_t width, int arrays, int dtype)
-{
-    const int64_t row = width * esize(dtype);
-    return row % 16 == 0 && lvg_aligned16(a) && lvg_aligned16(b) && arrays * rows * row >= (int64_t)64 << 20;
-}
+// Matrices of 64 MB and more, in aligned rows, go past the caches, the operands (each value is read by one lane, once) and the results (the next
+// operator would not find them there): 16384 rows of 4096 bfloat16 with residual, forward and backward, 257 us with plain accesses, 224 us with
+// the stores past the caches, 193 us with the loads too; 8192 rows of 8192 to 8 bits 38.6 and 33.9 us.
+constexpr int64_t kLarge = (int64_t)64 << 20;
+bool aligned_rows(const void* p, int64_t stride, int dtype) { return !p || (lvg_aligned16(p) && stride * esize(dtype) % 16 == 0); }
+bool large(int64_t rows, int64_t width, int arrays, int dtype) { return arrays * rows * width * esize(dtype) >= kLarge; }
 
 // Rows of one launch: a grid holds fewer than 2^32 threads.
 constexpr int64_t kLaunchRows = (int64_t)1 << 23;
@@ -563,7 +562,9 @@ extern "C" int lvg_rms_norm(const void* x, const void* residual, const void* wei
     LVG_REQUIRE(x && y && (!quantize || scale) && (!sum || residual) && (!rest || sum), "lvg_rms_norm: missing pointer");
     LVG_REQUIRE(x_stride >= 0 && residual_stride >= 0, "lvg_rms_norm: negative row stride");
     LVG_REQUIRE(eps >= 0.f, "lvg_rms_norm: eps must not be negative");
-    NormArgs a = {x, residual, weight, y, sum, dtype == LVG_F32 ? nullptr : static_cast<uint16_t*>(rest), rstd, scale, rows, width, x_stride, residual_stride, width, eps, !quantize && past_caches(y, sum, rows, width, sum ? 2 : 1, dtype)};
+    NormArgs a = {x, residual, weight, y, sum, dtype == LVG_F32 ? nullptr : static_cast<uint16_t*>(rest), rstd, scale, rows, width, x_stride, residual_stride, width, eps, false, false};
+    a.past = !quantize && large(rows, width, sum ? 2 : 1, dtype) && aligned_rows(y, width, dtype) && aligned_rows(sum, width, dtype);
+    a.once = large(rows, width, residual ? 2 : 1, dtype) && aligned_rows(x, x_stride, dtype) && aligned_rows(residual, residual_stride, dtype);
     const Plan k = plan(width, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     #define LVG_TYPE(T) { if (quantize) launch_norm<T, true, true>(a, k, s); else launch_norm<T, false, true>(a, k, s); }
@@ -578,7 +579,7 @@ extern "C" int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t r
     LVG_REQUIRE(rows_ok(rows, width), "lvg_quantize_rows: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
     if (rows == 0) return LVG_OK;
     LVG_REQUIRE(x && q && scale && x_stride >= 0, "lvg_quantize_rows: missing pointer or negative row stride");
-    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f, false};
+    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f, false, large(rows, width, 1, dtype) && aligned_rows(x, x_stride, dtype)};
     const Plan k = plan(width, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) launch_norm<float, true, false>(a, k, s);
@@ -614,7 +615,9 @@ extern "C" int lvg_rms_norm_backward(const void* dy, const void* dsum, const voi
     const int slots = back_slots(rows, width, dtype);
     float* const coef = k.waves ? nullptr : static_cast<float*>(work);
     float* const part = dw ? static_cast<float*>(work) + (k.waves ? 0 : (rows + 3) / 4 * 4) : nullptr;
-    NormBackArgs a = {dy, dsum, s_in, dtype == LVG_F32 ? nullptr : static_cast<const uint16_t*>(rest), weight, rstd, dx, part, coef, rows, width, dy_stride, dsum_stride, s_stride, past_caches(dx, nullptr, rows, width, 1, dtype)};
+    NormBackArgs a = {dy, dsum, s_in, dtype == LVG_F32 ? nullptr : static_cast<const uint16_t*>(rest), weight, rstd, dx, part, coef, rows, width, dy_stride, dsum_stride, s_stride, false, false};
+    a.past = large(rows, width, 1, dtype) && aligned_rows(dx, width, dtype);
+    a.once = large(rows, width, 2, dtype) && aligned_rows(dy, dy_stride, dtype) && aligned_rows(dsum, dsum_stride, dtype) && aligned_rows(s_in, s_stride, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) launch_back<float>(a, k, slots, s);
     else if (dtype == LVG_F16) launch_back<f16_t>(a, k, slots, s);

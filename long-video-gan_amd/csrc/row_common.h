@@ -35,11 +35,18 @@ template <class T> __device__ __forceinline__ void load_row(const T* p, int64_t 
 
 // The same in two steps, for loads that are to be on their way early: the raw vector, then its values.
 template <class T> struct RawRow { T v[Elem<T>::kVec]; };
-template <class T> __device__ __forceinline__ RawRow<T> load_raw(const T* p, int64_t n)
+// once: 16-byte aligned rows of more than the caches hold, read by nobody else.
+template <class T> __device__ __forceinline__ RawRow<T> load_raw(const T* p, int64_t n, bool once = false)
 {
     constexpr int V = Elem<T>::kVec;
     RawRow<T> r;
-    if (n >= V) __builtin_memcpy(&r, p, 16);
+    if (n >= V && once)
+    {
+        typedef uint32_t vec __attribute__((ext_vector_type(4)));
+        const vec w = __builtin_nontemporal_load(reinterpret_cast<const vec*>(p));
+        __builtin_memcpy(&r, &w, 16);
+    }
+    else if (n >= V) __builtin_memcpy(&r, p, 16);
     else
     {
         __builtin_memset(&r, 0, 16);

@@ -367,6 +367,8 @@ def test_results_larger_than_the_caches_gpu(dtype):
     for shape in ((8300, 4096), (70000, 520)):
         x, w, r, dy, ds = (rand(*sh, seed=i, dtype=dtype) for i, sh in enumerate([shape, shape[-1:], shape, shape, shape]))
         check_norm(x, w, r, dy=dy, ds=ds)
+        q, scale = rn.quantize_rows(x.detach())
+        check_8bit_rows(q, scale, x.detach().double(), 0.0)
 
 
 @pytest.mark.gpu
