@@ -63,14 +63,17 @@ struct SlopeArgs
     int         kind;
     int         lanes;         // threads of a workgroup along the columns, a power of two
     float       alpha, gain;
+    bool        once;          // large and aligned: dy, slopes and dz go past the caches
 };
 
-// A thread owns one vector of columns (gated: of both halves, dy is read once) and takes its rows four at a time, all loads first.
+// A thread owns one vector of columns (gated: of both halves, dy is read once) and walks down its rows. One row at a time: several rows' loads ahead of
+// their use cost more waves than they gain (8192 x 2 x 8192 bfloat16: 314 us with four rows, 172 with one or two; 156 with loads and stores past the
+// caches, 4.5 TB/s).
 template <class T, int H>
 __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
 {
     typedef typename Kept<T>::S S;
-    constexpr int V = Elem<T>::kVec, R = 2, kE = Elem<S>::kVec;        // kE: derivatives of a 16-byte vector
+    constexpr int V = Elem<T>::kVec, kE = Elem<S>::kVec;               // kE: derivatives of a 16-byte vector
     const int64_t quads = (p.cols + 3) / 4;
     __shared__ float sums[256][V + 1];
     const int tid = threadIdx.x, cl = tid & (p.lanes - 1), rl = tid / p.lanes, rstep = 256 / p.lanes;
@@ -82,52 +85,43 @@ __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
     for (int h = 0; h < H; h++)
         #pragma unroll
         for (int i = 0; i < V; i++) db[h][i] = 0.f;
-    // N rows from m0 on; WHOLE: the thread's vector is not cut by the last column. No branch lies between the loads.
-    auto take = [&](int64_t m0, auto count, auto isWhole)
+    // WHOLE: the thread's vector is not cut by the last column
+    auto walk = [&](auto isWhole, auto isOnce)
     {
-        constexpr int N = decltype(count)::value;
-        constexpr bool WHOLE = decltype(isWhole)::value != 0;
+        constexpr bool WHOLE = decltype(isWhole)::value != 0, once = decltype(isOnce)::value != 0;
         const int64_t have = WHOLE ? V : left;
-        RawRow<T> g[N];
-        RawRow<S> d[N][H][V / kE];
-        uint32_t bits[N][H];
-        uint8_t c[N][V];
-        #pragma unroll
-        for (int r = 0; r < N; r++) g[r] = load_raw<T>(static_cast<const T*>(p.dy) + (m0 + r * rstep) * p.lddy + n, have);
-        if (p.kind == LVG_SLOPE_SMOOTH)
+        for (int64_t m = r0 + rl; m < r1; m += rstep)
         {
-            #pragma unroll
-            for (int r = 0; r < N; r++)
+            const RawRow<T> g = load_raw<T>(static_cast<const T*>(p.dy) + m * p.lddy + n, have, once);
+            RawRow<S> d[H][V / kE];
+            uint32_t bits[H];
+            uint8_t c[V];
+            if (p.kind == LVG_SLOPE_SMOOTH)
+            {
                 #pragma unroll
                 for (int h = 0; h < H; h++)
                 {
-                    const int64_t row = (m0 + r * rstep) * H + h;
+                    const int64_t row = m * H + h;
                     #pragma unroll
-                    for (int k = 0; k < V / kE; k++) d[r][h][k] = load_raw<S>(static_cast<const S*>(p.slopes) + row * p.cols + n + kE * k, have - kE * k);
+                    for (int k = 0; k < V / kE; k++) d[h][k] = load_raw<S>(static_cast<const S*>(p.slopes) + row * p.cols + n + kE * k, have - kE * k, once);
                     if constexpr (Kept<T>::kBits)
                     {
                         const uint8_t* at = reinterpret_cast<const uint8_t*>(static_cast<const S*>(p.slopes) + p.rows * H * p.cols) + row * quads + n / 4;
-                        bits[r][h] = at[0];
-                        if (WHOLE || have > 4) bits[r][h] |= (uint32_t)at[1] << 8;
+                        bits[h] = at[0];
+                        if (WHOLE || have > 4) bits[h] |= (uint32_t)at[1] << 8;
                     }
                 }
-        }
-        else if (p.kind == LVG_SLOPE_CODE)
-        {
-            #pragma unroll
-            for (int r = 0; r < N; r++)
+            }
+            else if (p.kind == LVG_SLOPE_CODE)
             {
-                const uint8_t* s = static_cast<const uint8_t*>(p.slopes) + (m0 + r * rstep) * p.cols + n;
-                if (WHOLE) __builtin_memcpy(c[r], s, V);
+                const uint8_t* s = static_cast<const uint8_t*>(p.slopes) + m * p.cols + n;
+                if (WHOLE) __builtin_memcpy(c, s, V);
                 else
                 {
                     #pragma unroll
-                    for (int i = 0; i < V; i++) c[r][i] = i < have ? s[i] : (uint8_t)0;
+                    for (int i = 0; i < V; i++) c[i] = i < have ? s[i] : (uint8_t)0;
                 }
             }
-        }
-        #pragma unroll
-        for (int r = 0; r < N; r++)
             #pragma unroll
             for (int h = 0; h < H; h++)
             {
@@ -135,28 +129,25 @@ __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
                 #pragma unroll
                 for (int i = 0; i < V; i++)
                 {
-                    v[i] = row_load(g[r].v[i]);
+                    v[i] = row_load(g.v[i]);
                     if (p.kind == LVG_SLOPE_SMOOTH)
                     {
-                        const float s = row_load(d[r][h][i / kE].v[i % kE]);
-                        if constexpr (Kept<T>::kBits) v[i] *= __uint_as_float(__float_as_uint(s) | (bits[r][h] >> (2 * i) & 3u) << 14);
+                        const float s = row_load(d[h][i / kE].v[i % kE]);
+                        if constexpr (Kept<T>::kBits) v[i] *= __uint_as_float(__float_as_uint(s) | (bits[h] >> (2 * i) & 3u) << 14);
                         else v[i] *= s;
                     }
-                    else if (p.kind == LVG_SLOPE_CODE) v[i] = c[r][i] == 2 ? v[i] : c[r][i] == 1 ? v[i] * p.alpha : 0.f;
+                    else if (p.kind == LVG_SLOPE_CODE) v[i] = c[i] == 2 ? v[i] : c[i] == 1 ? v[i] * p.alpha : 0.f;
                     v[i] *= p.gain;
                     db[h][i] += v[i];
                 }
-                if (p.dz) store_row<T>(static_cast<T*>(p.dz) + (m0 + r * rstep) * p.lddz + h * p.cols + n, have, v);
+                if (p.dz) store_row<T>(static_cast<T*>(p.dz) + m * p.lddz + h * p.cols + n, have, v, once);
             }
+        }
     };
-    auto run = [&](auto isWhole)
-    {
-        int64_t m0 = r0 + rl;
-        for (; m0 + (R - 1) * rstep < r1; m0 += R * rstep) take(m0, Const<R>(), isWhole);
-        for (; m0 < r1; m0 += rstep) take(m0, Const<1>(), isWhole);
-    };
-    if (left >= V) run(Const<1>());
-    else if (left > 0) run(Const<0>());
+    // (with `once` every vector is whole and aligned)
+    if (p.once && left >= V) walk(Const<1>(), Const<1>());
+    else if (left >= V) walk(Const<1>(), Const<0>());
+    else if (left > 0) walk(Const<0>(), Const<0>());
     if (!p.part) return;
     #pragma unroll
     for (int h = 0; h < H; h++)
@@ -534,7 +525,9 @@ extern "C" int lvg_linear_backward(const void* dy, const void* slopes, const voi
     if (!none && (!plain || db))
     {
         float* part = db ? reinterpret_cast<float*>(mem + k.dz) : nullptr;
-        SlopeArgs a = {dy, slopes, plain ? nullptr : mem, part, rows, outer, dy_stride, k.dzStride, slope_kind, slope_lanes(outer, esize_of(dtype)), alpha, plain ? 1.f : gain};
+        SlopeArgs a = {dy, slopes, plain ? nullptr : mem, part, rows, outer, dy_stride, k.dzStride, slope_kind, slope_lanes(outer, esize_of(dtype)), alpha, plain ? 1.f : gain, false};
+        const int es = esize_of(dtype);
+        a.once = rows * total * es >= (int64_t)64 << 20 && lvg_aligned16(dy) && (dy_stride * es) % 16 == 0 && (outer * es) % 16 == 0 && (!slopes || lvg_aligned16(slopes));
         const dim3 grid((unsigned)lvg_ceil_div(lvg_ceil_div(outer, 16 / esize_of(dtype)), a.lanes), (unsigned)k.slots), block(256);
         #define LVG_TYPE(T) { \
             if (halves == 2) hipLaunchKernelGGL((token_slope_kernel<T, 2>), grid, block, 0, s, a); \
