@@ -280,10 +280,10 @@ template <class O, bool GATED> __device__ __forceinline__ void finish4(const Fin
         if (f.clamp >= 0.f)
         {
             inside = !(fabsf(a[i]) >= f.clamp);         // (a NaN is inside: it stays one)
-            if (!inside) { a[i] = a[i] > 0.f ? f.clamp : -f.clamp; d[i] = 0.f; }
+            if (!inside) { a[i] = a[i] > 0.f ? f.clamp : -f.clamp; d[i] = -0.f; }     // (-0: nothing passes, see token_slope_kernel)
         }
-        // 0: no gradient, 1: alpha (lrelu's lower side; relu has alpha 0), 2: one
-        code |= (uint32_t)(!inside ? 0 : (f.act != LVG_ACT_LINEAR && !(v[i] > 0.f)) ? 1 : 2) << (8 * i);
+        // 0: no gradient (cut, or relu's lower side), 1: alpha (lrelu's), 2: one
+        code |= (uint32_t)(!inside || (f.act == LVG_ACT_RELU && v[i] <= 0.f) ? 0 : (f.act == LVG_ACT_LRELU && !(v[i] > 0.f)) ? 1 : 2) << (8 * i);
     }
     if (f.slopeKind == LVG_SLOPE_SMOOTH) at.keep(f, 0, f.vec, d);
     else if (f.slopeKind == LVG_SLOPE_CODE)

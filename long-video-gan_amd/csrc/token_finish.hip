@@ -132,9 +132,10 @@ __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
                     v[i] = row_load(g.v[i]);
                     if (p.kind == LVG_SLOPE_SMOOTH)
                     {
-                        const float s = row_load(d[h][i / kE].v[i % kE]);
-                        if constexpr (Kept<T>::kBits) v[i] *= __uint_as_float(__float_as_uint(s) | (bits[h] >> (2 * i) & 3u) << 14);
-                        else v[i] *= s;
+                        float s = row_load(d[h][i / kE].v[i % kE]);
+                        if constexpr (Kept<T>::kBits) s = __uint_as_float(__float_as_uint(s) | (bits[h] >> (2 * i) & 3u) << 14);
+                        // (the clamp's -0 stops infinities and NaNs too; gated units have no clamp)
+                        v[i] = H == 1 && __float_as_uint(s) == 0x80000000u ? 0.f : v[i] * s;
                     }
                     else if (p.kind == LVG_SLOPE_CODE) v[i] = c[i] == 2 ? v[i] : c[i] == 1 ? v[i] * p.alpha : 0.f;
                     v[i] *= p.gain;

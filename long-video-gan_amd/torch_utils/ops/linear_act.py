@@ -159,8 +159,7 @@ class _LinearAct(torch.autograd.Function):
         kind = slope_kind(act, False) if needed and (act != 'linear' or clamp >= 0) else SLOPE_NONE
         y, slopes = _forward(x, weight, b, residual, act, alpha, gain, clamp, None, None, x.dtype, False, kind)
         ctx.save_for_backward(x, weight, slopes)
-        # (relu's lower side has no gradient whatever alpha a caller passed)
-        ctx.args = kind, 0.0 if act == 'relu' else alpha, gain
+        ctx.args = kind, alpha, gain
         return y
 
     @staticmethod

@@ -710,3 +710,42 @@ def test_second_derivatives_are_refused_gpu():
     g, = torch.autograd.grad(la.linear_act(x, w, act='tanh').sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows', [5, 70, 300])
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('act,clamp', [('relu', None), ('relu', 2.0), ('lrelu', 0.25), ('swish', 0.25), ('tanh', 0.25)])
+def test_infinite_gradients_where_none_passes_gpu(act, clamp, dtype, rows):
+    # relu's lower side and what the clamp cut take no gradient at all, infinite or NaN ones neither. Sums are +-1 exactly: sum(x w) = s, |s| = 1.
+    outer, inner = 72, 40
+    x = torch.zeros(rows, inner)
+    x[:, 0] = 1
+    w = torch.zeros(outer, inner)
+    w[:, 0] = torch.tensor([1.0, -1.0]).repeat(outer // 2)
+    x, w = (t.to('cuda', dtype).requires_grad_() for t in (x, w))
+    y = la.linear_act(x, w, act=act, gain=1.0, clamp=clamp)
+    dy = torch.ones(rows, outer, device='cuda', dtype=dtype)
+    cut = torch.zeros(outer, dtype=torch.bool)
+    if act == 'relu':
+        cut[1::2] = True                                   # sums of -1
+    else:
+        cut[0::2] = True                                   # 1, 0.73 and 0.76 are cut at 0.25; the lower side:
+        cut[1::2] = act != 'lrelu'                         # -0.2 is not, -0.27 and -0.76 are
+    dy[0, cut.cuda()] = torch.inf
+    dy[-1, cut.cuda()] = torch.nan
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    # relu's upper side: slope 1 (1 is below the clamp of 2); lrelu's lower side: 0.2; nothing else passes
+    slope = torch.zeros(outer, dtype=torch.float64)
+    if act == 'relu':
+        slope[0::2] = 1
+    elif act == 'lrelu':
+        slope[1::2] = 0.2
+    want_x = torch.zeros(rows, inner, dtype=torch.float64)
+    want_x[:, 0] = (slope * w.detach().double().cpu()[:, 0]).sum()
+    want_w = torch.zeros(outer, inner, dtype=torch.float64)
+    want_w[:, 0] = slope * rows
+    # dz is rounded once (lrelu: 0.2), the sum of equal signs once more: two half steps; the float32 sums of up to 300 terms: 300 of theirs
+    bound = 2 * torch.finfo(dtype).eps / 2 + 300 * 2.0 ** -24
+    for got, want in ((dx, want_x), (dw, want_w)):
+        assert ((got.double().cpu() - want).abs() <= bound * want.abs()).all()
