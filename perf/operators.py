@@ -10,7 +10,6 @@ All four work on matrices of rows (a row is one token, one frame's latent or one
 `run` computes the plain form in float32 (`own` False) or calls the operators (`own` True). Training cases return the result
 and every gradient; cases of type e4m3 multiply 8-bit rows by 8-bit weights, each with its scales."""
 
-import functools
 import math
 import os
 import sys
@@ -28,7 +27,6 @@ _EPS = 1e-6
 _GAINS = {'linear': 1.0, 'lrelu': math.sqrt(2), 'relu': math.sqrt(2), 'swish': math.sqrt(2), 'tanh': 1.0, 'sigmoid': 1.0, 'softplus': 1.0}
 
 
-@functools.lru_cache(maxsize=None)      # a user's program imports once
 def _ops():
     package = os.path.join(_ROOT, 'long-video-gan_amd')
     if package not in sys.path:
