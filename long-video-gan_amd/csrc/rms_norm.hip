@@ -161,7 +161,8 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
             #pragma unroll
             for (int i = 0; i < V; i++) if (i < left) top = max(top, magnitude(v[j][i]));
         }
-        const float scale = row_scale(row_largest<W>(top, tops, wave)), inv = 1.f / scale;
+        const float scale = row_scale(row_largest<W>(top, tops, wave));
+        const Divisor by(scale);
         if (t == 0) p.scale[row] = scale;
         uint8_t* q = static_cast<uint8_t*>(p.y) + row * p.ldy;
         #pragma unroll
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
             const int64_t at = (int64_t)(j * 64 * W + t) * V, left = p.width - at;
             uint32_t w[V / 4];
             #pragma unroll
-            for (int i = 0; i < V; i += 4) w[i / 4] = pack_e4m3(v[j][i] * inv, v[j][i + 1] * inv, v[j][i + 2] * inv, v[j][i + 3] * inv);
+            for (int i = 0; i < V; i += 4) w[i / 4] = pack_e4m3(by.quotient(v[j][i]), by.quotient(v[j][i + 1]), by.quotient(v[j][i + 2]), by.quotient(v[j][i + 3]));
             if (left >= V) __builtin_memcpy(q + at, w, V);
             else
             {
@@ -239,7 +240,7 @@ __global__ __launch_bounds__(256) void rms_norm_wide_kernel(NormArgs p)
         #pragma unroll
         for (int i = 0; i < V; i++) v[i] = p.weight ? v[i] * r * w[i] : v[i] * r;
     };
-    float inv = 1.f;
+    float scale = 1.f;
     if (QUANT)
     {
         uint32_t top = 0;
@@ -250,10 +251,10 @@ __global__ __launch_bounds__(256) void rms_norm_wide_kernel(NormArgs p)
             #pragma unroll
             for (int i = 0; i < V; i++) if (at + i < p.width) top = max(top, magnitude(v[i]));
         }
-        const float scale = row_scale(row_largest<4>(top, tops, wave));
+        scale = row_scale(row_largest<4>(top, tops, wave));
         if (threadIdx.x == 0) p.scale[row] = scale;
-        inv = 1.f / scale;
     }
+    const Divisor by(scale);
     for (int64_t at = (int64_t)threadIdx.x * V; at < p.width; at += 256 * V)
     {
         float v[V];
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(256) void rms_norm_wide_kernel(NormArgs p)
             #pragma unroll
             for (int i = 0; i < V; i += 4)
             {
-                const uint32_t w = pack_e4m3(v[i] * inv, v[i + 1] * inv, v[i + 2] * inv, v[i + 3] * inv);
+                const uint32_t w = pack_e4m3(by.quotient(v[i]), by.quotient(v[i + 1]), by.quotient(v[i + 2]), by.quotient(v[i + 3]));
                 #pragma unroll
                 for (int k = 0; k < 4; k++) if (at + i + k < p.width) q[i + k] = (uint8_t)(w >> (8 * k));
             }

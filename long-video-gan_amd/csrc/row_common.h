@@ -130,6 +130,24 @@ __device__ __forceinline__ float row_scale(uint32_t largest)
     return s < kScaleMin ? kScaleMin : s;
 }
 
+// Quotients by one scale, rounded as a division rounds them. The reciprocal and what its rounding left give a quotient within one unit in the last
+// place; the exact remainder corrects it to the nearest value (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000", 1990).
+// Values of 16 bits meet e4m3's ties often: with the rounded reciprocal alone 4 % of the rows of 8192 bfloat16 hold a code that is off by a step. A
+// division an element would take three times the instructions.
+struct Divisor
+{
+    float scale, inv, rest;
+    __device__ __forceinline__ explicit Divisor(float s) : scale(s), inv(1.f / s), rest(fmaf(-s, inv, 1.f) * inv)
+    {
+        if (isinf(s)) scale = rest = 0.f;          // finite / infinity = 0, infinity / infinity = NaN
+    }
+    __device__ __forceinline__ float quotient(float v) const
+    {
+        const float q = fmaf(v, inv, v * rest);
+        return fmaf(fmaf(-q, scale, v), inv, q);
+    }
+};
+
 } // namespace
 
 // out [width] (type dtype) = gain * sum over the slots of part [slots][width] (rms_norm.hip).

@@ -61,7 +61,8 @@ def quantize_rows(x, impl='cuda'):
 
 
 def _quantize_ref(v):
-    scale = (v.abs().amax(dim=-1) / _rows.E4M3_MAX).clamp(min=_rows.SCALE_MIN)
+    top = v.abs().amax(dim=-1)
+    scale = (top / top.new_full((), _rows.E4M3_MAX)).clamp(min=_rows.SCALE_MIN)         # (a tensor: torch multiplies by a number's reciprocal on the GPU)
     return (v / scale.unsqueeze(-1)).clamp(-_rows.E4M3_MAX, _rows.E4M3_MAX).to(torch.float8_e4m3fn), scale
 
 

@@ -1,0 +1,56 @@
+"""Operators on token rows at the edges of what their documentation allows: values far from one, infinite gradients, derivative and trace modes that
+pass an autograd function by, sizes near the limits of a launch, what a backward pass keeps and allocates. Bounds as in tests/helpers/token_rows.py."""
+
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwad
+
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), 'helpers'))
+import token_rows as tr  # noqa: E402
+from test_token_rows import check_norm, rand  # noqa: E402
+
+from torch_utils.ops import _hip
+from torch_utils.ops import gated_ff as gf
+from torch_utils.ops import linear_act as la
+from torch_utils.ops import rms_norm as rn
+
+F32, F16, BF16, E4M3 = torch.float32, torch.float16, torch.bfloat16, torch.float8_e4m3fn
+DTYPES = [F32, F16, BF16]
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'long-video-gan_amd', 'csrc')
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# 8-bit rows.
+
+def same_bits(a, b):
+    return torch.equal(a.cpu().view(torch.uint8), b.cpu().view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('shape', [(300, 5), (300, 64), (7, 515), (64, 4100), (64, 8192), (5, 40000)])
+def test_8bit_rows_are_the_quotients_gpu(shape, dtype):
+    """q = x / scale, one rounding of the float32 quotient: the plain form's bits, on either device. Values of 16 bits meet e4m3's ties often."""
+    size = torch.exp(0.4 * torch.randn(shape[1], generator=torch.Generator().manual_seed(2)))
+    x = (rand(*shape, seed=1, device='cpu') * size).to(dtype).cuda()
+    q, scale = rn.quantize_rows(x)
+    for want_q, want_scale in (rn.quantize_rows(x.cpu()), rn.quantize_rows(x, impl='ref')):
+        assert torch.equal(scale.cpu(), want_scale.cpu())
+        assert same_bits(q, want_q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('width', [64, 515, 4100, 8192, 40000])
+def test_8bit_norm_rows_are_the_quotients_gpu(width, dtype):
+    """Rows of +-1 have a mean square of exactly one, so the norm to 8 bits is the weight with their signs, to 8 bits."""
+    w = rand(width, seed=1, dtype=dtype)
+    x = torch.where(rand(9, width, seed=2) > 0, 1.0, -1.0).to(dtype)
+    q, scale = rn.rms_norm(x, w, eps=0.0, quantize=True)
+    want_q, want_scale = rn.quantize_rows((x.float() * w.float()).cpu())
+    assert torch.equal(scale.cpu(), want_scale) and same_bits(q, want_q)
