@@ -570,7 +570,7 @@ int lvg_rms_norm(const void* x, const void* residual, const void* weight, void* 
                  int64_t rows, int64_t width, int64_t x_stride, int64_t residual_stride, float eps, int dtype, int quantize, void* stream);
 
 /*
- * Gradient of lvg_rms_norm: with g = weight * dy, dx = rstd g - s rstd^3 mean(g s) + dsum (dsum: gradient of sum's other uses, or NULL); dx is also
+ * Gradient of lvg_rms_norm: with g = weight * dy and n = s rstd, dx = rstd (g - n mean(g n)) + dsum (dsum: gradient of sum's other uses, or NULL); dx is also
  * the residual's gradient. dw [width] = sum over rows of dy s rstd (or NULL). s, rest: the forward pass's sum and
  * rest; x and NULL where it had no residual. dx and dw are dense, of type dtype.
  * work: lvg_rms_norm_backward_work(...) bytes, 16-byte aligned; weight: whether dw is asked for.

@@ -2,7 +2,9 @@
 //
 //   s = x + residual,   r = 1 / sqrt(mean(s^2) + eps),   y = weight * s * r
 //   q = y / scale in e4m3,   scale = max |y| of the row / 448               (quantize)
-//   ds_in = r g - s r^3 mean(g s) + ds,   g = weight * dy,   dweight = sum over rows of dy s r
+//   ds_in = r (g - n mean(g n)) + ds,   n = s r,   g = weight * dy,   dweight = sum over rows of dy n
+//
+// (n is about one: the cube of r, which the same gradient can be written with, leaves float32's range from rows of 1e13 and 1e-13 on.)
 //
 // What a program otherwise spells as add, square, mean, rsqrt, two products, an absolute maximum and a cast: eight passes over the rows where
 // one has to read x and residual and write s and y. The gradient reads the sum as it was stored, rounded; two bits a value that the forward pass
@@ -339,13 +341,13 @@ __global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormB
             #pragma unroll
             for (int i = 0; i < V; i++)
             {
-                const float g = row_load(now.g[j].v[i]), s = sum_at(now, j, i);
-                dw[j][i] = fmaf(g, s * r, dw[j][i]);
-                dot = fmaf(g * w[j][i], s, dot);
+                const float g = row_load(now.g[j].v[i]), n = sum_at(now, j, i) * r;
+                dw[j][i] = fmaf(g, n, dw[j][i]);
+                dot = fmaf(g * w[j][i], n, dot);
             }
         }
         dot = row_total<W>(dot, sums[turn], wave);         // (two sets: a wave may reach the next row's while another still reads this one's)
-        const float c = r * r * r * (dot / (float)p.width);
+        const float c = dot / (float)p.width;
         #pragma unroll
         for (int j = 0; j < NV; j++)
         {
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormB
             #pragma unroll
             for (int i = 0; i < V; i++)
             {
-                v[i] = fmaf(row_load(now.g[j].v[i]) * w[j][i], r, -c * sum_at(now, j, i));
+                v[i] = fmaf(sum_at(now, j, i) * r, -c, row_load(now.g[j].v[i]) * w[j][i]) * r;
                 if (p.ds) v[i] += row_load(now.d[j].v[i]);
             }
             store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, p.width - at, v, p.past);
@@ -400,6 +402,7 @@ __global__ __launch_bounds__(256) void rms_norm_back_coef_kernel(NormBackArgs p)
     const int64_t row = blockIdx.x;
     const T* dy = static_cast<const T*>(p.dy) + row * p.lddy;
     const T* s = static_cast<const T*>(p.s) + row * p.lds;
+    const float r = p.rstd[row];
     float dot = 0.f;
     for (int64_t at = (int64_t)threadIdx.x * V; at < p.width; at += 256 * V)
     {
@@ -409,11 +412,10 @@ __global__ __launch_bounds__(256) void rms_norm_back_coef_kernel(NormBackArgs p)
         kept_sum<T>(p, row, at, sv);
         if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w);
         #pragma unroll
-        for (int i = 0; i < V; i++) dot = fmaf(p.weight ? g[i] * w[i] : g[i], sv[i], dot);
+        for (int i = 0; i < V; i++) dot = fmaf(p.weight ? g[i] * w[i] : g[i], sv[i] * r, dot);
     }
     dot = row_total<4>(dot, sums, threadIdx.x >> 6);
-    const float r = p.rstd[row];
-    if (threadIdx.x == 0) p.coef[row] = r * r * r * (dot / (float)p.width);
+    if (threadIdx.x == 0) p.coef[row] = dot / (float)p.width;
 }
 
 template <class T>
@@ -437,8 +439,9 @@ __global__ __launch_bounds__(256) void rms_norm_back_wide_kernel(NormBackArgs p)
         #pragma unroll
         for (int i = 0; i < V; i++)
         {
-            dw[i] = fmaf(g[i], sv[i] * r, dw[i]);
-            g[i] = fmaf(g[i] * w[i], r, -c * sv[i]) + (p.ds ? d[i] : 0.f);
+            const float n = sv[i] * r;
+            dw[i] = fmaf(g[i], n, dw[i]);
+            g[i] = fmaf(n, -c, g[i] * w[i]) * r + (p.ds ? d[i] : 0.f);
         }
         store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, left, g);
     }

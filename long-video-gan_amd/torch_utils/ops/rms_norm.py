@@ -71,7 +71,7 @@ def _rms_norm_ref(x, weight, residual, eps, quantize):
     s = x.float()
     if residual is not None:
         s = s + residual.float()
-    y = s * torch.rsqrt(s.square().mean(dim=-1, keepdim=True) + eps)
+    y = s / torch.sqrt(s.square().mean(dim=-1, keepdim=True) + eps)        # (rsqrt's gradient forms a cube that leaves float32's range)
     if weight is not None:
         y = y * weight.float()
     out = _quantize_ref(y) if quantize else (y.to(x.dtype),)

@@ -54,3 +54,24 @@ def test_8bit_norm_rows_are_the_quotients_gpu(width, dtype):
     q, scale = rn.rms_norm(x, w, eps=0.0, quantize=True)
     want_q, want_scale = rn.quantize_rows((x.float() * w.float()).cpu())
     assert torch.equal(scale.cpu(), want_scale) and same_bits(q, want_q)
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# Norm of rows far from one.
+
+@pytest.mark.parametrize('size', [1e15, 1e-15])
+def test_plain_norm_gradient_of_rows_far_from_one_cpu(size):
+    x, w, r, dy = (rand(*s, seed=i, device='cpu') for i, s in enumerate([(4, 9), (9,), (4, 9), (4, 9)]))
+    check_norm(x * size, w, r * size, eps=0.0, dy=dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [F32, BF16])
+@pytest.mark.parametrize('size', [1e15, 1e-15])
+@pytest.mark.parametrize('shape', [(9, 70), (5, 515), (9, 2500), (7, 8200), (3, 40000)])
+def test_norm_gradient_of_rows_far_from_one_gpu(shape, size, dtype):
+    """The cube of the reciprocal root leaves float32's range long before the gradient does."""
+    x, w, r, dy = (rand(*s, seed=i) for i, s in enumerate([shape, shape[-1:], shape, shape]))
+    x, r = (x * size).to(dtype), (r * size).to(dtype)
+    check_norm(x.clone(), w.to(dtype), r, eps=0.0, dy=dy.to(dtype))
+    check_norm(x.clone(), None, None, eps=0.0, dy=dy.to(dtype))
