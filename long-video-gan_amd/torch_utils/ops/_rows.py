@@ -4,6 +4,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _hip
 
@@ -38,6 +39,12 @@ def wants_grad(*tensors) -> bool:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def watched(*tensors) -> bool:
+    """Whether a call has to go through its autograd function: for gradients; while a trace is recorded, which would otherwise see the results'
+    allocations alone; and while forward derivatives are taken, which the function refuses where an input has one (the kernels have none)."""
+    return forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None or wants_grad(*tensors)         # pylint: disable=protected-access
 
 
 @functools.lru_cache(maxsize=4096)

@@ -30,8 +30,8 @@ def gated_ff(x, weight, b=None, act='swish', alpha=None, gain=1.0, x_scale=None,
     _, alpha, gain, _ = _resolve(act, alpha, gain, None)
     if impl == 'ref' or not x.is_cuda:
         return _gated_ff_ref(x, weight, b, act, alpha, gain, x_scale, weight_scale, out_dtype)
-    if _rows.wants_grad(x, weight, b):
-        return _GatedFF.apply(x, weight, b, act, alpha, gain)
+    if _rows.watched(x, weight, b):
+        return _GatedFF.apply(x, weight, b, x_scale, weight_scale, act, alpha, gain, out_dtype)
     return _forward(x, weight, b, None, act, alpha, gain, -1.0, x_scale, weight_scale, out_dtype, True, SLOPE_NONE)[0]
 
 
@@ -43,8 +43,9 @@ def _gated_ff_ref(x, weight, b, act, alpha, gain, x_scale, weight_scale, out_dty
 
 class _GatedFF(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, b, act, alpha, gain):
-        h, slopes = _forward(x, weight, b, None, act, alpha, gain, -1.0, None, None, x.dtype, True, SLOPE_SMOOTH)
+    def forward(ctx, x, weight, b, x_scale, weight_scale, act, alpha, gain, out_dtype):
+        kind = SLOPE_SMOOTH if any(ctx.needs_input_grad[:3]) and x_scale is None else SLOPE_NONE
+        h, slopes = _forward(x, weight, b, None, act, alpha, gain, -1.0, x_scale, weight_scale, out_dtype, True, kind)
         ctx.save_for_backward(x, weight, slopes)
         return h
 
@@ -53,4 +54,4 @@ class _GatedFF(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, slopes = ctx.saved_tensors
         # (the gain is in the slopes)
-        return *_backward(dy, x, weight, slopes, SLOPE_SMOOTH, 2, 0.0, 1.0, *ctx.needs_input_grad[:3]), None, None, None
+        return _backward(dy, x, weight, slopes, SLOPE_SMOOTH, 2, 0.0, 1.0, *ctx.needs_input_grad[:3]) + (None,) * 6

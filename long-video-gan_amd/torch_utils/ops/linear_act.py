@@ -31,10 +31,10 @@ def linear_act(x, weight, b=None, residual=None, act='linear', alpha=None, gain=
         out_dtype:    dtype of the result: x's, or for 8-bit x float16 or bfloat16 (default bfloat16).
         impl:         'cuda' (HIP kernels when x is on the GPU) or 'ref' (plain PyTorch).
 
-    Differentiable once in x, weight, b and residual (not with 8-bit operands). Sums are float32 (8-bit operands: the matrix unit adds the products of
-    eight neighbours with 13 bits below the largest of them, these sums are float32); the result is rounded once. A backward pass that is
-    captured into a graph needs leaves that no eager autograd graph still holds (torch ties a leaf's accumulation node to the stream of the graph
-    that made it): drop eager results, or detach them, before the capture."""
+    Differentiable once in x, weight, b and residual (not with 8-bit operands), backward; a dual tensor of a forward derivative is refused. Sums are
+    float32 (8-bit operands: the matrix unit adds the products of eight neighbours with 13 bits below the largest of them, these sums are float32);
+    the result is rounded once. A backward pass that is captured into a graph needs leaves that no eager autograd graph still holds (torch ties a
+    leaf's accumulation node to the stream of the graph that made it): drop eager results, or detach them, before the capture."""
     assert impl in ['ref', 'cuda']
     out_dtype = _check(x, weight, b, x_scale, weight_scale, out_dtype, halves=1)
     if residual is not None:
@@ -44,8 +44,8 @@ def linear_act(x, weight, b=None, residual=None, act='linear', alpha=None, gain=
     _, alpha, gain, clamp = _resolve(act, alpha, gain, clamp)
     if impl == 'ref' or not x.is_cuda:
         return _linear_act_ref(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype)
-    if _rows.wants_grad(x, weight, b, residual):
-        return _LinearAct.apply(x, weight, b, residual, act, alpha, gain, clamp)
+    if _rows.watched(x, weight, b, residual):
+        return _LinearAct.apply(x, weight, b, residual, x_scale, weight_scale, act, alpha, gain, clamp, out_dtype)
     return _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype, False, SLOPE_NONE)[0]
 
 
@@ -154,10 +154,10 @@ def _backward(dy, x, weight, slopes, kind, halves, alpha, gain, need_x, need_w, 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, b, residual, act, alpha, gain, clamp):
-        needed = any(ctx.needs_input_grad[:3])
+    def forward(ctx, x, weight, b, residual, x_scale, weight_scale, act, alpha, gain, clamp, out_dtype):
+        needed = any(ctx.needs_input_grad[:3]) and x_scale is None         # (set for leaves under no_grad too)
         kind = slope_kind(act, False) if needed and (act != 'linear' or clamp >= 0) else SLOPE_NONE
-        y, slopes = _forward(x, weight, b, residual, act, alpha, gain, clamp, None, None, x.dtype, False, kind)
+        y, slopes = _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype, False, kind)
         ctx.save_for_backward(x, weight, slopes)
         ctx.args = kind, alpha, gain
         return y
@@ -171,4 +171,4 @@ class _LinearAct(torch.autograd.Function):
         dx = dw = db = None
         if any(need[:3]):
             dx, dw, db = _backward(dy, x, weight, slopes, kind, 1, alpha, gain, *need[:3])
-        return dx, dw, db, dy if need[3] else None, None, None, None, None
+        return (dx, dw, db, dy if need[3] else None) + (None,) * 7

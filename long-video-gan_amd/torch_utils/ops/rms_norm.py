@@ -23,7 +23,8 @@ def rms_norm(x, weight=None, residual=None, eps=1e-8, quantize=False, impl='cuda
         impl:     'cuda' (HIP kernels when x is on the GPU) or 'ref' (plain PyTorch).
 
     Returns y; with quantize (q, scale), scale float32 [...]; with a residual also s (rounded to x's dtype) behind them. The norm is taken of
-    the sum before that rounding. Differentiable once in x, weight and residual, through y and s; not with quantize."""
+    the sum before that rounding. Differentiable once in x, weight and residual, through y and s, backward (a dual
+    tensor of a forward derivative is refused); not with quantize."""
     assert impl in ['ref', 'cuda']
     assert isinstance(x, torch.Tensor) and x.ndim >= 1 and x.shape[-1] >= 1 and x.dtype in _rows.ROW_DTYPES
     assert eps >= 0
@@ -31,12 +32,11 @@ def rms_norm(x, weight=None, residual=None, eps=1e-8, quantize=False, impl='cuda
         assert weight.shape == x.shape[-1:] and weight.dtype == x.dtype and weight.device == x.device
     if residual is not None:
         assert residual.shape == x.shape and residual.dtype == x.dtype and residual.device == x.device
-    grad = _rows.wants_grad(x, weight, residual)
-    assert not (quantize and grad), '8-bit rows have no gradient'
+    assert not (quantize and _rows.wants_grad(x, weight, residual)), '8-bit rows have no gradient'
     if impl == 'ref' or not x.is_cuda:
         out = _rms_norm_ref(x, weight, residual, eps, quantize)
-    elif grad:
-        out = _RmsNorm.apply(x, weight, residual, eps)
+    elif _rows.watched(x, weight, residual):
+        out = _RmsNorm.apply(x, weight, residual, eps, quantize)
     else:
         y, scale, total, _, _ = _forward(x, weight, residual, eps, quantize, False)
         out = tuple(t for t in (y, scale, total) if t is not None)
@@ -51,13 +51,7 @@ def quantize_rows(x, impl='cuda'):
     assert not _rows.wants_grad(x), '8-bit rows have no gradient'
     if impl == 'ref' or not x.is_cuda:
         return _quantize_ref(x.float())
-    width = x.shape[-1]
-    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
-    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    x2 = _rows.rows_of(x, width)
-    if x2.shape[0]:
-        _rows.launch(x.device, 'lvg_quantize_rows', x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], width, _rows.row_stride(x2), _rows.type_code(x.dtype))
-    return q, scale
+    return _QuantizeRows.apply(x) if _rows.watched() else _quantize(x)
 
 
 def _quantize_ref(v):
@@ -102,13 +96,32 @@ def _forward(x, weight, residual, eps, quantize, keep):
     return y, scale, total, rstd, rest
 
 
+def _quantize(x):
+    width = x.shape[-1]
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    x2 = _rows.rows_of(x, width)
+    if x2.shape[0]:
+        _rows.launch(x.device, 'lvg_quantize_rows', x2.data_ptr(), q.data_ptr(), scale.data_ptr(), x2.shape[0], width, _rows.row_stride(x2), _rows.type_code(x.dtype))
+    return q, scale
+
+
+class _QuantizeRows(torch.autograd.Function):
+    """For calls that are watched (see _rows.watched); rows that ask for a gradient have been refused."""
+    @staticmethod
+    def forward(ctx, x):
+        return _quantize(x)
+
+
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        y, _, total, rstd, rest = _forward(x, weight, residual, eps, False, True)
+    def forward(ctx, x, weight, residual, eps, quantize):
+        keep = any(ctx.needs_input_grad) and not quantize
+        y, scale, total, rstd, rest = _forward(x, weight, residual, eps, quantize, keep)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if total is None else total, weight, rstd, rest)
-        return (y,) if total is None else (y, total)
+        if keep:
+            ctx.save_for_backward(x if total is None else total, weight, rstd, rest)
+        return tuple(t for t in (y, scale, total) if t is not None)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -137,4 +150,4 @@ class _RmsNorm(torch.autograd.Function):
             _rows.launch(dev, 'lvg_rms_norm_backward', dy2.data_ptr(), None if ds2 is None else ds2.data_ptr(), s2.data_ptr(), None if rest is None else rest.data_ptr(),
                          None if weight is None else weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), None if dw is None else dw.data_ptr(), None if work is None else work.data_ptr(), size, rows, width,
                          _rows.row_stride(dy2), 0 if ds2 is None else _rows.row_stride(ds2), _rows.row_stride(s2), code)
-        return dx if need_x else None, dw, dx if need_r else None, None
+        return dx if need_x else None, dw, dx if need_r else None, None, None

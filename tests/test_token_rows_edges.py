@@ -75,3 +75,71 @@ def test_norm_gradient_of_rows_far_from_one_gpu(shape, size, dtype):
     x, r = (x * size).to(dtype), (r * size).to(dtype)
     check_norm(x.clone(), w.to(dtype), r, eps=0.0, dy=dy.to(dtype))
     check_norm(x.clone(), None, None, eps=0.0, dy=dy.to(dtype))
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# Modes that watch tensors' operations.
+
+def every_operator(device):
+    """(name, function of one float tensor [6, 64], that tensor) for each operator's form without gradients."""
+    w, r, nw = rand(80, 64, seed=2, device=device, scale=0.125), rand(6, 80, seed=3, device=device), rand(64, seed=4, device=device)
+    return [('linear', lambda x: la.linear_act(x, w, residual=r, act='swish')),
+            ('gated', lambda x: gf.gated_ff(x, w)),
+            ('norm', lambda x: rn.rms_norm(x, nw)),
+            ('norm and sum', lambda x: rn.rms_norm(x, nw, residual=x)),
+            ('norm to 8 bits', lambda x: rn.rms_norm(x, nw, residual=x, quantize=True)),
+            ('8 bits', rn.quantize_rows)], rand(6, 64, seed=1, device=device)
+
+
+def test_forward_derivatives_of_the_plain_forms_cpu():
+    calls, x = every_operator('cpu')
+    with fwad.dual_level():
+        for name, call in calls[:4]:
+            out = call(fwad.make_dual(x, torch.ones_like(x)))
+            assert fwad.unpack_dual(out[0] if isinstance(out, tuple) else out).tangent is not None, name
+
+
+@pytest.mark.gpu
+def test_forward_derivatives_are_refused_gpu():
+    """The kernels have no forward derivative: a dual tensor is refused, never taken for its value alone."""
+    calls, x = every_operator('cuda')
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        for name, call in calls:
+            for grads in (True, False):
+                with torch.set_grad_enabled(grads), pytest.raises(NotImplementedError):
+                    call(dual)
+                    pytest.fail(name)
+        w = rand(80, 64, seed=2)
+        with pytest.raises(NotImplementedError):
+            la.linear_act(x, fwad.make_dual(w, torch.ones_like(w)))
+    q, s = rn.quantize_rows(x)
+    qw, sw = rn.quantize_rows(w)
+    with fwad.dual_level():
+        for op in (la.linear_act, gf.gated_ff):
+            with pytest.raises(NotImplementedError):
+                op(q, qw, x_scale=fwad.make_dual(s, torch.ones_like(s)), weight_scale=sw)
+    # calls without a dual tensor go on while one is about, with leaves under no_grad too
+    b, nw = rand(80, seed=5, dtype=BF16).requires_grad_(True), rand(64, seed=4).requires_grad_(True)
+    with torch.no_grad():
+        plain = [lambda: la.linear_act(q, qw, b, x_scale=s, weight_scale=sw), lambda: gf.gated_ff(q, qw, b, x_scale=s, weight_scale=sw),
+                 lambda: rn.rms_norm(x, nw, quantize=True)[1], lambda: rn.rms_norm(x, nw), lambda: gf.gated_ff(x, w.requires_grad_(True))]
+        want = [call() for call in plain]
+        with fwad.dual_level():
+            assert all(torch.equal(call(), t) for call, t in zip(plain, want))
+
+
+@pytest.mark.gpu
+def test_traced_calls_run_the_kernels_gpu():
+    calls, x = every_operator('cuda')
+    other = rand(6, 64, seed=9)
+    q, s = rn.quantize_rows(x)
+    qw, sw = rn.quantize_rows(rand(80, 64, seed=2))
+    calls.append(('8-bit linear', lambda x: la.linear_act(q, qw, x_scale=s * x[:, 0].abs(), weight_scale=sw)))
+    calls.append(('8-bit gated', lambda x: gf.gated_ff(q, qw, x_scale=s * x[:, 0].abs(), weight_scale=sw)))
+    for name, call in calls:
+        traced = torch.jit.trace(call, (x,), check_trace=False)
+        for t in (other, x):
+            got, want = traced(t), call(t)
+            for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+                assert same_bits(a.contiguous(), b.contiguous()), name
