@@ -537,7 +537,7 @@ int lvg_split32_stack(const float* x, void* out, int64_t pixels, int channels, i
  * element is itself times its row's scale. b, residual, slopes may be NULL.
  * slopes (16-byte aligned, lvg_linear_slope_bytes(...) bytes) receives what lvg_linear_backward multiplies gradients with: slope_kind 1: the derivatives
  * with respect to the sums, [rows, outer] (gated [rows, 2 outer]: the gate's and the up half's) in float32, or in bfloat16 with two more bits a
- * value behind them (-0 where the clamp cut: a gradient there is 0 even if dy is not finite); 2: one byte an element (0: clamped, or relu's lower
+ * value behind them (a mark where the clamp cut, or a gate's relu: a gradient there is 0 even if dy is not finite); 2: one byte an element (0: clamped, or relu's lower
  * side, 1: alpha, 2: one; linear, relu and lrelu only); 0: none.
  * work: lvg_linear_act_work(...) bytes, 16-byte aligned (0 bytes: NULL will do); nothing in it outlives the call.
  */

@@ -170,6 +170,11 @@ template <class O, bool GATED> __device__ __forceinline__ void prepare4(const Fi
     }
 }
 
+// In a derivative's place: no gradient passes here, whatever it is (what a clamp cut, a gate on relu's lower side). A pattern that no arithmetic
+// gives, a signalling NaN, and one that 18 bits hold: a derivative that has merely become zero, of either sign, still makes a NaN of an infinite gradient.
+constexpr uint32_t kCutBits = 0xffa54000u;
+__device__ __forceinline__ float cut_mark() { return __uint_as_float(kCutBits); }
+
 // A row's derivatives, `cols` for each of H halves: float32 or, for bfloat16, the upper 18 bits of the float32 (rounded; zeros, ones and what else
 // bfloat16 holds stay exact): 16 of them as an element of type S, the other two in bytes for four columns each.
 template <class O> struct Kept            { typedef float S;  static constexpr bool kBits = false; };
@@ -260,7 +265,7 @@ template <class O, bool GATED> __device__ __forceinline__ void finish4(const Fin
         for (int i = 0; i < 4; i++)
         {
             up[i] = a[i] * f.gain;              // dh/du
-            d[i] = d[i] * u[i] * f.gain;        // dh/dg
+            d[i] = f.act == LVG_ACT_RELU && v[i] <= 0.f ? cut_mark() : d[i] * u[i] * f.gain;        // dh/dg
             a[i] = up[i] * u[i];
         }
         if (want)
@@ -280,7 +285,7 @@ template <class O, bool GATED> __device__ __forceinline__ void finish4(const Fin
         if (f.clamp >= 0.f)
         {
             inside = !(fabsf(a[i]) >= f.clamp);         // (a NaN is inside: it stays one)
-            if (!inside) { a[i] = a[i] > 0.f ? f.clamp : -f.clamp; d[i] = -0.f; }     // (-0: nothing passes, see token_slope_kernel)
+            if (!inside) { a[i] = a[i] > 0.f ? f.clamp : -f.clamp; d[i] = cut_mark(); }
         }
         // 0: no gradient (cut, or relu's lower side), 1: alpha (lrelu's), 2: one
         code |= (uint32_t)(!inside || (f.act == LVG_ACT_RELU && v[i] <= 0.f) ? 0 : (f.act == LVG_ACT_LRELU && !(v[i] > 0.f)) ? 1 : 2) << (8 * i);

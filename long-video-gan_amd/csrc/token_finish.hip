@@ -134,8 +134,8 @@ __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
                     {
                         float s = row_load(d[h][i / kE].v[i % kE]);
                         if constexpr (Kept<T>::kBits) s = __uint_as_float(__float_as_uint(s) | (bits[h] >> (2 * i) & 3u) << 14);
-                        // (the clamp's -0 stops infinities and NaNs too; gated units have no clamp)
-                        v[i] = H == 1 && __float_as_uint(s) == 0x80000000u ? 0.f : v[i] * s;
+                        // (the mark stops infinities and NaNs too; nothing cuts a gated unit's up half)
+                        v[i] = h == 0 && __float_as_uint(s) == kCutBits ? 0.f : v[i] * s;
                     }
                     else if (p.kind == LVG_SLOPE_CODE) v[i] = c[i] == 2 ? v[i] : c[i] == 1 ? v[i] * p.alpha : 0.f;
                     v[i] *= p.gain;

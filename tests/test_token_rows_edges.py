@@ -78,6 +78,50 @@ def test_norm_gradient_of_rows_far_from_one_gpu(shape, size, dtype):
 
 
 # --------------------------------------------------------------------------------------------------------------------
+# Gradients that no derivative lets through, and those that one of zero does not stop.
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows', [5, 70, 300])
+def test_infinite_gradients_at_a_gates_lower_side_gpu(rows, dtype):
+    """relu's lower side passes no gradient to the gate, infinite or NaN ones neither. All sums are +-1 exactly."""
+    outer, inner = 72, 40
+    x, w = torch.zeros(rows, inner), torch.zeros(2 * outer, inner)
+    x[:, 0] = 1
+    w[:outer, 0] = torch.tensor([1.0, -1.0]).repeat(outer // 2)
+    w[outer:, 0] = 1
+    x, w, b = (t.to('cuda', dtype).requires_grad_() for t in (x, w, torch.zeros(2 * outer)))
+    dy = torch.ones(rows, outer, device='cuda', dtype=dtype)
+    dy[0, 1::2] = torch.inf
+    dy[-1, 1::2] = torch.nan
+    dw, db = torch.autograd.grad(gf.gated_ff(x, w, b, act='relu'), (w, b), dy)
+    want = torch.zeros(outer, dtype=dtype, device='cuda')
+    want[0::2] = rows
+    assert torch.equal(db[:outer], want) and torch.equal(dw[:outer, 0], want) and not dw[:outer, 1:].any()
+    # the up projection's derivative is act = 0 there, and 0 times infinity is no number
+    assert bool(db[outer + 1::2].isnan().all()) and torch.equal(db[outer::2], want[0::2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rows', [5, 70])
+def test_nan_gradients_pass_a_derivative_of_zero_gpu(rows, dtype):
+    """Where nothing is cut a NaN gradient stays one, also where the derivative has become zero (swish of -200)."""
+    outer, inner = 8, 40
+    x, w = torch.zeros(rows, inner), torch.zeros(2 * outer, inner)
+    x[:, 0] = 1
+    w[:outer, 0] = -200
+    w[outer:, 0] = 1
+    x, w = (t.to('cuda', dtype).requires_grad_() for t in (x, w))
+    for y in (la.linear_act(x, w[:outer], act='swish'), la.linear_act(x, w[:outer], act='swish', clamp=1.0), gf.gated_ff(x, w)):
+        dy = torch.ones_like(y)
+        dy[2, 3] = torch.nan
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
+        assert bool(dx[2, 0].isnan()) and bool(dw[3, 0].isnan())
+        assert bool(torch.isfinite(dx[3:]).all()) and bool(torch.isfinite(dw[4:outer]).all())
+
+
+# --------------------------------------------------------------------------------------------------------------------
 # Modes that watch tensors' operations.
 
 def every_operator(device):
