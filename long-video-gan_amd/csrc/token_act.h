@@ -141,18 +141,33 @@ template <class T> __device__ __forceinline__ void quad_past(T* p, const Quad<T>
     __builtin_nontemporal_store(w, reinterpret_cast<pair*>(p));
 }
 
+// The scale of a row of 8-bit values in two factors, the second a power of two: a sum (0, or 2^-18 to 2^48) times the first, times the column's scale,
+// times the second neither overflows nor underflows on the way where the result does not, as the product of the two scales can.
+struct RowScale
+{
+    float most, rest;
+    __device__ __forceinline__ RowScale() {}
+    __device__ __forceinline__ explicit RowScale(float s)
+    {
+        const float m = fabsf(s);
+        rest = m > 0x1p70f ? 0x1p64f : m < 0x1p-70f ? 0x1p-64f : 1.f;
+        most = m > 0x1p70f ? s * 0x1p-64f : m < 0x1p-70f ? s * 0x1p64f : s;
+    }
+    __device__ __forceinline__ float of(float v, float column) const { return v * most * column * rest; }
+};
+
 // Four neighbouring sums, row m, columns n .. n + 3 (those below cols): scales and bias. v: sums; gated: v of the gate half, u of the up half.
 template <class O, bool GATED> __device__ __forceinline__ void prepare4(const Finish& f, int64_t m, int64_t n, float* v, float* u)
 {
     const int64_t left = f.cols - n;
     if (f.qs)
     {
-        const float s = f.qs[m];
+        const RowScale s(f.qs[m]);
         #pragma unroll
         for (int i = 0; i < 4; i++) if (i < left)
         {
-            v[i] *= s * f.ps[n + i];
-            if (GATED) u[i] *= s * f.ps[f.cols + n + i];
+            v[i] = s.of(v[i], f.ps[n + i]);
+            if (GATED) u[i] = s.of(u[i], f.ps[f.cols + n + i]);
         }
     }
     if (f.bias)

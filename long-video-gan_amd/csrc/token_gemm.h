@@ -339,12 +339,12 @@ template <class O, bool GATED> struct Columns
     {
         if (f.qs)
         {
-            const float s = f.qs[m];
+            const RowScale s(f.qs[m]);
             #pragma unroll
             for (int i = 0; i < 4; i++)
             {
-                v[i] *= s * scale[i];
-                if (GATED) u[i] *= s * scaleUp[i];
+                v[i] = s.of(v[i], scale[i]);
+                if (GATED) u[i] = s.of(u[i], scaleUp[i]);
             }
         }
         #pragma unroll
@@ -613,11 +613,11 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
             for (int pass = 0; pass < MT; pass++)
             {
                 const int64_t m = rowOf(pass);
-                float scale[kTurns];
+                RowScale scale[kTurns];
                 if (sizeof(T) == 1)
                 {
                     #pragma unroll
-                    for (int t = 0; t < kTurns; t++) scale[t] = !kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f;
+                    for (int t = 0; t < kTurns; t++) scale[t] = RowScale(!kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f);
                 }
                 float v[kTurns][4], u[4];
                 #pragma unroll
@@ -627,7 +627,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                     #pragma unroll
                     for (int k = 0; k < 4; k++)
                     {
-                        if (sizeof(T) == 1) v[t][k] *= scale[t] * cols.scale[k];
+                        if (sizeof(T) == 1) v[t][k] = scale[t].of(v[t][k], cols.scale[k]);
                         v[t][k] = (v[t][k] + cols.bias[k]) * f.gain + (kRes ? row_load(res[t].v[k]) : 0.f);
                     }
                 }
@@ -655,11 +655,11 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
             for (int pass = 0; pass < MT; pass++)
             {
                 const int64_t m = rowOf(pass);
-                float scale[kTurns];
+                RowScale scale[kTurns];
                 if (sizeof(T) == 1)
                 {
                     #pragma unroll
-                    for (int t = 0; t < kTurns; t++) scale[t] = !kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f;
+                    for (int t = 0; t < kTurns; t++) scale[t] = RowScale(!kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f);
                 }
                 const Place<O, 2> at(f, m, n);
                 float v[kTurns][4], u[kTurns][4];
@@ -672,7 +672,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                     #pragma unroll
                     for (int k = 0; k < 4; k++)
                     {
-                        if (sizeof(T) == 1) { v[t][k] *= scale[t] * cols.scale[k]; u[t][k] *= scale[t] * cols.scaleUp[k]; }
+                        if (sizeof(T) == 1) { v[t][k] = scale[t].of(v[t][k], cols.scale[k]); u[t][k] = scale[t].of(u[t][k], cols.scaleUp[k]); }
                         v[t][k] += cols.bias[k];
                         u[t][k] += cols.biasUp[k];
                     }

@@ -56,6 +56,27 @@ def test_8bit_norm_rows_are_the_quotients_gpu(width, dtype):
     assert torch.equal(scale.cpu(), want_scale) and same_bits(q, want_q)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows', [5, 70])
+@pytest.mark.parametrize('sx,sw,value,count', [(1.15625 * 2.0 ** -72, 1.15625 * 2.0 ** -72, 256.0, 64), (2.0 ** 40, 2.0 ** 100, 2.0 ** -9, 1), (2.0 ** 110, 2.0 ** -60, 256.0, 64),
+                                               (2.0 ** -60, 2.0 ** 110, 256.0, 64)])
+def test_8bit_products_with_scales_far_from_one_gpu(rows, sx, sw, value, count):
+    """Results in range come out right where the product of the two scales, or of one of them and the sum, leaves float32's range; a sum of zero stays
+    zero. Sums are exact, the scales' two products rounded once each, and the result."""
+    inner, outer = 64, 48
+    x, w = torch.zeros(rows, inner), torch.zeros(2 * outer, inner)
+    x[:, :count], w[:, :count] = value, value
+    x[1] = 0
+    q, qw, s = x.to(E4M3).cuda(), w.to(E4M3).cuda(), torch.full((rows,), sx, device='cuda')
+    v = (x.double() @ w.double().t()).cuda()
+    g = v[:, :outer] * (sx * sw)
+    tr.assert_within(la.linear_act(q, qw[:outer], x_scale=s, weight_scale=torch.full((outer,), sw, device='cuda')), g, tr.rounded(g, 2 * tr.F32_ULP * g.abs(), BF16), 'y')
+    su = 2.0 ** -round(math.log2(float(v.max()) * sx))           # the up half is about one
+    h = gf.gated_ff(q, qw, act='linear', x_scale=s, weight_scale=torch.tensor([sw, su]).repeat_interleave(outer).cuda())
+    want = g * v[:, outer:] * (sx * su)
+    tr.assert_within(h, want, tr.rounded(want, 6 * tr.F32_ULP * want.abs(), BF16), 'h')
+
+
 # --------------------------------------------------------------------------------------------------------------------
 # Norm of rows far from one.
 
