@@ -9,7 +9,7 @@ import torch
 
 from . import _rows
 from .bias_act import _resolve, activation_funcs
-from .linear_act import SLOPE_SMOOTH, SLOPE_NONE, _backward, _check, _forward, _sums_ref
+from .linear_act import SLOPE_SMOOTH, SLOPE_NONE, _backward, _check, _forward, _sums_ref, keep_operands
 
 
 def gated_ff(x, weight, b=None, act='swish', alpha=None, gain=1.0, x_scale=None, weight_scale=None, out_dtype=None, impl='cuda'):
@@ -46,7 +46,7 @@ class _GatedFF(torch.autograd.Function):
     def forward(ctx, x, weight, b, x_scale, weight_scale, act, alpha, gain, out_dtype):
         kind = SLOPE_SMOOTH if any(ctx.needs_input_grad[:3]) and x_scale is None else SLOPE_NONE
         h, slopes = _forward(x, weight, b, None, act, alpha, gain, -1.0, x_scale, weight_scale, out_dtype, True, kind)
-        ctx.save_for_backward(x, weight, slopes)
+        keep_operands(ctx, x, weight, slopes)
         return h
 
     @staticmethod
@@ -54,4 +54,4 @@ class _GatedFF(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, slopes = ctx.saved_tensors
         # (the gain is in the slopes)
-        return _backward(dy, x, weight, slopes, SLOPE_SMOOTH, 2, 0.0, 1.0, *ctx.needs_input_grad[:3]) + (None,) * 6
+        return _backward(dy, x, weight, slopes, ctx.inner, SLOPE_SMOOTH, 2, 0.0, 1.0, *ctx.needs_input_grad[:3]) + (None,) * 6

@@ -133,22 +133,32 @@ def _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_sc
     return y, slopes
 
 
-def _backward(dy, x, weight, slopes, kind, halves, alpha, gain, need_x, need_w, need_b):
-    """Gradients of x, weight and b from dy [..., outer]; kind SLOPE_NONE: dy itself times the gain is the gradient of the sums."""
-    total, inner = weight.shape
-    outer = total // halves
-    x2, w2, dy2 = _rows.rows_of(x, inner), _rows.rows_of(weight, inner), _rows.rows_of(dy, outer)
-    rows, device = x2.shape[0], x.device
-    dx = x2.new_empty(x.shape) if need_x else None
-    dw = x2.new_empty((total, inner)) if need_w else None
-    db = x2.new_empty(total) if need_b else None
-    code = _rows.type_code(x.dtype)
+def keep_operands(ctx, x, weight, slopes):
+    """Saves what the gradients asked for read: the rows for the weight's, the weight for the rows'."""
+    need_x, need_w = ctx.needs_input_grad[:2]
+    ctx.save_for_backward(x if need_w else None, weight if need_x else None, slopes)
+    ctx.inner = weight.shape[1]
+
+
+def _backward(dy, x, weight, slopes, inner, kind, halves, alpha, gain, need_x, need_w, need_b):
+    """Gradients of x, weight and b from dy [..., outer]; kind SLOPE_NONE: dy itself times the gain is the gradient of the sums. x and weight as
+    keep_operands saves them."""
+    outer = dy.shape[-1]
+    total = outer * halves
+    dy2 = _rows.rows_of(dy, outer)
+    x2, w2 = (None if t is None else _rows.rows_of(t, inner) for t in (x, weight))
+    rows, device = dy2.shape[0], dy.device
+    dx = dy2.new_empty((*dy.shape[:-1], inner)) if need_x else None
+    dw = dy2.new_empty((total, inner)) if need_w else None
+    db = dy2.new_empty(total) if need_b else None
+    code = _rows.type_code(dy.dtype)
     size = _rows.query('lvg_linear_backward_work', rows, outer, inner, halves, kind, need_x + 2 * need_w + 4 * need_b, code)
     work = _rows.work_of(size, device)
-    _rows.launch(device, 'lvg_linear_backward', dy2.data_ptr(), None if slopes is None else slopes.data_ptr(), x2.data_ptr(), w2.data_ptr(),
+    _rows.launch(device, 'lvg_linear_backward', dy2.data_ptr(), None if slopes is None else slopes.data_ptr(),
+                 None if x2 is None else x2.data_ptr(), None if w2 is None else w2.data_ptr(),
                  None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
-                 None if work is None else work.data_ptr(), size, rows, outer, inner, _rows.row_stride(dy2), _rows.row_stride(x2), _rows.row_stride(w2),
-                 halves, kind, alpha, gain, code)
+                 None if work is None else work.data_ptr(), size, rows, outer, inner, _rows.row_stride(dy2),
+                 0 if x2 is None else _rows.row_stride(x2), 0 if w2 is None else _rows.row_stride(w2), halves, kind, alpha, gain, code)
     return dx, dw, db
 
 
@@ -158,17 +168,16 @@ class _LinearAct(torch.autograd.Function):
         needed = any(ctx.needs_input_grad[:3]) and x_scale is None         # (set for leaves under no_grad too)
         kind = slope_kind(act, False) if needed and (act != 'linear' or clamp >= 0) else SLOPE_NONE
         y, slopes = _forward(x, weight, b, residual, act, alpha, gain, clamp, x_scale, weight_scale, out_dtype, False, kind)
-        ctx.save_for_backward(x, weight, slopes)
-        ctx.args = kind, alpha, gain
+        keep_operands(ctx, x, weight, slopes)
+        ctx.args = kind, 1, alpha, gain
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, slopes = ctx.saved_tensors
-        kind, alpha, gain = ctx.args
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            dx, dw, db = _backward(dy, x, weight, slopes, kind, 1, alpha, gain, *need[:3])
+            dx, dw, db = _backward(dy, x, weight, slopes, ctx.inner, *ctx.args, *need[:3])
         return (dx, dw, db, dy if need[3] else None) + (None,) * 7

@@ -120,7 +120,8 @@ class _RmsNorm(torch.autograd.Function):
         y, scale, total, rstd, rest = _forward(x, weight, residual, eps, quantize, keep)
         ctx.set_materialize_grads(False)
         if keep:
-            ctx.save_for_backward(x if total is None else total, weight, rstd, rest)
+            need_weight = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
+            ctx.save_for_backward(x if total is None else total, weight if need_weight else None, rstd, rest)
         return tuple(t for t in (y, scale, total) if t is not None)
 
     @staticmethod
@@ -133,7 +134,7 @@ class _RmsNorm(torch.autograd.Function):
             # only the sum was used
             dx = ds
             if need_w:
-                dw = torch.zeros_like(weight)
+                dw = s.new_zeros(s.shape[-1])
         else:
             width = s.shape[-1]
             s2, dy2 = _rows.rows_of(s, width), _rows.rows_of(dy, width)

@@ -208,3 +208,38 @@ def test_traced_calls_run_the_kernels_gpu():
             got, want = traced(t), call(t)
             for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
                 assert same_bits(a.contiguous(), b.contiguous()), name
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# What a backward pass keeps, allocates and does.
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('op', ['linear', 'gated'])
+def test_operands_a_gradient_does_not_need_are_not_kept_gpu(op):
+    """A frozen weight's rows may change in place before the backward pass, rows without a gradient let the weight change."""
+    call = (lambda x, w: la.linear_act(x, w, act='swish')) if op == 'linear' else gf.gated_ff
+    base, w = rand(9, 64, seed=1).requires_grad_(True), rand(80, 64, seed=2, scale=0.125)
+    want, = torch.autograd.grad(call(base, w).sum(), base)
+    hidden = base * 1
+    y = call(hidden, w).sum()
+    with torch.no_grad():
+        hidden.mul_(2)
+    assert torch.equal(torch.autograd.grad(y, base)[0], want)
+    x, leaf = base.detach(), w.clone().requires_grad_(True)
+    want, = torch.autograd.grad(call(x, leaf).sum(), leaf)
+    y = call(x, leaf).sum()
+    with torch.no_grad():
+        leaf.zero_()
+    assert torch.equal(torch.autograd.grad(y, leaf)[0], want)
+
+
+@pytest.mark.gpu
+def test_a_norm_weight_may_change_before_its_own_gradient_gpu():
+    x, r, dy = (rand(9, 70, seed=i) for i in range(3))
+    w = rand(70, seed=3).requires_grad_(True)
+    want, = torch.autograd.grad(rn.rms_norm(x, w, residual=r)[0], w, dy)
+    y, total = rn.rms_norm(x, w, residual=r)
+    with torch.no_grad():
+        w.zero_()
+    assert torch.equal(torch.autograd.grad(y, w, dy, retain_graph=True)[0], want)
+    assert not torch.autograd.grad(total, w, dy)[0].any()
