@@ -7,6 +7,7 @@
 
 namespace {
 
+constexpr int64_t kGridBlocks = ((int64_t)1 << 24) - 1;  // workgroups of 256: a grid holds fewer than 2^32 threads
 constexpr float kE4m3Max = 448.f;
 constexpr float kScaleMin = 5.421010862427522e-20f;     // 2^-64: the scale of a row of zeros; its reciprocal is still finite
 

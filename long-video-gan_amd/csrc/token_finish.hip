@@ -197,7 +197,7 @@ bool size_ok(int64_t v) { return v >= 0 && v <= (int64_t)0x7fffffff; }
 
 int64_t part_pitch(int64_t cols, bool gated) { return (cols + 3) / 4 * 4 * (gated ? 2 : 1); }
 
-bool streams(int64_t rows, int form) { return rows <= kStreamRows && (form == LVG_TOKEN_FORWARD || form == LVG_TOKEN_GATED); }
+bool streams(int64_t rows, int64_t cols, int form) { return rows <= kStreamRows && cols <= kStreamCols && (form == LVG_TOKEN_FORWARD || form == LVG_TOKEN_GATED); }
 
 int layout_p(int form) { return form == LVG_TOKEN_ROW_GRAD || form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG; }
 int layout_q(int form) { return form == LVG_TOKEN_WEIGHT_GRAD ? DOWN : ALONG; }
@@ -213,44 +213,9 @@ int64_t pad16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 // one more launch (about 4 us). Operands whose sizes make their rows start at odd places are repacked first, in one launch for both, where the
 // product is long enough to pay for it (3000 x 1501 -> 3000, bfloat16: 62 us, and 79 us through registers; 1237 x 771 -> 515: 19 and 14 us).
 
-struct TokenPlan { int tile, splits; bool pack; };
+constexpr int64_t kPackBlocks = (int64_t)1 << 23;         // of a repacking launch, 4 KiB each: more than 32 GiB go through registers as they are
 
-TokenPlan token_plan(int64_t rows, int64_t cols, int64_t inner, int es, int form)
-{
-    static const struct { int bm, bn, held; double cycles[2], alone[2], more; } kTile[3] = {     // [float32]
-        {256, 256, 1, {3000., 15400.}, {3000., 15400.}, 22000.},
-        {128, 128, 2, {1000., 4000.}, {1450., 4100.}, 9000.},
-        {64, 128, 3, {700., 2050.}, {1150., 2100.}, 5000.}};
-    const bool gated = form == LVG_TOKEN_GATED, f32 = es == 4;
-    const int64_t steps = std::max<int64_t>(1, lvg_ceil_div(inner * es, 128)), width = cols * (gated ? 2 : 1);
-    const int64_t pBytes = layout_p(form) == ALONG ? inner * es : cols * es;       // of an operand's row
-    const bool odd = pBytes % 16 != 0 || (layout_q(form) == ALONG && form != LVG_TOKEN_ROW_GRAD && (inner * es) % 16 != 0);
-    TokenPlan best = {LVG_TILE_128, 1, false};
-    double least = 1e300;
-    for (int pack = 0; pack <= (odd ? 1 : 0); pack++)
-    {
-        // (bytes of the operands, read and written; bytes a cycle)
-        const double packing = pack ? 12000. + 2. * es * (double)inner * ((double)width + (layout_q(form) == ALONG && form != LVG_TOKEN_ROW_GRAD ? (double)rows : 0.)) / 1500. : 0.;
-        const double slow = odd && !pack ? (f32 ? 1.25 : 1.8) : 1.;
-        for (int t = 0; t < 3; t++)
-        {
-            if (es == 1 && odd && !pack && t == LVG_TILE_256) continue;
-            const int64_t tiles = lvg_ceil_div(rows, kTile[t].bm) * lvg_ceil_div(cols, kTile[t].bn / (gated ? 2 : 1));
-            for (int64_t splits = 1; splits <= 64 && splits <= steps; splits = splits < 4 ? splits + 1 : splits * 3 / 2)
-            {
-                if (splits > 1 && (tiles * splits > 2048 || (double)rows * (double)width > 1e9)) break;
-                const int64_t each = lvg_ceil_div(steps, splits);
-                if (lvg_ceil_div(steps, each) != splits) continue;
-                const int64_t perCu = lvg_ceil_div(tiles * splits, 256), rounds = lvg_ceil_div(perCu, kTile[t].held);
-                const double held = (double)std::min<int64_t>(perCu, kTile[t].held);
-                double cost = packing + (double)rounds * ((double)each * slow * std::max(kTile[t].alone[f32], held * kTile[t].cycles[f32]) + kTile[t].more);
-                if (splits > 1) cost += 8000. + (double)splits * (double)rows * (double)width * 8. / 3000.;
-                if (cost < least) { least = cost; best = {t, (int)splits, pack != 0}; }
-            }
-        }
-    }
-    return best;
-}
+struct TokenPlan { int tile, splits; bool pack; };
 
 // Workspace: the parts, then the repacked operands.
 struct Work { int64_t part, p, q, all; };
@@ -269,10 +234,49 @@ Work work_of(const TokenPlan& k, int64_t rows, int64_t cols, int64_t inner, int 
     return w;
 }
 
+TokenPlan token_plan(int64_t rows, int64_t cols, int64_t inner, int es, int form)
+{
+    static const struct { int bm, bn, held; double cycles[2], alone[2], more; } kTile[3] = {     // [float32]
+        {256, 256, 1, {3000., 15400.}, {3000., 15400.}, 22000.},
+        {128, 128, 2, {1000., 4000.}, {1450., 4100.}, 9000.},
+        {64, 128, 3, {700., 2050.}, {1150., 2100.}, 5000.}};
+    const bool gated = form == LVG_TOKEN_GATED, f32 = es == 4;
+    const int64_t steps = std::max<int64_t>(1, lvg_ceil_div(inner * es, 128)), width = cols * (gated ? 2 : 1);
+    const int64_t pBytes = layout_p(form) == ALONG ? inner * es : cols * es;       // of an operand's row
+    const Work copies = work_of({0, 1, true}, rows, cols, inner, es, form);
+    const bool odd = pBytes % 16 != 0 || (layout_q(form) == ALONG && form != LVG_TOKEN_ROW_GRAD && (inner * es) % 16 != 0);
+    TokenPlan best = {LVG_TILE_128, 1, false};
+    double least = 1e300;
+    for (int pack = 0; pack <= (odd && (copies.p + copies.q) / 4096 < kPackBlocks ? 1 : 0); pack++)
+    {
+        // (bytes of the operands, read and written; bytes a cycle)
+        const double packing = pack ? 12000. + 2. * es * (double)inner * ((double)width + (layout_q(form) == ALONG && form != LVG_TOKEN_ROW_GRAD ? (double)rows : 0.)) / 1500. : 0.;
+        const double slow = odd && !pack ? (f32 ? 1.25 : 1.8) : 1.;
+        for (int t = 0; t < 3; t++)
+        {
+            if (es == 1 && odd && !pack && t == LVG_TILE_256) continue;
+            const int64_t tiles = lvg_ceil_div(rows, kTile[t].bm) * lvg_ceil_div(cols, kTile[t].bn / (gated ? 2 : 1));
+            if (tiles > kGridBlocks) continue;
+            for (int64_t splits = 1; splits <= 64 && splits <= steps; splits = splits < 4 ? splits + 1 : splits * 3 / 2)
+            {
+                if (splits > 1 && (tiles * splits > 2048 || (double)rows * (double)width > 1e9)) break;
+                const int64_t each = lvg_ceil_div(steps, splits);
+                if (lvg_ceil_div(steps, each) != splits) continue;
+                const int64_t perCu = lvg_ceil_div(tiles * splits, 256), rounds = lvg_ceil_div(perCu, kTile[t].held);
+                const double held = (double)std::min<int64_t>(perCu, kTile[t].held);
+                double cost = packing + (double)rounds * ((double)each * slow * std::max(kTile[t].alone[f32], held * kTile[t].cycles[f32]) + kTile[t].more);
+                if (splits > 1) cost += 8000. + (double)splits * (double)rows * (double)width * 8. / 3000.;
+                if (cost < least) { least = cost; best = {t, (int)splits, pack != 0}; }
+            }
+        }
+    }
+    return best;
+}
+
 int64_t work_bytes(int64_t rows, int64_t cols, int64_t inner, int dtype, int form)
 {
     const int es = esize_of(dtype);
-    if (!streams(rows, form)) return work_of(token_plan(rows, cols, inner, es, form), rows, cols, inner, es, form).all;
+    if (!streams(rows, cols, form)) return work_of(token_plan(rows, cols, inner, es, form), rows, cols, inner, es, form).all;
     const bool gated = form == LVG_TOKEN_GATED;
     const int splits = token_stream_splits(rows, cols, inner * es, gated);
     return splits > 1 ? (int64_t)splits * rows * part_pitch(cols, gated) * 4 : 0;
@@ -314,7 +318,7 @@ int launch_pack(const PackArgs& p, int es, hipStream_t s)
 {
     const int64_t blocks = lvg_ceil_div(p.chunks[0] + p.chunks[1], 256);
     if (blocks == 0) return LVG_OK;
-    if (blocks > ((int64_t)1 << 23)) { lvg_set_error("token product: operands of %lld bytes to repack", (long long)blocks * 4096); return LVG_ERR_INVALID; }
+    if (blocks > kPackBlocks) { lvg_set_error("token product: operands of %lld bytes to repack", (long long)blocks * 4096); return LVG_ERR_INVALID; }
     const dim3 grid((unsigned)blocks), block(256);
     if (es == 4) hipLaunchKernelGGL(token_pack_kernel<float>, grid, block, 0, s, p);
     else if (es == 2) hipLaunchKernelGGL(token_pack_kernel<bf16_t>, grid, block, 0, s, p);
@@ -348,7 +352,7 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
     f.vec = cols % 4 == 0 && whole(f.bias, 0) && whole(f.residual, f.ldr) && whole(f.out, f.ldo) && (!f.slopes || lvg_aligned16(f.slopes));
     f.past = gated && os == 2 && rows * cols * os + slope_bytes(rows, cols, 2, f.slopeKind, out_dtype) >= (int64_t)64 << 20;
     int rc, splits;
-    if (streams(rows, form))
+    if (streams(rows, cols, form))
     {
         splits = token_stream_splits(rows, cols, a.inner * es, gated);
         a.part = splits > 1 ? static_cast<float*>(work) : nullptr;
@@ -397,7 +401,7 @@ int run_product(TokenArgs& a, int form, int dtype, int out_dtype, void* work, in
         a.splits = splits;
         a.tilesM = (int)lvg_ceil_div(rows, bm);
         a.tilesN = (int)lvg_ceil_div(cols, bn);
-        LVG_REQUIRE((int64_t)a.tilesM * a.tilesN <= ((int64_t)1 << 22), "%s: a result of %lld x %lld", what, (long long)rows, (long long)cols);
+        LVG_REQUIRE((int64_t)a.tilesM * a.tilesN <= kGridBlocks, "%s: a result of %lld x %lld", what, (long long)rows, (long long)cols);
         a.tiles = a.tilesM * a.tilesN;
         if (dtype == LVG_E4M3)      rc = token_launch_8bit(form, k.tile, direct, out_dtype, a, s);
         else if (dtype == LVG_F32)  rc = token_launch_f32(form, k.tile, direct, a, s);

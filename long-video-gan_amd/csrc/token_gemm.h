@@ -769,7 +769,7 @@ namespace {
 template <class T, class O, int PL, int QL, bool GATED> int token_launch_form(int tile, bool direct, const TokenArgs& a, hipStream_t s)
 {
     const int64_t blocks = (int64_t)a.tiles * a.splits;
-    if (blocks > ((int64_t)1 << 22)) { lvg_set_error("token product: %lld workgroups", (long long)blocks); return LVG_ERR_INVALID; }
+    if (blocks > kGridBlocks) { lvg_set_error("token product: %lld workgroups", (long long)blocks); return LVG_ERR_INVALID; }
     const dim3 grid((unsigned)blocks);
     #define LVG_TILE(ID, BM, BN, WR, WC, STAGED) if (tile == ID) { \
         if (direct) hipLaunchKernelGGL((token_gemm_kernel<T, O, BM, BN, WR, WC, PL, QL, GATED, true>), grid, dim3(WR * WC * 64), 0, s, a); \

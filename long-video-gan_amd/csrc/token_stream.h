@@ -17,6 +17,6 @@ struct StreamArgs
     Finish      fin;
 };
 
-constexpr int64_t kStreamRows = 32;
+constexpr int64_t kStreamRows = 32, kStreamCols = (int64_t)1 << 26;       // (16 columns a workgroup of 512 threads; wider results go through the tiles)
 int token_stream_splits(int64_t rows, int64_t cols, int64_t bytes, bool gated);
 int token_stream_launch(const StreamArgs& a, int dtype, int out_dtype, bool gated, int splits, hipStream_t s);

@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kWaves * 64) void token_stream_kernel(StreamArgs a)
 template <class T, class O> int launch(const StreamArgs& a, bool gated, int splits, hipStream_t s)
 {
     const bool many = a.rows > 16;
-    if (a.cols > ((int64_t)1 << 26)) { lvg_set_error("token product of a few rows: %lld columns", (long long)a.cols); return LVG_ERR_INVALID; }     // (threads of a grid)
+    if (a.cols > kStreamCols) { lvg_set_error("token product of a few rows: %lld columns", (long long)a.cols); return LVG_ERR_INVALID; }
     const dim3 grid((unsigned)lvg_ceil_div(a.cols, many && !gated ? 32 : 16), (unsigned)splits), block(kWaves * 64);
     if (!many)
     {

@@ -243,3 +243,33 @@ def test_a_norm_weight_may_change_before_its_own_gradient_gpu():
         w.zero_()
     assert torch.equal(torch.autograd.grad(y, w, dy, retain_graph=True)[0], want)
     assert not torch.autograd.grad(total, w, dy)[0].any()
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# Sizes near the limits of a launch.
+
+def test_repacking_is_not_planned_past_one_launch_cpu():
+    """Operands in odd rows that are too many for one repacking launch go through registers: the workspace holds no copy of them."""
+    assert _hip.lib().lvg_linear_act_work(1 << 22, 4096, 4097, 2, 0) < 1 << 32
+
+
+@pytest.mark.gpu
+def test_more_tiles_than_two_to_the_22nd_gpu():
+    rows = (1 << 28) + 64
+    x = torch.zeros(rows, 8, dtype=BF16, device='cuda')
+    x[-300:] = rand(300, 8, seed=1, dtype=BF16)
+    w = rand(1, 8, seed=2, dtype=BF16)
+    y = la.linear_act(x, w)
+    assert torch.equal(y[-300:], la.linear_act(x[-300:].clone(), w)) and not y[:-300].any()
+
+
+@pytest.mark.gpu
+def test_more_columns_than_two_to_the_26th_gpu():
+    outer = (1 << 26) + 24
+    x = rand(1, 8, seed=1, dtype=BF16)
+    w = torch.zeros(outer, 8, dtype=BF16, device='cuda')
+    w[-300:] = rand(300, 8, seed=2, dtype=BF16)
+    y = la.linear_act(x, w)
+    v, off = tr.sums64(x, w[-300:], None)
+    tr.assert_within(y[:, -300:], v, tr.rounded(v, off, BF16), 'y')
+    assert not y[:, :-300].any()
