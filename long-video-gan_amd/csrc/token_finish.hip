@@ -211,7 +211,10 @@ int64_t pad16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 // it has one; measured at 2.1 GHz on direct operands: 256 rows 1.45 us; 128: 0.48 and 0.7 us; 64: 0.33 and 0.57 us. Rows that go through registers
 // cost 1.8 times as much (float32: 1.25). Splitting the summed index fills the chip when there are few tiles, and costs the float32 parts' way to memory and back and
 // one more launch (about 4 us). Operands whose sizes make their rows start at odd places are repacked first, in one launch for both, where the
-// product is long enough to pay for it (3000 x 1501 -> 3000, bfloat16: 62 us, and 79 us through registers; 1237 x 771 -> 515: 19 and 14 us).
+// product is long enough to pay for it (3000 x 1501 -> 3000, bfloat16: 62 us, and 79 us through registers; 1237 x 771 -> 515: 19 and 14 us). A linear
+// layer's backward pass reads dy as it is: in odd rows it takes both operands through registers, where the repacked other one still pays, by aligned
+// loads and whole chunks at its edge (8192 x 1501 -> 3001, bfloat16, training step: 636 us, and 896 without; 1536 -> 3001: 535 us, counted as direct or
+// as slow steps).
 
 constexpr int64_t kPackBlocks = (int64_t)1 << 23;         // of a repacking launch, 4 KiB each: more than 32 GiB go through registers as they are
 
@@ -488,7 +491,7 @@ BackWork back_work(int64_t rows, int64_t outer, int64_t inner, int halves, int k
     BackWork w = {0, pad16(outer * halves * es) / es, 0, 0, 0, 0};
     if (rows == 0 || outer == 0) return w;
     w.slots = slope_slots(rows, outer, es);
-    if (kind != LVG_SLOPE_NONE) w.dz = rows * w.dzStride * es;
+    if (kind != LVG_SLOPE_NONE && (dx || dw)) w.dz = rows * w.dzStride * es;
     if (db) w.part = pad16((int64_t)w.slots * halves * outer * 4);
     if (dx && inner) w.product = work_bytes(rows, inner, outer * halves, dtype, LVG_TOKEN_ROW_GRAD);
     if (dw && inner) w.product = std::max(w.product, work_bytes(outer * halves, inner, rows, dtype, LVG_TOKEN_WEIGHT_GRAD));
@@ -524,13 +527,13 @@ extern "C" int lvg_linear_backward(const void* dy, const void* slopes, const voi
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool plain = slope_kind == LVG_SLOPE_NONE;               // dy times the gain is the gradient of the sums
     char* const mem = static_cast<char*>(work);
-    const void* dz = plain ? dy : mem;
+    const void* dz = plain ? dy : mem;                             // (the column sums alone leave none)
     const int64_t dzStride = plain ? dy_stride : k.dzStride, total = outer * halves;
     if (none && db && outer) row_column_sum(nullptr, db, 0, total, 0.f, dtype, s);
     if (!none && (!plain || db))
     {
         float* part = db ? reinterpret_cast<float*>(mem + k.dz) : nullptr;
-        SlopeArgs a = {dy, slopes, plain ? nullptr : mem, part, rows, outer, dy_stride, k.dzStride, slope_kind, slope_lanes(outer, esize_of(dtype)), alpha, plain ? 1.f : gain, false};
+        SlopeArgs a = {dy, slopes, k.dz ? mem : nullptr, part, rows, outer, dy_stride, k.dzStride, slope_kind, slope_lanes(outer, esize_of(dtype)), alpha, plain ? 1.f : gain, false};
         const int es = esize_of(dtype);
         a.once = rows * total * es >= (int64_t)64 << 20 && lvg_aligned16(dy) && (dy_stride * es) % 16 == 0 && (outer * es) % 16 == 0 && (!slopes || lvg_aligned16(slopes));
         const dim3 grid((unsigned)lvg_ceil_div(lvg_ceil_div(outer, 16 / esize_of(dtype)), a.lanes), (unsigned)k.slots), block(256);

@@ -245,6 +245,33 @@ def test_a_norm_weight_may_change_before_its_own_gradient_gpu():
     assert not torch.autograd.grad(total, w, dy)[0].any()
 
 
+def test_a_bias_gradient_alone_takes_its_column_sums_alone_cpu():
+    lib = _hip.lib()
+    for dtype, size in ((0, 4), (2, 2)):
+        rows, outer = 5000, 512
+        alone, with_dz = (lib.lvg_linear_backward_work(rows, outer, 64, 1, 1, grads, dtype) for grads in (4, 5))
+        assert 0 < alone < rows * outer * size <= with_dz
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ['linear', 'lrelu', 'swish'])
+def test_a_bias_gradient_alone_gpu(act):
+    x, w, b, dy = rand(700, 64, seed=1, dtype=BF16), rand(90, 64, seed=2, dtype=BF16, scale=0.125), rand(90, seed=3, dtype=BF16), rand(700, 90, seed=4, dtype=BF16)
+    b.requires_grad_(True)
+    alone, = torch.autograd.grad(la.linear_act(x, w, b, act=act), b, dy)
+    x.requires_grad_(True)
+    assert torch.equal(alone, torch.autograd.grad(la.linear_act(x, w, b, act=act), (b, x), dy)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [F16, BF16, F32])
+@pytest.mark.parametrize('size', [(1100, 771, 515), (1100, 768, 515), (1100, 771, 512), (3000, 1501, 1003), (40, 129, 9001)])
+def test_linear_layers_of_odd_widths_train_gpu(size, dtype):
+    from test_token_rows import check_linear
+    m, k, n = size
+    check_linear(rand(m, k, seed=1, dtype=dtype), rand(n, k, seed=2, dtype=dtype, scale=k ** -0.5), rand(n, seed=3, dtype=dtype), None, dy=rand(m, n, seed=5, dtype=dtype))
+
+
 # --------------------------------------------------------------------------------------------------------------------
 # Sizes near the limits of a launch.
 
