@@ -300,3 +300,14 @@ def test_more_columns_than_two_to_the_26th_gpu():
     v, off = tr.sums64(x, w[-300:], None)
     tr.assert_within(y[:, -300:], v, tr.rounded(v, off, BF16), 'y')
     assert not y[:, :-300].any()
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# Build.
+
+def test_objects_depend_on_the_makefile_cpu():
+    """Compiler flags stand in the Makefile: a change to it rebuilds every object."""
+    plan = subprocess.run(['make', '-n', '-W', 'Makefile', '-C', CSRC], capture_output=True, text=True, check=True).stdout
+    for name in os.listdir(CSRC):
+        if name.endswith('.hip'):
+            assert f'-c {name} ' in plan, name
