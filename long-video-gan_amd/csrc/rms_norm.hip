@@ -28,7 +28,7 @@ struct NormArgs
     float*       scale;        // [rows], 8-bit results
     int64_t      rows, width, ldx, ldr, ldy;
     float        eps;
-    bool         past, once;   // results are stored past the caches, operands loaded past them
+    bool         once;         // operands are loaded past the caches
 };
 
 struct NormBackArgs
@@ -43,7 +43,7 @@ struct NormBackArgs
     float*       part;         // [slots][width] or NULL
     float*       coef;         // [rows]: wide rows only
     int64_t      rows, width, lddy, ldds, lds;
-    bool         past, once;
+    bool         past, once;   // the result is stored past the caches, operands loaded past them
 };
 
 template <class T> __device__ __forceinline__ void store_rest(const NormArgs& p, int64_t row, int64_t at, const float* v)
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
                 const int64_t at = (int64_t)(j * 64 * W + t) * V;
                 #pragma unroll
                 for (int i = 0; i < V; i++) v[j][i] += row_load(rr[j].v[i]);
-                if (p.sum) store_row<T>(static_cast<T*>(p.sum) + row * p.width + at, p.width - at, v[j], p.past);
+                if (p.sum) store_row<T>(static_cast<T*>(p.sum) + row * p.width + at, p.width - at, v[j]);
                 store_rest<T>(p, row, at, v[j]);
             }
         }
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs p)
         for (int j = 0; j < NV; j++)
         {
             const int64_t at = (int64_t)(j * 64 * W + t) * V;
-            store_row<T>(y + at, p.width - at, v[j], p.past);
+            store_row<T>(y + at, p.width - at, v[j]);
         }
     }
 }
@@ -487,9 +487,11 @@ Plan plan(int64_t width, int dtype)
     return {0, 0};
 }
 
-// Matrices of 64 MB and more, in aligned rows, go past the caches, the operands (each value is read by one lane, once) and the results (the next
-// operator would not find them there): 16384 rows of 4096 bfloat16 with residual, forward and backward, 257 us with plain accesses, 224 us with
-// the stores past the caches, 193 us with the loads too; 8192 rows of 8192 to 8 bits 38.6 and 33.9 us.
+// Matrices of 64 MB and more, in aligned rows: operands are loaded past the caches, each value is read by one lane, once, and leaves them to what is
+// written and read next (four norms with residual in a row, inputs and results in turn, bfloat16: 16384 x 4096 325 us, and 384 with plain loads; 32768 x
+// 1024 166 and 169; a norm and the sum of its two results, 16384 x 4096: 137 and 159). Results of the forward pass are stored through the caches, where
+// the next operator finds part of them (past them: 357, 187 and 152 us). The gradient is stored past them: four such steps with gradients, 32768 x 1024,
+// 429 us, and 441 through the caches; 16384 x 4096 670 and 670; 65536 x 1024 807 and 822.
 constexpr int64_t kLarge = (int64_t)64 << 20;
 bool aligned_rows(const void* p, int64_t stride, int dtype) { return !p || (lvg_aligned16(p) && stride * esize(dtype) % 16 == 0); }
 bool large(int64_t rows, int64_t width, int arrays, int dtype) { return arrays * rows * width * esize(dtype) >= kLarge; }
@@ -566,8 +568,7 @@ extern "C" int lvg_rms_norm(const void* x, const void* residual, const void* wei
     LVG_REQUIRE(x && y && (!quantize || scale) && (!sum || residual) && (!rest || sum), "lvg_rms_norm: missing pointer");
     LVG_REQUIRE(x_stride >= 0 && residual_stride >= 0, "lvg_rms_norm: negative row stride");
     LVG_REQUIRE(eps >= 0.f, "lvg_rms_norm: eps must not be negative");
-    NormArgs a = {x, residual, weight, y, sum, dtype == LVG_F32 ? nullptr : static_cast<uint16_t*>(rest), rstd, scale, rows, width, x_stride, residual_stride, width, eps, false, false};
-    a.past = !quantize && large(rows, width, sum ? 2 : 1, dtype) && aligned_rows(y, width, dtype) && aligned_rows(sum, width, dtype);
+    NormArgs a = {x, residual, weight, y, sum, dtype == LVG_F32 ? nullptr : static_cast<uint16_t*>(rest), rstd, scale, rows, width, x_stride, residual_stride, width, eps, false};
     a.once = large(rows, width, residual ? 2 : 1, dtype) && aligned_rows(x, x_stride, dtype) && aligned_rows(residual, residual_stride, dtype);
     const Plan k = plan(width, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -583,7 +584,7 @@ extern "C" int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t r
     LVG_REQUIRE(rows_ok(rows, width), "lvg_quantize_rows: bad size (%lld rows of %lld)", (long long)rows, (long long)width);
     if (rows == 0) return LVG_OK;
     LVG_REQUIRE(x && q && scale && x_stride >= 0, "lvg_quantize_rows: missing pointer or negative row stride");
-    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f, false, large(rows, width, 1, dtype) && aligned_rows(x, x_stride, dtype)};
+    NormArgs a = {x, nullptr, nullptr, q, nullptr, nullptr, nullptr, scale, rows, width, x_stride, 0, width, 0.f, large(rows, width, 1, dtype) && aligned_rows(x, x_stride, dtype)};
     const Plan k = plan(width, dtype);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == LVG_F32) launch_norm<float, true, false>(a, k, s);
