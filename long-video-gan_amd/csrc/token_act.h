@@ -146,7 +146,6 @@ template <class T> __device__ __forceinline__ void quad_past(T* p, const Quad<T>
 struct RowScale
 {
     float most, rest;
-    __device__ __forceinline__ RowScale() {}
     __device__ __forceinline__ explicit RowScale(float s)
     {
         const float m = fabsf(s);
@@ -155,6 +154,9 @@ struct RowScale
     }
     __device__ __forceinline__ float of(float v, float column) const { return v * most * column * rest; }
 };
+
+// Scales whose product alone will do: it stays in range, and loses two bits at most where both are near 2^-64 (the scale of rows of zeros).
+__device__ __forceinline__ bool plain_scale(float s) { return fabsf(s) >= 0x1p-64f && fabsf(s) <= 0x1p60f; }
 
 // Four neighbouring sums, row m, columns n .. n + 3 (those below cols): scales and bias. v: sums; gated: v of the gate half, u of the up half.
 template <class O, bool GATED> __device__ __forceinline__ void prepare4(const Finish& f, int64_t m, int64_t n, float* v, float* u)

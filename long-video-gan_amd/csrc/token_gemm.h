@@ -437,6 +437,32 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
     {
         start(0, s0, lds);
         start(1, s0, lds);
+    }
+    // 8 bit: whether the plain product of two scales will do for all of this wave's results; asked for here, while the first step's tiles travel. The results'
+    // quick ways out take it then (norm, gated unit, 8-bit rows, projection, 8192 x 4096 -> 8192: two factors there cost 16 us of 786, this test 10 of 792).
+    bool plainScales = true;
+    if (sizeof(T) == 1 && !a.part)
+    {
+        constexpr int kCols = NT * 32 / (GATED ? 2 : 1);
+        bool plain = true;
+        #pragma unroll
+        for (int i = 0; i < MT * 32; i += 64)
+        {
+            const int64_t m = m0 + wr * MT * 32 + i + lane;
+            if (i + lane < MT * 32 && m < a.fin.rows) plain = plain && plain_scale(a.fin.qs[m]);
+        }
+        #pragma unroll
+        for (int i = 0; i < kCols; i += 64)
+        {
+            const int64_t n = n0 + wc * kCols + i + lane;
+            if (i + lane >= kCols || n >= a.fin.cols) continue;
+            plain = plain && plain_scale(a.fin.ps[n]);
+            if (GATED) plain = plain && plain_scale(a.fin.ps[a.fin.cols + n]);
+        }
+        plainScales = __all(plain);
+    }
+    if (s0 < s1)
+    {
         pl.end(lds);
         ql.end(lds + BN * 128);
         meet();
@@ -613,11 +639,11 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
             for (int pass = 0; pass < MT; pass++)
             {
                 const int64_t m = rowOf(pass);
-                RowScale scale[kTurns];
+                float scale[kTurns];
                 if (sizeof(T) == 1)
                 {
                     #pragma unroll
-                    for (int t = 0; t < kTurns; t++) scale[t] = RowScale(!kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f);
+                    for (int t = 0; t < kTurns; t++) scale[t] = !kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f;
                 }
                 float v[kTurns][4], u[4];
                 #pragma unroll
@@ -627,7 +653,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                     #pragma unroll
                     for (int k = 0; k < 4; k++)
                     {
-                        if (sizeof(T) == 1) v[t][k] = scale[t].of(v[t][k], cols.scale[k]);
+                        if (sizeof(T) == 1) v[t][k] *= scale[t] * cols.scale[k];
                         v[t][k] = (v[t][k] + cols.bias[k]) * f.gain + (kRes ? row_load(res[t].v[k]) : 0.f);
                     }
                 }
@@ -655,11 +681,11 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
             for (int pass = 0; pass < MT; pass++)
             {
                 const int64_t m = rowOf(pass);
-                RowScale scale[kTurns];
+                float scale[kTurns];
                 if (sizeof(T) == 1)
                 {
                     #pragma unroll
-                    for (int t = 0; t < kTurns; t++) scale[t] = RowScale(!kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f);
+                    for (int t = 0; t < kTurns; t++) scale[t] = !kEdge || m + t * kRows < f.rows ? f.qs[m + t * kRows] : 0.f;
                 }
                 const Place<O, 2> at(f, m, n);
                 float v[kTurns][4], u[kTurns][4];
@@ -672,7 +698,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
                     #pragma unroll
                     for (int k = 0; k < 4; k++)
                     {
-                        if (sizeof(T) == 1) { v[t][k] = scale[t].of(v[t][k], cols.scale[k]); u[t][k] = scale[t].of(u[t][k], cols.scaleUp[k]); }
+                        if (sizeof(T) == 1) { v[t][k] *= scale[t] * cols.scale[k]; u[t][k] *= scale[t] * cols.scaleUp[k]; }
                         v[t][k] += cols.bias[k];
                         u[t][k] += cols.biasUp[k];
                     }
@@ -705,21 +731,21 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
     };
     if constexpr (GATED)
     {
-        if (f.act == LVG_ACT_SWISH)
+        if (f.act == LVG_ACT_SWISH && plainScales)
         {
             if (f.slopeKind == LVG_SLOPE_SMOOTH) { if (inside) gate(Const<1>(), Const<0>()); else gate(Const<1>(), Const<1>()); }
             else                              { if (inside) gate(Const<0>(), Const<0>()); else gate(Const<0>(), Const<1>()); }
             return;
         }
     }
-    else if (f.act == LVG_ACT_LINEAR && f.slopeKind == LVG_SLOPE_NONE && f.clamp < 0.f)
+    else if (f.act == LVG_ACT_LINEAR && f.slopeKind == LVG_SLOPE_NONE && f.clamp < 0.f && plainScales)
     {
         if (f.residual) { if (inside) straight(Const<1>(), Const<0>()); else straight(Const<1>(), Const<1>()); }
         else            { if (inside) straight(Const<0>(), Const<0>()); else straight(Const<0>(), Const<1>()); }
         return;
     }
 
-    // Every other activation, one turn at a time; a turn's residual is asked for before the turn ahead of it stores.
+    // Every other activation (and scales far from one), one turn at a time; a turn's residual is asked for before the turn ahead of it stores.
     halves([&](auto h)
     {
         const int64_t n = colOf(h.value), left = f.cols - n;
