@@ -9,9 +9,14 @@
 // What a program otherwise spells as add, square, mean, rsqrt, two products, an absolute maximum and a cast: eight passes over the rows where
 // one has to read x and residual and write s and y. The gradient reads the sum as it was stored, rounded; two bits a value that the forward pass
 // keeps beside it (a third of the rounding's half step up, down, or neither) bring it three times closer to what the norm was taken of, for 3 % of
-// the traffic: without them the weight's gradient is 1.5 times as far from the exact one as its own rounding makes it. One row is held in the registers of one wave (up to 8 vectors a lane) or of a workgroup of
-// four, so each value is read once and written once; the sums are float32 and their order is fixed. Rows of more than 4 x 64 x 8 vectors take
-// two passes over the row, the second of which finds it in L2.
+// the traffic: without them the weight's gradient is 1.5 times as far from the exact one as its own rounding makes it. The sums are float32 and
+// their order is fixed.
+//
+// A row is held in the registers of one wave (up to 2 vectors a lane) or of four (up to 8: 16384 values of 16 bits, 8192 of float32), so each value is
+// read once and written once. Wider rows are read again, from L2 where they fit it: twice by the plain norm and by quantisation, three times by the norm
+// to 8 bits (mean, maximum, result). The gradient keeps three vectors of a row and of the next one: one wave up to one vector a lane, then four, then
+// eight with up to two (8192 values of 16 bits; float32 four, 8192 too); of wider rows a first pass takes the coefficient, a second one
+// the columns (4096 rows of 16384 bfloat16 with residual, both directions: 467 us, 1.1 GB at 2.3 TB/s, where 8192 rows of 8192 take 203).
 #include "row_common.h"
 
 namespace {
@@ -277,13 +282,13 @@ __global__ __launch_bounds__(256) void rms_norm_wide_kernel(NormArgs p)
 }
 
 // Gradient: a workgroup takes rows blockIdx.x, + gridDim.x, ... (W == 1: its four waves a row each) and keeps the weight's gradient of its
-// rows in registers; the four waves' sums meet in LDS in wave order and go to part[blockIdx.x][width]. The next row's three vectors are asked
-// for before this one's are used (NV <= 4: they fit the registers), so that memory does not wait for the row's reduction.
+// rows in registers; they go to part[blockIdx.x][width] (W == 1: the four waves' sums meet in LDS in wave order). The next row's three vectors
+// are asked for before this one's are used, so that memory does not wait for the row's reduction.
 template <class T, int W, int NV>
 __global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormBackArgs p)
 {
     constexpr int V = Elem<T>::kVec;
-    constexpr bool kAhead = NV <= 4;
+    static_assert(NV <= 4 && (W != 1 || NV == 1), "two rows fit the registers; one wave a row takes one vector a lane");
     __shared__ float sums[2][W == 1 ? 4 : W];
     __shared__ float cols[W == 1 ? 64 * V : 1];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -295,7 +300,7 @@ __global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormB
         const int64_t at = (int64_t)(j * 64 * W + t) * V;
         #pragma unroll
         for (int i = 0; i < V; i++) { dw[j][i] = 0.f; w[j][i] = 1.f; }
-        if (kAhead && p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w[j]);
+        if (p.weight) load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w[j]);
     }
     struct Row { RawRow<T> g[NV], s[NV], d[NV]; uint32_t rest[NV]; float r; };
     auto load = [&](Row& x, int64_t row)
@@ -327,17 +332,12 @@ __global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormB
     if (row < p.rows) load(now, row);
     for (; row < p.rows; row += step, turn ^= 1)
     {
-        if (kAhead && row + step < p.rows) load(next, row + step);
+        if (row + step < p.rows) load(next, row + step);
         const float r = now.r;
         float dot = 0.f;
         #pragma unroll
         for (int j = 0; j < NV; j++)
         {
-            if (!kAhead && p.weight)
-            {
-                const int64_t at = (int64_t)(j * 64 * W + t) * V;
-                load_row<T>(static_cast<const T*>(p.weight) + at, p.width - at, w[j]);
-            }
             #pragma unroll
             for (int i = 0; i < V; i++)
             {
@@ -361,35 +361,30 @@ __global__ __launch_bounds__(W == 8 ? 512 : 256) void rms_norm_back_kernel(NormB
             }
             store_row<T>(static_cast<T*>(p.dx) + row * p.width + at, p.width - at, v, p.past);
         }
-        if (kAhead) now = next;
-        else if (row + step < p.rows) load(now, row + step);
+        now = next;
     }
     if (!p.part) return;
     float* out = p.part + (int64_t)blockIdx.x * p.width;
+    if (W == 1)
+    {
+        for (int k = 0; k < 4; k++)         // the waves add in turn
+        {
+            if (wave == k)
+            {
+                #pragma unroll
+                for (int i = 0; i < V; i++) cols[lane * V + i] = k == 0 ? dw[0][i] : cols[lane * V + i] + dw[0][i];
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < 64 * V; i += 256) if (i < p.width) out[i] = cols[i];
+        return;
+    }
     #pragma unroll
     for (int j = 0; j < NV; j++)
     {
         const int64_t at = (int64_t)(j * 64 * W + t) * V;
-        if (W == 1)
-        {
-            for (int k = 0; k < 4; k++)         // the waves add in turn
-            {
-                if (wave == k)
-                {
-                    #pragma unroll
-                    for (int i = 0; i < V; i++) cols[lane * V + i] = k == 0 ? dw[j][i] : cols[lane * V + i] + dw[j][i];
-                }
-                __syncthreads();
-            }
-            for (int i = threadIdx.x; i < 64 * V; i += 256)
-                if ((int64_t)j * 64 * V + i < p.width) out[(int64_t)j * 64 * V + i] = cols[i];
-            __syncthreads();
-        }
-        else
-        {
-            #pragma unroll
-            for (int i = 0; i < V; i++) if (at + i < p.width) out[at + i] = dw[j][i];
-        }
+        #pragma unroll
+        for (int i = 0; i < V; i++) if (at + i < p.width) out[at + i] = dw[j][i];
     }
 }
 

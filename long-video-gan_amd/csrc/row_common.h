@@ -88,9 +88,9 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
     return (uint32_t)w;
 }
 
-// Two bits beside a rounded value: what rounding v to T left, in units of two thirds of half a step: -1, 0 or 1 (+ 1), a third of it at most is lost. A half step is 2^(exponent - 8) (bfloat16) or - 11 (float16).
-// A half step is 2^(exponent - 11) of float16; bfloat16 is the upper half of a float32, a half step 0x8000 of its lower half (zeros, infinities and
-// NaNs stay what they are: nothing is left of them, or it stays within their patterns).
+// Two bits beside a rounded value: what rounding v to T left, in units of two thirds of half a step: -1, 0 or 1 (+ 1), a third of it at most is lost.
+// A half step is 2^(exponent - 11) of float16 (its subnormals' is larger: theirs stay within the half step itself); bfloat16 is the upper half of a
+// float32, a half step 0x8000 of its lower half (zeros, infinities and NaNs stay what they are: nothing is left of them, or it stays within their patterns).
 __device__ __forceinline__ float half_step(float rounded) { return __uint_as_float(__float_as_uint(rounded) & 0x7f800000u) * 0.00048828125f; }
 template <class T> __device__ __forceinline__ uint32_t rest_code(float v)
 {

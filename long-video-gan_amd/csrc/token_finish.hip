@@ -68,7 +68,7 @@ struct SlopeArgs
 
 // A thread owns one vector of columns (gated: of both halves, dy is read once) and walks down its rows. One row at a time: several rows' loads ahead of
 // their use cost more waves than they gain (8192 x 2 x 8192 bfloat16: 314 us with four rows, 172 with one or two; 156 with loads and stores past the
-// caches, 4.5 TB/s).
+// caches, 4.5 TB/s, and the training step with its products 1594 -> 1553 us; as part of a block's step no difference).
 template <class T, int H>
 __global__ __launch_bounds__(256) void token_slope_kernel(SlopeArgs p)
 {

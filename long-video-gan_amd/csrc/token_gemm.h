@@ -473,7 +473,7 @@ __global__ __launch_bounds__(WR * WC * 64) void token_gemm_kernel(TokenArgs a)
     if (DIRECT)
     {
         // Steps whose second next one is whole: no branches. The sends for a step lie between the products of the group behind the barrier that
-        // frees its buffer and of the group after that, one for two products: one for each costs 16-bit products 6 % (8192^3: 805 -> 893 us). The
+        // frees its buffer and of the group after that, one for two products: one for each costs 16-bit products 11 % (8192^3: 805 -> 893 us). The
         // 8-bit step has two groups of products twice as long, all its sends lie in the first of them and have a whole step to arrive (8192 x 4096
         // -> 4096: 133 -> 121 us).
         auto spread = [&](int k, int half, int step, uint32_t pt)
