@@ -552,7 +552,7 @@ int lvg_linear_act(const void* x, const void* w, const void* b, const void* resi
  * Gradients of lvg_linear_act from dy [rows, outer] and the slopes it left (halves: 1, or 2 for a gated unit; w has halves * outer rows):
  *   dz = dy * slopes * gain  (slope_kind 0: dy * gain; 2: alpha stands for code 1),
  *   dx [rows, inner] = dz . w,   dw [halves * outer, inner] = dz^T . x,   db [halves * outer] = column sums of dz.
- * dx, dw, db are dense and have type dtype; those that are NULL are not computed. A gated unit's slopes hold its gain: pass gain 1.
+ * dx, dw, db are dense and have type dtype; those that are NULL are not computed; w may be NULL without dx, x without dw. A gated unit's slopes hold its gain: pass gain 1.
  * work: lvg_linear_backward_work(...) bytes, 16-byte aligned; grads: 1 (dx) | 2 (dw) | 4 (db) of those asked for.
  */
 int64_t lvg_linear_backward_work(int64_t rows, int64_t outer, int64_t inner, int halves, int slope_kind, int grads, int dtype);
@@ -580,7 +580,7 @@ int lvg_rms_norm_backward(const void* dy, const void* dsum, const void* s, const
                           void* work, int64_t work_size, int64_t rows, int64_t width, int64_t dy_stride, int64_t dsum_stride, int64_t s_stride,
                           int dtype, void* stream);
 
-/* q [rows, width] e4m3 = x / scale, scale [rows] = max |x| of the row / 448 (2^-64 at least). q is dense. */
+/* q [rows, width] e4m3 = x / scale (the float32 quotient, rounded), scale [rows] = max |x| of the row / 448 (2^-64 at least). q is dense. */
 int lvg_quantize_rows(const void* x, void* q, float* scale, int64_t rows, int64_t width, int64_t x_stride, int dtype, void* stream);
 
 #ifdef __cplusplus

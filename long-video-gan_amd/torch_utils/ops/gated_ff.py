@@ -23,7 +23,8 @@ def gated_ff(x, weight, b=None, act='swish', alpha=None, gain=1.0, x_scale=None,
         gain:         scale of the result (1: unlike in `bias_act`, no activation brings its own).
         x_scale, weight_scale, out_dtype, impl: as in `linear_act`; weight_scale is [2 * outer].
 
-    Returns [..., outer]. Differentiable once in x, weight and b (not with 8-bit operands). Sums are float32; the result is rounded once."""
+    Returns [..., outer]. Differentiable once in x, weight and b (not with 8-bit operands), backward; a dual tensor of a forward derivative is
+    refused. Sums are float32; the result is rounded once."""
     assert impl in ['ref', 'cuda']
     out_dtype = _check(x, weight, b, x_scale, weight_scale, out_dtype, halves=2)
     assert act in activation_funcs

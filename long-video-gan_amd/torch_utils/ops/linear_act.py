@@ -25,7 +25,8 @@ def linear_act(x, weight, b=None, residual=None, act='linear', alpha=None, gain=
         weight:       [outer, inner] in x's dtype.
         b:            [outer] in the result's dtype, or None.
         residual:     [..., outer] in the result's dtype, added last, or None.
-        act:          key of `bias_act.activation_funcs`; alpha, gain, clamp as in `bias_act` (None = the activation's default / no clamp).
+        act:          key of `bias_act.activation_funcs`; alpha, gain, clamp as in `bias_act` (None = the activation's default / no clamp). As in its
+                      kernel, a value that lies on the clamp exactly passes no gradient (the plain form, torch.clamp, passes it).
         x_scale:      8-bit x only: float32 [...], the value of an element is itself times its row's scale.
         weight_scale: 8-bit x only: float32 [outer], likewise for the rows of the weight.
         out_dtype:    dtype of the result: x's, or for 8-bit x float16 or bfloat16 (default bfloat16).
